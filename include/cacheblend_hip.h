@@ -87,6 +87,47 @@ int cbk_paged_scatter(const void* in_k_dev, const void* in_v_dev, int64_t in_tok
                       int32_t* bad_slots_dev, cbk_stream_t stream);
 
 /*
+ * Append: the keys and values [num_tokens, heads, head_dim] of a batch into
+ * the pages at slots_dev, the keys -- and, into query_out, the queries
+ * [num_tokens, q_heads, head_dim] (q_heads 0: none) -- rotated to positions_dev
+ * on the way (NULL: no rotation). Row p of cos_sin is rotary_dim / 2 cosines,
+ * then as many sines; dims past rotary_dim are copied. Pairs of dims lie
+ * rotary_dim / 2 apart (neox) or side by side; (x, y) becomes (x c - y s,
+ * y c + x s), products and differences rounded to float32, then once to the
+ * type. key_out (NULL: none) receives the rotated keys as well. Strides in
+ * ELEMENTS of the inputs' dtype; the outputs may be the inputs themselves, no
+ * other overlap. head_dim <= 512.
+ * int4 != 0: the pages hold 4-bit rows, per head head_dim / 2 bytes of codes
+ * (dim 2i in the low half of byte i), then per 32 dims a bf16 step and a bf16
+ * offset: value = offset + step * code (head_dim a multiple of 32, row_bytes =
+ * heads * head_dim / 32 * 20, 4-byte aligned pages). offset: the 32 values'
+ * lowest, rounded down; step: a 15th of highest - offset, rounded up; a group
+ * with a value that is not finite is NaN. Keys are rotated and both are
+ * rounded to codes in 64 bits.
+ * Tokens with a slot or position out of range leave the pages as they are; a
+ * position out of range gives zero rows in query_out and key_out. Slots of
+ * tokens that are written must differ.
+ */
+int cbk_paged_append(const cbk_kv_desc* kv, const int64_t* slots_dev, int64_t num_tokens, const void* key_dev,
+                     int64_t key_token_stride, int64_t key_head_stride, const void* value_dev,
+                     int64_t value_token_stride, int64_t value_head_stride, const void* query_dev,
+                     int64_t query_token_stride, int64_t query_head_stride, int64_t q_heads, int64_t heads,
+                     int64_t head_dim, int32_t dtype, int32_t int4, const int64_t* positions_dev,
+                     const void* cos_sin_dev, int64_t cos_sin_row_stride_elems, int64_t cos_sin_rows,
+                     int32_t cos_sin_dtype, int64_t rotary_dim, int32_t neox, void* query_out_dev,
+                     int64_t query_out_token_stride, int64_t query_out_head_stride, void* key_out_dev,
+                     int64_t key_out_token_stride, int64_t key_out_head_stride, cbk_stream_t stream);
+
+/*
+ * Gather of 4-bit pages: out_{k,v}[t] = the values, in `dtype`, of the rows at
+ * slot t; [num_tokens, heads, head_dim] each, 16-byte aligned rows. A slot out
+ * of range gives a zero row.
+ */
+int cbk_paged_gather_int4(const cbk_kv_desc* kv, const int64_t* slots_dev, int64_t num_tokens, int64_t heads,
+                          int64_t head_dim, int32_t dtype, void* out_k_dev, void* out_v_dev, int64_t out_token_stride,
+                          cbk_stream_t stream);
+
+/*
  * Multi-layer gather in one launch per 64 layers: for layer l,
  * out + l*out_layer_stride + c*out_plane_stride + t*out_token_stride
  * receives plane c of kv[l] at slot t. All layers share the geometry of

@@ -61,6 +61,16 @@ _SIGNATURES = {
         ctypes.c_int,
         [c_vp, c_vp, c_i64, ctypes.POINTER(KVDesc), c_vp, c_i64, c_vp, c_vp],
     ),
+    "cbk_paged_append": (
+        ctypes.c_int,
+        [ctypes.POINTER(KVDesc), c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
+         c_i64, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_i64, c_i64, c_i32, c_i64, c_i32, c_vp, c_i64, c_i64,
+         c_vp, c_i64, c_i64, c_vp],
+    ),
+    "cbk_paged_gather_int4": (
+        ctypes.c_int,
+        [ctypes.POINTER(KVDesc), c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp],
+    ),
     "cbk_paged_gather_layers": (
         ctypes.c_int,
         [ctypes.POINTER(KVDesc), c_i32, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp],
@@ -227,6 +237,14 @@ def check(rc: int, what: str) -> None:
 def stream_handle(device: torch.device) -> int:
     """hipStream_t of torch's current stream on ``device``."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device, fn, *args) -> int:
+    """``fn(*args)`` with ``device`` current: a launch takes its stream's device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def require_device(tensor: torch.Tensor, what: str) -> None:

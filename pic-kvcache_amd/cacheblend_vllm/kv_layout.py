@@ -204,6 +204,208 @@ def scatter_paged_kv(
     _native.check(rc, "scatter_paged_kv")
 
 
+INT4_GROUP = 32  # dims of a 4-bit row that share a step and an offset
+
+
+def int4_row_bytes(head_size: int) -> int:
+    """Bytes of one head's row in 4-bit pages: ``head_size / 2`` of codes (dim
+    ``2i`` in the low half of byte ``i``), then a bf16 step and a bf16 offset
+    for every 32 dims; a dim's value is ``offset + step * code``. A 4-bit layer
+    is an ordinary paged layer of ``uint8`` with rows ``[kv_heads,
+    int4_row_bytes(head_size)]``, so everything here that moves rows moves it."""
+    if head_size <= 0 or head_size % INT4_GROUP:
+        raise ValueError(f"4-bit rows need a head size that is a multiple of {INT4_GROUP}, not {head_size}")
+    return head_size // INT4_GROUP * (INT4_GROUP // 2 + 4)
+
+
+def int4_geometry(plane: torch.Tensor) -> tuple[int, int]:
+    """(kv_heads, head_size) of a 4-bit plane ``[num_blocks, block_size, kv_heads, bytes]``."""
+    per_group = INT4_GROUP // 2 + 4
+    if plane.dtype != torch.uint8 or plane.ndim != 4 or plane.shape[3] == 0 or plane.shape[3] % per_group:
+        raise ValueError(
+            f"4-bit pages must be uint8 [num_blocks, block_size, kv_heads, a multiple of {per_group}], "
+            f"got {plane.dtype} {tuple(plane.shape)}"
+        )
+    return plane.shape[2], plane.shape[3] // per_group * INT4_GROUP
+
+
+def _check_rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, out: bool = False) -> None:
+    """[tokens, heads, head_size] with contiguous dims, of ``like``'s type and device; rows apart if written."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must match the keys' dtype and device")
+    if t.stride(2) != 1 and shape[2] > 1:
+        raise ValueError(f"{name} rows must hold contiguous dims")
+    if out and ((shape[1] > 1 and t.stride(1) < shape[2]) or
+                (shape[0] > 1 and t.stride(0) < (shape[1] - 1) * t.stride(1) + shape[2])):
+        raise ValueError(f"{name} rows must not overlap")
+
+
+def append_paged_kv(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    kv_layer: KVLayer,
+    slot_mapping: torch.Tensor,
+    block_size: int,
+    positions: torch.Tensor | None = None,
+    rotary_emb=None,
+    query: torch.Tensor | None = None,
+    query_out: torch.Tensor | None = None,
+    key_out: torch.Tensor | None = None,
+) -> torch.Tensor | None:
+    """Append a batch's ``key`` and ``value`` ``[tokens, kv_heads, head_size]`` to a
+    paged layer in place, the keys rotated to ``positions`` on the way: a
+    prefill's or a decode step's rotation and ``scatter_paged_kv`` in one launch
+    (cbk_paged_append).
+
+    ``rotary_emb`` (``head_size``, ``is_neox_style``, ``cos_sin_cache`` ``[rows,
+    rotary_dim]``, optionally ``rotary_dim``) and ``positions`` come together, or
+    neither, and the keys go in as they are. ``query`` ``[tokens, q_heads,
+    head_size]`` is rotated beside them and returned, in ``query_out`` if given;
+    ``key_out`` receives the rotated keys as well (for ``prompt_attention``).
+    The outputs may be the inputs themselves, but must not overlap otherwise.
+    Head sizes up to 512, any strides with contiguous dims.
+
+    The layer has the inputs' type, or is a 4-bit layer (:func:`int4_row_bytes`):
+    per 32 dims the offset is the lowest value, rounded down, and the step a
+    15th of the rest, rounded up; 32 dims with an infinity or a NaN are NaN.
+
+    Slots and positions on the host are checked (``IndexError``). On the device
+    they are not read back: a token with a slot out of range (-1, padding) or a
+    position outside the table leaves the pages alone, and the latter gives zero
+    rows in the outputs. The slots that are written must differ from each other:
+    of two tokens with one slot, either's values may stay.
+    """
+    desc, plane = kv_desc(kv_layer, block_size)
+    if key.dim() != 3:
+        raise ValueError("key must be [tokens, kv_heads, head_size]")
+    if key.dtype not in _native.DTYPE_CODES:
+        raise ValueError(f"dtype {key.dtype} is not supported")
+    if key.device != plane.device:
+        raise ValueError(f"key is on {key.device}, the cache on {plane.device}")
+    shape = tuple(key.shape)
+    tokens, heads, head_size = shape
+    _check_rows(key, "key", shape, key)
+    _check_rows(value, "value", shape, key)
+    int4 = plane.dtype == torch.uint8
+    if int4:
+        if int4_geometry(plane) != (heads, head_size):
+            raise ValueError(f"4-bit pages of {tuple(plane.shape[2:])} bytes a token do not hold rows of {shape[1:]}")
+    elif plane.dtype != key.dtype or tuple(plane.shape[2:]) != shape[1:]:
+        raise ValueError(
+            f"the pages hold {plane.dtype} rows {tuple(plane.shape[2:])}, the keys are {key.dtype} {shape[1:]}"
+        )
+    q_heads = 0
+    if query is not None:
+        if query.dim() != 3:
+            raise ValueError("query must be [tokens, q_heads, head_size]")
+        q_heads = query.shape[1]
+        q_shape = (tokens, q_heads, head_size)
+        _check_rows(query, "query", q_shape, key)
+        if query_out is None:
+            query_out = torch.empty(q_shape, dtype=query.dtype, device=query.device)
+        else:
+            _check_rows(query_out, "query_out", q_shape, key, out=True)
+    elif query_out is not None:
+        raise ValueError("query_out needs a query")
+    if key_out is not None:
+        _check_rows(key_out, "key_out", shape, key, out=True)
+    if slot_mapping.numel() != tokens:
+        raise ValueError(f"{slot_mapping.numel()} slots for {tokens} tokens")
+    if (positions is None) != (rotary_emb is None):
+        raise ValueError("positions and rotary_emb come together")
+    table, rotary_dim, neox = None, 0, True
+    if rotary_emb is not None:
+        table = getattr(rotary_emb, "cos_sin_cache", None)
+        if not isinstance(table, torch.Tensor) or table.ndim != 2:
+            raise ValueError("rotation requires a two-dimensional RoPE cos_sin_cache")
+        rope_size, neox = int(rotary_emb.head_size), bool(rotary_emb.is_neox_style)
+        rotary_dim = int(getattr(rotary_emb, "rotary_dim", rope_size))
+        if rope_size != head_size or rotary_dim <= 0 or rotary_dim % 2 or rotary_dim > head_size:
+            raise ValueError(f"rotary_dim {rotary_dim} of head_size {rope_size} does not fit keys of {head_size}")
+        if table.shape[0] == 0 or table.shape[1] != rotary_dim:
+            raise ValueError(f"cos_sin_cache is {tuple(table.shape)}, expected [rows, {rotary_dim}]")
+        if positions.numel() != tokens:
+            raise ValueError(f"{positions.numel()} positions for {tokens} tokens")
+        if positions.device.type == "cpu" and tokens:
+            lo, hi = int(positions.min()), int(positions.max())
+            if lo < 0 or hi >= table.shape[0]:
+                raise IndexError(f"positions in [{lo}, {hi}] outside the {table.shape[0]} rows of the cos_sin_cache")
+    if tokens == 0:
+        return query_out
+    if heads == 0 or head_size == 0:
+        raise ValueError("key must have heads and dims")
+    device = key.device
+    slots = _device_slots(slot_mapping.reshape(-1), device, desc.num_blocks * block_size)
+    pos = None
+    if table is not None:
+        pos = positions.reshape(-1).to(device=device, dtype=torch.int64).contiguous()
+        if table.dtype not in _native.DTYPE_CODES:
+            table = table.float()
+        table = table.to(device)
+        if table.stride(1) != 1:
+            table = table.contiguous()
+    q = (query.data_ptr(), query.stride(0), query.stride(1)) if q_heads else (None, 0, 0)
+    q_to = (query_out.data_ptr(), query_out.stride(0), query_out.stride(1)) if q_heads else (None, 0, 0)
+    k_to = (key_out.data_ptr(), key_out.stride(0), key_out.stride(1)) if key_out is not None else (None, 0, 0)
+    rope = (pos.data_ptr(), table.data_ptr(), table.stride(0), table.shape[0], _native.DTYPE_CODES[table.dtype],
+            rotary_dim, int(neox)) if pos is not None else (None, None, 0, 0, 0, 0, 0)
+    rc = _native.on_device(
+        device, _native.load().cbk_paged_append, desc, slots.data_ptr(), tokens, key.data_ptr(), key.stride(0),
+        key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), *q, q_heads, heads, head_size,
+        _native.DTYPE_CODES[key.dtype], int(int4), *rope, *q_to, *k_to, _native.stream_handle(device),
+    )
+    _native.check(rc, "append_paged_kv")
+    return query_out
+
+
+def gather_paged_kv_int4(
+    kv_layer: KVLayer,
+    slot_mapping: torch.Tensor,
+    block_size: int,
+    dtype: torch.dtype = torch.bfloat16,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`gather_paged_kv` of a 4-bit layer (:func:`int4_row_bytes`) as values
+    ``[2, tokens, kv_heads, head_size]`` of ``dtype`` (or ``out``'s): one launch
+    (cbk_paged_gather_int4). Slots as there."""
+    desc, plane = kv_desc(kv_layer, block_size)
+    heads, head_size = int4_geometry(plane)
+    tokens = int(slot_mapping.numel())
+    shape = (2, tokens, heads, head_size)
+    if out is not None:
+        if tuple(out.shape) != shape:
+            raise ValueError(f"gather output has shape {tuple(out.shape)}, expected {shape}")
+        if out.device != plane.device:
+            raise ValueError("gather output must be on the KV cache's device")
+        dtype = out.dtype
+    if dtype not in _native.DTYPE_CODES:
+        raise ValueError(f"dtype {dtype} is not supported")
+    target = torch.empty(shape, dtype=dtype, device=plane.device) if out is None else out
+    if tokens == 0 or heads == 0:
+        return target
+    es = target.element_size()
+    direct = (
+        _plane_rows_ok(target[0])
+        and target.stride(0) != 0
+        and (tokens == 1 or target.stride(1) >= heads * head_size)
+        and (target.data_ptr() | target.stride(0) * es | target.stride(1) * es) % 16 == 0
+    )
+    dst = target if direct else torch.empty(shape, dtype=dtype, device=plane.device)
+    row = dst.stride(1) if tokens > 1 else heads * head_size
+    slots = _device_slots(slot_mapping.reshape(-1), plane.device, desc.num_blocks * block_size)
+    rc = _native.on_device(
+        plane.device, _native.load().cbk_paged_gather_int4, desc, slots.data_ptr(), tokens, heads, head_size,
+        _native.DTYPE_CODES[dtype], dst[0].data_ptr(), dst[1].data_ptr(), row * es,
+        _native.stream_handle(plane.device),
+    )
+    _native.check(rc, "gather_paged_kv_int4")
+    if dst is not target:
+        target.copy_(dst)
+    return target
+
+
 def _layer_descs(kv_layers: Sequence[KVLayer], block_size: int):
     if len(kv_layers) == 0:
         raise ValueError("at least one KV layer is required")

@@ -22,6 +22,20 @@ void clear_error();
     if (!(cond)) return ::cbk::set_error(CBK_ERR_INVALID, __VA_ARGS__); \
   } while (0)
 
+// The checks of a paged layer's descriptor (planes = 1: K alone).
+inline int validate_desc(const cbk_kv_desc* kv, int planes = 2) {
+  CBK_REQUIRE(kv != nullptr, "kv descriptor is NULL");
+  CBK_REQUIRE(kv->k_base != nullptr && (kv->v_base != nullptr || planes == 1), "kv base pointer is NULL");
+  CBK_REQUIRE(kv->num_blocks > 0 && kv->block_size > 0, "num_blocks and block_size must be positive");
+  CBK_REQUIRE(kv->row_bytes > 0, "row_bytes must be positive");
+  CBK_REQUIRE(kv->num_blocks * kv->block_size < (int64_t(1) << 32),
+              "num_blocks * block_size must be below 2^32");
+  CBK_REQUIRE(kv->token_stride >= kv->row_bytes, "token_stride smaller than a row");
+  CBK_REQUIRE(kv->block_stride >= kv->token_stride * kv->block_size || kv->block_size == 1,
+              "block_stride smaller than a block");
+  return CBK_OK;
+}
+
 // Returns CBK_OK, or CBK_ERR_LAUNCH with the HIP error of the last launch.
 int launch_status(const char* what);
 

@@ -232,19 +232,6 @@ __global__ __launch_bounds__(kChunkThreads) void scatter_chunks_kernel(const Chu
   chunks_body<VEC, false>(a);
 }
 
-int validate_desc(const cbk_kv_desc* kv, int planes = 2) {
-  CBK_REQUIRE(kv != nullptr, "kv descriptor is NULL");
-  CBK_REQUIRE(kv->k_base != nullptr && (kv->v_base != nullptr || planes == 1), "kv base pointer is NULL");
-  CBK_REQUIRE(kv->num_blocks > 0 && kv->block_size > 0, "num_blocks and block_size must be positive");
-  CBK_REQUIRE(kv->row_bytes > 0, "row_bytes must be positive");
-  CBK_REQUIRE(kv->num_blocks * kv->block_size < (int64_t(1) << 32),
-              "num_blocks * block_size must be below 2^32");
-  CBK_REQUIRE(kv->token_stride >= kv->row_bytes, "token_stride smaller than a row");
-  CBK_REQUIRE(kv->block_stride >= kv->token_stride * kv->block_size || kv->block_size == 1,
-              "block_stride smaller than a block");
-  return CBK_OK;
-}
-
 int launch_paged(bool gather, const cbk_kv_desc* kv, int32_t num_layers, const int64_t* slots,
                  int64_t num_tokens, char* c_base, int64_t c_layer_stride, int64_t c_plane_stride,
                  int64_t c_token_stride, int32_t* bad, hipStream_t stream, int planes = 2) {
