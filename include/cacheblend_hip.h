@@ -435,6 +435,29 @@ int cbk_blend_attention_ws(const void* q_dev, int64_t q_row_stride_elems, const 
                            float scale, int32_t dtype, void* out_dev, int64_t out_row_stride_elems,
                            void* workspace_dev, size_t workspace_bytes, cbk_stream_t stream);
 
+/*
+ * Attention of each sequence's latest tokens over its context in 4-bit pages
+ * (cbk_paged_append's rows): q [batch, rows, hq, head_dim] (strides in
+ * elements, dims contiguous), row r of sequence b the token at place len_b -
+ * rows + r of its context, which sees the keys up to its own:
+ *   out[b, r, h] = sum_k softmax_k( scale q[b, r, h] . key[k, h/G] ) value[k, h/G]
+ * with the logits, the softmax and the sums in float32. lens [batch] int32
+ * (clamped to 0 .. table_width * block_size); tables [batch, table_width] int32,
+ * row stride in entries: key k of a sequence is in page tables[k / block_size].
+ * A page out of range holds no keys; a row that sees none is zero. head_dim 64
+ * or 128, pages 4-byte aligned (16: the faster transfers at head_dim 128).
+ * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
+ * function gives on the current device, max_len = table_width * block_size.
+ */
+size_t cbk_paged_attention_int4_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
+                                                int64_t max_len);
+int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+                             int64_t batch, int64_t rows, int64_t hq, const cbk_kv_desc* kv, int64_t hkv,
+                             int64_t head_dim, const int32_t* tables_dev, int64_t table_stride, int64_t table_width,
+                             const int32_t* lens_dev, float scale, int32_t dtype, void* out_dev,
+                             int64_t out_batch_stride, int64_t out_row_stride, int64_t out_head_stride,
+                             void* workspace_dev, size_t workspace_bytes, cbk_stream_t stream);
+
 /* Workspace bytes cbk_sparse_q_scores needs. Per (query, head), queries padded
  * to a multiple of 64: 264 bytes (row statistics, a dense copy of the query row
  * sized for head_dim 128) and 8 per key range (8 ranges; up to 64 while they

@@ -1,4 +1,5 @@
-"""Side-forward attention of the selected queries on MI355X.
+"""Attention on MI355X: of the selected queries, and of single tokens over 4-bit
+pages.
 
 ``blend_attention`` keeps the signature of ``Qwen3BlendExecutor._attention``
 (cacheblend_vllm/ascend.py:798-846): queries ``[Nq, Hq, D]`` at absolute
@@ -15,6 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
+from .kv_layout import KVLayer, int4_geometry, kv_desc
 
 
 def blend_attention(
@@ -72,4 +74,109 @@ def blend_attention(
         _native.ptr(ws), nbytes, _native.stream_handle(query.device),
     )
     _native.check(rc, "blend_attention")
+    return out
+
+
+def _whole_int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Whole numbers as int32 on ``device``; what int32 does not hold stays out of range."""
+    if t.dtype != torch.int32:
+        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+            raise ValueError(f"whole numbers expected, got {t.dtype}")
+        if t.dtype in (torch.int64, torch.uint32, torch.uint64):
+            t = t.to(torch.int64).clamp(-1, (1 << 31) - 1)
+    return t.to(device=device, dtype=torch.int32, non_blocking=True)
+
+
+def _check_out(out: torch.Tensor, query: torch.Tensor) -> None:
+    """An output of ``query``'s shape and type whose rows lie apart."""
+    if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
+        raise ValueError(f"out must be {tuple(query.shape)} {query.dtype} on {query.device}")
+    if out.stride(-1) != 1:
+        raise ValueError("out rows must hold contiguous dims")
+    span = out.shape[-1]
+    for n, stride in sorted(zip(out.shape[:-1], out.stride()[:-1]), key=lambda d: d[1]):
+        if n > 1 and stride < span:
+            raise ValueError("out rows must not overlap")
+        span += (n - 1) * stride
+
+
+def paged_attention_int4(
+    query: torch.Tensor,
+    kv_layer: KVLayer,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    scale: float,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each sequence's latest tokens over its context in 4-bit pages
+    (``kv_layout.append_paged_kv`` to a ``uint8`` layer): a decode step.
+
+    ``query`` is ``[batch, q_heads, head_size]``, one token a sequence, or ``[batch,
+    rows, q_heads, head_size]``: the last ``rows`` tokens, each of which sees the
+    keys up to its own. Key ``k`` of sequence ``b`` is in page ``block_tables[b, k //
+    block_size]``; ``context_lens[b]`` counts the keys, those of ``query``'s tokens
+    among them (append before attending). Head sizes 64 and 128; logits, softmax
+    and sums in float32, whatever the queries' type.
+
+    Lengths on the host are checked, and the tables where both are there
+    (``IndexError``). On the device they are not read back: lengths are clamped
+    to what a table holds, a page outside the cache holds no keys, and a row that
+    sees no key is zero.
+    """
+    _native.require_device(query, "query")
+    if query.dim() not in (3, 4):
+        raise ValueError("query must be [batch, q_heads, head_size] or [batch, rows, q_heads, head_size]")
+    if query.dtype not in _native.DTYPE_CODES:
+        raise ValueError(f"dtype {query.dtype} is not supported")
+    desc, plane = kv_desc(kv_layer, block_size)
+    hkv, d = int4_geometry(plane)
+    device = query.device
+    if plane.device != device:
+        raise ValueError(f"query is on {device}, the cache on {plane.device}")
+    q = query if query.dim() == 4 else query.unsqueeze(1)
+    batch, rows, hq = q.shape[:3]
+    if q.shape[3] != d:
+        raise ValueError(f"query head size {q.shape[3]} does not match the pages' {d}")
+    if d not in (64, 128):
+        raise ValueError(f"head size {d}: 64 or 128 supported")
+    if hkv == 0 or hq % hkv or (hq == 0 and batch * rows):
+        raise ValueError(f"query heads ({hq}) must be divisible by KV heads ({hkv})")
+    if q.stride(3) != 1:
+        raise ValueError("query rows must hold contiguous dims")
+    if block_tables.dim() != 2 or block_tables.shape[0] != batch or context_lens.numel() != batch:
+        raise ValueError(f"{tuple(block_tables.shape)} block tables and {context_lens.numel()} lengths for {batch} sequences")
+    width = block_tables.shape[1]
+    if context_lens.device.type == "cpu" and batch:
+        lo, hi = int(context_lens.min()), int(context_lens.max())
+        if lo < 0 or hi > width * block_size:
+            raise IndexError(f"context lengths in [{lo}, {hi}] outside the {width} blocks of {block_size}")
+        if block_tables.device.type == "cpu":
+            used = torch.arange(width) * block_size < context_lens.reshape(-1, 1)
+            pages = block_tables[used]
+            if pages.numel() and (int(pages.min()) < 0 or int(pages.max()) >= desc.num_blocks):
+                raise IndexError(f"block tables hold pages outside [0, {desc.num_blocks})")
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    else:
+        _check_out(out, query)
+    if batch * rows * hq == 0:
+        return out
+    tables = _whole_int32(block_tables, device)
+    if width and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    lens = _whole_int32(context_lens.reshape(-1), device).contiguous()
+    o = out if out.dim() == 4 else out.unsqueeze(1)
+    lib = _native.load()
+    nbytes = _native.on_device(device, lib.cbk_paged_attention_int4_workspace_bytes, batch, rows, hq, hkv, d,
+                               width * block_size)
+    # from torch's allocator on every call: a captured graph then owns its own
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    rc = _native.on_device(
+        device, lib.cbk_paged_attention_int4, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), batch, rows, hq,
+        desc, hkv, d, tables.data_ptr() if width else None, tables.stride(0), width, lens.data_ptr(), float(scale),
+        _native.DTYPE_CODES[query.dtype], o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), ws.data_ptr(), ws.numel(),
+        _native.stream_handle(device),
+    )
+    _native.check(rc, "paged_attention_int4")
     return out

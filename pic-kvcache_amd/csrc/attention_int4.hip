@@ -1,0 +1,743 @@
+// Attention of a sequence's latest tokens over its context in 4-bit pages
+// (int4_rows.hpp) for gfx950:
+//
+//   out[b, r, h] = sum_k softmax_k( scale q[b, r, h] . key[k, h / G] ) value[k, h / G]
+//
+// over keys k <= len_b - R + r of sequence b (row r of its R rows is the
+// token at that place), G = Hq / Hkv.
+//
+// Bound by HBM: 0.625 bytes a key or value element, each read once for all
+// heads of a group. The codes go to the matrix cores as they are. With key
+// element offset + step * n, n the 4-bit code, and 32 dims g sharing both,
+//
+//   q . key   = sum_g step_g (sum_{d in g} q_d n_d) + offset_g (sum_{d in g} q_d)
+//   out_d     = sum_k (p_k step_g) n_d + sum_k p_k offset_g
+//
+// so the inner sums are v_mfma_f32_16x16x32_bf16 products of small whole
+// numbers, exact in bf16, made from the codes by one and-or per two: 0x4300 | n
+// is 128 + n, and 128 times the other operand's sum is taken off again (for
+// float32 the codes are converted, without the 128). The other operand is cut
+// into bf16 parts: q exactly (one part for bf16, two for f16, three for
+// float32), p step into two (2^-15 of it is lost) or three.
+//
+// A wave takes 64 keys of one KV head at a time, K and V rows staged in its own
+// LDS by DMA (K two tiles ahead, V one: no barrier in the loop), and 16 columns of S^T =
+// K . Q^T: VT column groups of 16 / VT rows each, for the rows of the group
+// are often fewer than 16. The Q operand of a 16-key tile is zero outside the
+// tile's column group, so VT tiles share an accumulator and the softmax's work
+// on the VALU is spread over all columns.
+// Tile t's row m is key 16 (m / 4) + 4 t + m % 4 of the 64, so that lane (j =
+// lane / 16, c) holds, over the four tiles, keys 16 j .. 16 j + 15: those whose
+// codes of one dim a ds_read_tr4_b64 hands to lane group j.
+//
+// The sequences' 64-key tiles, one after another, are cut into as many equal
+// ranges as fill the GPU; a workgroup takes one range of one KV head (and row
+// tile), its four waves every fourth tile, whatever sequences they belong to.
+// A sequence that one range holds whole is written at once, the others'
+// partial results are merged by a second launch.
+#include <cmath>
+#include <type_traits>
+
+#include "int4_rows.hpp"
+
+namespace cbk {
+namespace {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTile = 64;      // keys of a wave's step
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kRescale = 8.f;  // log2 headroom before the reference maximum is raised
+
+struct Int4AttnArgs {
+  const void* q;
+  void* out;
+  int64_t q_batch, q_row, q_head;        // elements
+  int64_t out_batch, out_row, out_head;
+  const char* k_base;
+  const char* v_base;
+  int64_t block_stride, token_stride;    // bytes
+  const int32_t* tables;
+  int64_t table_stride;                  // entries
+  const int32_t* lens;
+  uint32_t batch, rows, hq, hkv, group;  // rows: of a sequence
+  uint32_t num_blocks, max_len;
+  uint32_t row_tiles;                    // of 16 / VT (row, head of the group) pairs
+  uint32_t ranges;
+  float scale;
+  FastDiv block_div;
+  // partial results of range r's first (0) and last (1) unfinished sequence:
+  // entry ((2 r + which) hkv + kv head) * rows * group + row * group + head
+  float2* ml;
+  float* o;
+};
+
+// The tiles [first, end) of range r of `total` tiles.
+struct Ranges {
+  uint32_t each, more;  // tiles of a range; ranges that have one more
+  __device__ __forceinline__ Ranges(uint32_t total, uint32_t ranges) : each(total / ranges), more(total % ranges) {}
+  __device__ __forceinline__ uint32_t first(uint32_t r) const { return r * each + min(r, more); }
+  __device__ __forceinline__ uint32_t of(uint32_t tile) const {
+    const uint32_t big = more * (each + 1);
+    return tile < big ? tile / (each + 1) : more + (tile - big) / each;
+  }
+};
+
+__device__ __forceinline__ uint32_t context_of(const Int4AttnArgs& a, uint32_t b) {
+  return uint32_t(min(max(a.lens[b], 0), int32_t(a.max_len)));
+}
+
+__device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + kTile - 1) / kTile; }
+
+// All sequences' tiles, by a whole wave.
+__device__ uint32_t total_tiles(const Int4AttnArgs& a, uint32_t lane) {
+  uint32_t n = 0;
+  for (uint32_t b = lane; b < a.batch; b += 64) n += tiles_of(context_of(a, b));
+  return __builtin_amdgcn_readfirstlane(wave_sum_u32(n));
+}
+
+// LDS DMA from a 64-bit address per lane (the rows of pages anywhere): lane
+// l's 16 or 4 bytes land at lds + l * size. M0 and its waits as CBK_LDS_DMA's.
+#define CBK_LDS_DMA64(op)                                                                        \
+  "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 4\n\t" op " %1, off\n\ts_nop 0\n\ts_mov_b32 m0, %0"
+template <int PIECE>
+__device__ __forceinline__ void lds_dma(const char* addr, uint32_t lds) {
+  uint32_t saved;
+  if constexpr (PIECE == 16) {
+    asm volatile(CBK_LDS_DMA64("global_load_lds_dwordx4")
+                 : "=&s"(saved) : "v"(addr), "s"(__builtin_amdgcn_readfirstlane(int(lds))) : "memory");
+  } else {
+    asm volatile(CBK_LDS_DMA64("global_load_lds_dword")
+                 : "=&s"(saved) : "v"(addr), "s"(__builtin_amdgcn_readfirstlane(int(lds))) : "memory");
+  }
+}
+
+// 8 codes of a word as the 8 bf16 of an MFMA operand, in the order 0 4 1 5 2 6
+// 3 7: as 128 + n, or (EXACT) as n.
+template <bool EXACT>
+__device__ __forceinline__ s16x8 operand(uint32_t w) {
+  u32x4 r;
+  if constexpr (EXACT) {
+    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6, 1 3 5 7
+    auto f = [](uint32_t x, int byte) { return __float_as_uint(float((x >> (8 * byte)) & 0xffu)); };
+    auto pair = [](uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); };
+    r[0] = pair(f(even, 0), f(even, 2));
+    r[1] = pair(f(odd, 0), f(odd, 2));
+    r[2] = pair(f(even, 1), f(even, 3));
+    r[3] = pair(f(odd, 1), f(odd, 3));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  }
+  return __builtin_bit_cast(s16x8, r);
+}
+
+template <int DT> __device__ __forceinline__ float load_elem(const void* p, int64_t at);
+template <> __device__ __forceinline__ float load_elem<CBK_DTYPE_F32>(const void* p, int64_t at) {
+  return static_cast<const float*>(p)[at];
+}
+template <> __device__ __forceinline__ float load_elem<CBK_DTYPE_BF16>(const void* p, int64_t at) {
+  return bf16_bits_to_float(static_cast<const uint16_t*>(p)[at]);
+}
+template <> __device__ __forceinline__ float load_elem<CBK_DTYPE_F16>(const void* p, int64_t at) {
+  return float(static_cast<const _Float16*>(p)[at]);
+}
+template <int DT> __device__ __forceinline__ void store_elem(void* p, int64_t at, float x) {
+  if constexpr (DT == CBK_DTYPE_F32) static_cast<float*>(p)[at] = x;
+  else if constexpr (DT == CBK_DTYPE_BF16) static_cast<__bf16*>(p)[at] = __bf16(x);
+  else static_cast<_Float16*>(p)[at] = _Float16(x);
+}
+
+template <int DT> struct Parts;
+template <> struct Parts<CBK_DTYPE_BF16> { static constexpr int q = 1, p = 2; };
+template <> struct Parts<CBK_DTYPE_F16> { static constexpr int q = 2, p = 2; };
+template <> struct Parts<CBK_DTYPE_F32> { static constexpr int q = 3, p = 3; };
+
+template <int DT, int NG, int VT, int PIECE>
+__global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnArgs a) {
+  constexpr bool EXACT = DT == CBK_DTYPE_F32;
+  constexpr int QP = Parts<DT>::q, PP = Parts<DT>::p;
+  constexpr int D = 32 * NG, RB = kInt4GroupBytes * NG;  // dims and bytes of a head's row
+  constexpr int U = 4 / VT, COLS = 16 / VT;
+  constexpr uint32_t kBuf = kTile * RB;                  // one of K or V
+  constexpr uint32_t kPieces = RB / PIECE, kInsts = kTile * kPieces / 64;
+  constexpr uint32_t kWaveLds = 3 * kBuf;                // two K buffers, one of V: two workgroups per CU
+  static_assert(16 * D * 4 + 128 <= int(kWaveLds), "the wave's results fit its buffers");
+  // per wave: K buffers, V buffer; then the results of a sequence
+  __shared__ __attribute__((aligned(16))) char lds[kWaves][kWaveLds];
+  __shared__ uint32_t s_pages[kWaves][2][kTile];  // block table entries of two tiles' keys
+
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t j = lane >> 4, c = lane & 15;
+  // workgroups of one range (all KV heads and row tiles) on one XCD, one after
+  // another: a token's row is one piece of memory for all heads
+  const uint32_t units = a.hkv * a.row_tiles;
+  const uint32_t turn = blockIdx.x >> 3;
+  const uint32_t range = __builtin_amdgcn_readfirstlane((turn / units) * 8 + (blockIdx.x & 7));
+  if (range >= a.ranges) return;
+  const uint32_t unit = __builtin_amdgcn_readfirstlane(turn % units);
+  const uint32_t kvh = unit / a.row_tiles, row_tile = unit - kvh * a.row_tiles;
+
+  const Ranges cut(total_tiles(a, lane), a.ranges);
+  uint32_t at = cut.first(range);
+  const uint32_t end = cut.first(range + 1);
+  if (at == end) return;
+  // the sequence that holds tile `at`, and the tiles before it
+  uint32_t seq = 0, before = 0;
+  for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+    const uint32_t n = b0 + lane < a.batch ? tiles_of(context_of(a, b0 + lane)) : 0u;
+    const uint32_t upto = before + wave_inclusive_scan(n);
+    const uint64_t past = __ballot(upto > at);
+    if (past) {
+      const int first = __builtin_ctzll(past);
+      seq = b0 + uint32_t(first);
+      before = __builtin_amdgcn_readfirstlane(__shfl(int(upto - n), first));
+      break;
+    }
+    before = __builtin_amdgcn_readfirstlane(__shfl(int(upto), 63));
+  }
+  seq = __builtin_amdgcn_readfirstlane(seq);
+
+  // this lane's row (row, head of the group) and its column group
+  const uint32_t v = c / COLS, n_row = row_tile * COLS + c % COLS;
+  const bool live = n_row < a.rows * a.group;
+  const uint32_t qr = live ? n_row / a.group : 0, qh = kvh * a.group + (live ? n_row % a.group : 0);
+  // a negative scale goes into the queries
+  const float sign = a.scale < 0.f ? -1.f : 1.f, c2 = fabsf(a.scale) * kLog2e;
+  const uint32_t lds0 = lds_address(&lds[wave][0]), pages0 = lds_address(&s_pages[wave][0][0]);
+  // the selector that puts a float's upper half into the low (tile even) or high half of a word
+  const uint32_t place = v ? 0x03020c0cu : 0x0c0c0302u;
+
+  for (bool first_seq = true; at < end; first_seq = false) {
+    uint32_t len = context_of(a, seq);
+    while (before + tiles_of(len) <= at) {  // empty sequences, and on to the next
+      before += tiles_of(len);
+      len = context_of(a, ++seq);
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    len = __builtin_amdgcn_readfirstlane(len);
+    before = __builtin_amdgcn_readfirstlane(before);
+    const uint32_t seq_end = before + tiles_of(len);
+    const uint32_t stop = min(end, seq_end);
+    const bool whole = at == before && stop == seq_end;
+    const int32_t tile0 = int32_t(at - before + wave);           // the wave's first tile of the sequence
+    const int32_t count = max(0, (int32_t(stop - at) - int32_t(wave) + kWaves - 1) / kWaves);
+    const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
+    const int32_t last_key = live ? int32_t(len) - int32_t(a.rows) + int32_t(qr) : -1;  // the row sees keys up to it
+
+    // Q operands and the sums of their groups
+    s16x8 qf[QP][VT][NG];
+    float qs[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int64_t from = int64_t(seq) * a.q_batch + int64_t(qr) * a.q_row + int64_t(qh) * a.q_head + 32 * g + 8 * j;
+      float x[8], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = live ? sign * load_elem<DT>(a.q, from + e) : 0.f;
+        sum += x[e];
+      }
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      qs[g] = sum;
+#pragma unroll
+      for (int p = 0; p < QP; ++p) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(__float_as_uint(x[i + 4]), __float_as_uint(x[i]), 0x07060302u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] -= __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
+#pragma unroll
+        for (int t = 0; t < VT; ++t) qf[p][t][g] = __builtin_bit_cast(s16x8, VT == 1 || v == uint32_t(t) ? w : u32x4(0u));
+      }
+    }
+
+    float m = kNegInf, l = 0.f, zsum[NG];
+    f32x4 o[2 * NG], ones[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      zsum[g] = 0.f;
+      ones[g] = o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // The block table's entries of tile i's keys, by DMA; from them where the
+    // tile's rows are; and K or V of those rows, by DMA. Keys past the context,
+    // or in a page out of range, are read from the first page and masked: their
+    // bits of the result are clear.
+    auto entries = [&](int32_t i) __attribute__((always_inline)) {
+      const uint32_t key = min(uint32_t(tile0 + kWaves * i) * kTile + lane, len - 1);
+      lds_dma<4>(reinterpret_cast<const char*>(table + a.block_div.div(key)), pages0 + uint32_t(i & 1) * kTile * 4);
+    };
+    int64_t row = 0;  // of key `lane` of the tile located last, from the planes' bases
+    auto locate = [&](int32_t i) __attribute__((always_inline)) {
+      const uint32_t key = uint32_t(tile0 + kWaves * i) * kTile + lane;
+      const uint32_t page = s_pages[wave][i & 1][lane];
+      const bool held = key < len && page < a.num_blocks;
+      row = 0;
+      if (held) {
+        const uint32_t blk = a.block_div.div(key);
+        row = int64_t(page) * a.block_stride + int64_t(key - blk * a.block_div.d) * a.token_stride;
+      }
+      return __ballot(held);
+    };
+    auto request = [&](const char* base, uint32_t buf) __attribute__((always_inline)) {
+      const int lo = int(uint32_t(row)), hi = int(uint32_t(uint64_t(row) >> 32));
+      base += int64_t(kvh) * RB;
+#pragma unroll
+      for (uint32_t n = 0; n < kInsts; ++n) {
+        // piece 64 n + lane: of the buffer's row R, which is key 16 (R % 16 / 4) + 4 (R / 16) + R % 4
+        const uint32_t piece = 64 * n + lane, R = piece / kPieces, part = piece - R * kPieces;
+        const int from = int(16 * ((R >> 2) & 3) + 4 * (R >> 4) + (R & 3));
+        uint64_t off = uint64_t(uint32_t(__shfl(lo, from))) | (uint64_t(uint32_t(__shfl(hi, from))) << 32);
+        off += part * PIECE;
+        asm volatile("" : "+v"(off));  // (base + part would be kept in registers for every n)
+        lds_dma<PIECE>(base + int64_t(off), buf + n * 64 * PIECE);
+      }
+    };
+
+    uint64_t held = 0, held_next = 0;
+    CBK_WAIT_VM_LGKM0(0);  // nothing of the compiler's own in flight
+    if (count > 0) {
+      entries(0);
+      if (count > 1) entries(1);
+      CBK_WAIT_VM_LGKM0(0);
+      held = locate(0);
+      request(a.k_base, lds0);
+      request(a.v_base, lds0 + 2 * kBuf);
+      if (count > 2) entries(2);
+      if (count > 1) {
+        held_next = locate(1);
+        request(a.k_base, lds0 + kBuf);
+      }
+    }
+    for (int32_t i = 0; i < count; ++i) {
+      // requested in this order: K(i), V(i), the entries of tile i + 2, K(i + 1);
+      // K(i) has landed
+      if (i + 1 < count) CBK_WAIT_VM_LGKM0(2 * kInsts);
+      else CBK_WAIT_VM_LGKM0(kInsts);
+      asm volatile("" ::: "memory");
+      const char* kb = &lds[wave][(i & 1) * kBuf];
+      const char* vb = &lds[wave][2 * kBuf];
+      const int32_t key0 = (tile0 + kWaves * i) * kTile;
+      const uint64_t here = held;
+      const bool masked = here != ~uint64_t(0) || key0 + kTile > int32_t(len - a.rows + 1);
+
+      auto step = [&](auto mask) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask)::value;
+        // S^T: x[u][i] is the logit (log2 units) of key 16 j + 4 (u VT + v) + i and column c's row
+        f32x4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          __builtin_amdgcn_sched_barrier(0);
+          f32x4 acc[NG];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const float init = EXACT ? 0.f : -128.f * qs[g];
+            acc[g] = f32x4{init, init, init, init};
+#pragma unroll
+            for (int t = 0; t < VT; ++t) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + t) + c) * RB + 16 * g + 4 * j);
+              const s16x8 kf = operand<EXACT>(w);
+#pragma unroll
+              for (int p = 0; p < QP; ++p) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[p][t][g], acc[g], 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t* sw = reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
+            float s = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              s = fmaf(__uint_as_float(sw[g] << 16), acc[g][r], s);
+              s = fmaf(__uint_as_float(sw[g] & 0xffff0000u), qs[g], s);
+            }
+            x[u][r] = s * c2;
+          }
+        }
+        // which of the lane's keys its row sees: bit 4 t + i of `seen`
+        uint32_t seen = 0xffffu;
+        if constexpr (MASK) {
+          const int32_t left = last_key - key0 - int32_t(16 * j) + 1;  // of the lane's 16 keys
+          seen = uint32_t(here >> (16 * j)) & 0xffffu;
+          seen &= left <= 0 ? 0u : left >= 16 ? 0xffffu : (1u << left) - 1u;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!((seen >> (4 * (u * VT + v) + r)) & 1u)) x[u][r] = kNegInf;
+        }
+        float lm = x[0][0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) lm = fmaxf(lm, x[u][r]);
+        if (__any(lm > m + kRescale)) {  // rare: raise the reference of the columns that need it
+          float bm = fmaxf(lm, __shfl_xor(lm, 16));
+          bm = fmaxf(bm, __shfl_xor(bm, 32));
+          const float mn = fmaxf(m, bm);
+          const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= alpha;
+          float ao[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ao[r] = __shfl(alpha, int(4 * j + r));
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            zsum[g] *= alpha;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              o[2 * g][r] *= ao[r];
+              o[2 * g + 1][r] *= ao[r];
+              ones[g][r] *= ao[r];
+            }
+          }
+        }
+        const float ms = m == kNegInf ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - ms);  // p from here on
+            l += x[u][r];
+          }
+        // V(i) and the entries have landed
+        if (i + 1 < count) CBK_WAIT_VM_LGKM0(kInsts);
+        else CBK_WAIT_VM_LGKM0(0);
+        asm volatile("" ::: "memory");
+        // O += (p step) . n, the 32 keys of tiles 2 h and 2 h + 1 at a time: p step
+        // in bf16 parts, operand word r key r of the first tile in its low half,
+        // of the second in its high half
+        const uint32_t from = (16 * (c >> 2) + 4 * j + (c & 3)) * RB;  // the row of key 16 j + c
+        const s16x8 one = __builtin_bit_cast(s16x8, u32x4(0x3f803f80u));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          __builtin_amdgcn_sched_barrier(0);
+          u32x4 pw[NG][PP];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float y[NG][2 / VT];
+#pragma unroll
+            for (int t = 0; t < 2 / VT; ++t) {
+              const int u = h * (2 / VT) + t;
+              const uint32_t* sw = reinterpret_cast<const uint32_t*>(vb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
+              const bool sees = !MASK || ((seen >> (4 * (u * VT + v) + r)) & 1u);
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                const uint32_t word = sees ? sw[g] : 0u;  // a masked key's step and offset may be anything
+                y[g][t] = x[u][r] * __uint_as_float(word << 16);
+                zsum[g] = fmaf(x[u][r], __uint_as_float(word & 0xffff0000u), zsum[g]);
+              }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+              for (int q = 0; q < PP; ++q) {
+                if constexpr (VT == 1) {
+                  pw[g][q][r] = __builtin_amdgcn_perm(__float_as_uint(y[g][1]), __float_as_uint(y[g][0]), 0x07060302u);
+                } else {
+                  pw[g][q][r] = __builtin_amdgcn_perm(0u, __float_as_uint(y[g][0]), place);
+                }
+                if (q + 1 < PP)
+#pragma unroll
+                  for (int t = 0; t < 2 / VT; ++t) y[g][t] -= __uint_as_float(__float_as_uint(y[g][t]) & 0xffff0000u);
+              }
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                  (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) const void*)(vb + from + 16 * g + 8 * d)));
+              const s16x8 vf = operand<EXACT>(uint32_t(w[h]));
+#pragma unroll
+              for (int q = 0; q < PP; ++q)
+                o[2 * g + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(s16x8, pw[g][q]), vf, o[2 * g + d], 0, 0, 0);
+            }
+            if constexpr (!EXACT)
+#pragma unroll
+              for (int q = 0; q < PP; ++q)
+                ones[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(s16x8, pw[g][q]), one, ones[g], 0, 0, 0);
+          }
+        }
+      };
+      if (masked) step(std::true_type());
+      else step(std::false_type());
+
+      // the reads of this tile's buffers are done before the next requests into them
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      held = held_next;
+      if (i + 1 < count) request(a.v_base, lds0 + 2 * kBuf);
+      if (i + 3 < count) entries(i + 3);
+      if (i + 2 < count) {
+        held_next = locate(i + 2);
+        request(a.k_base, lds0 + uint32_t(i & 1) * kBuf);
+      }
+    }
+
+    // the wave's results, then all waves' and column groups' together
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      zsum[g] += __shfl_xor(zsum[g], 16);
+      zsum[g] += __shfl_xor(zsum[g], 32);
+    }
+    float* mine = reinterpret_cast<float*>(&lds[wave][0]);  // [16 columns][D], then m and l of each
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float z = __shfl(zsum[g], int(4 * j + r)) - (EXACT ? 0.f : 128.f * ones[g][r]);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) mine[(4 * j + r) * D + 32 * g + 16 * d + c] = o[2 * g + d][r] + z;
+      }
+    if (j == 0) {
+      mine[16 * D + 2 * c] = m;
+      mine[16 * D + 2 * c + 1] = l;
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < uint32_t(COLS * D); e += kThreads) {
+      const uint32_t row = e / D, dim = e - row * D, n = row_tile * COLS + row;
+      if (n >= a.rows * a.group) break;
+      float top = kNegInf, sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+        for (int t = 0; t < VT; ++t) top = fmaxf(top, reinterpret_cast<const float*>(&lds[w][0])[16 * D + 2 * (t * COLS + row)]);
+      const float ts = top == kNegInf ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+          const float* res = reinterpret_cast<const float*>(&lds[w][0]);
+          const uint32_t col = t * COLS + row;
+          const float f = __builtin_amdgcn_exp2f(res[16 * D + 2 * col] - ts);
+          sum = fmaf(f, res[16 * D + 2 * col + 1], sum);
+          acc = fmaf(f, res[col * D + dim], acc);
+        }
+      const uint32_t r = n / a.group, h = kvh * a.group + n % a.group;
+      if (whole) {
+        store_elem<DT>(a.out, int64_t(seq) * a.out_batch + int64_t(r) * a.out_row + int64_t(h) * a.out_head + dim,
+                       sum == 0.f ? 0.f : acc / sum);
+      } else {
+        const int64_t id = (int64_t(2 * range + (first_seq ? 0 : 1)) * a.hkv + kvh) * (a.rows * a.group) + n;
+        a.o[id * D + dim] = acc;
+        if (dim == 0) a.ml[id] = make_float2(top, sum);
+      }
+    }
+    __syncthreads();  // the buffers are free for the next sequence
+    at = stop;
+  }
+}
+
+// The sequences that more than one range holds, and those without keys: 32
+// lanes a row, each D / 32 dims.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void int4_attn_merge_kernel(const Int4AttnArgs a) {
+  constexpr int N = D / 32;
+  const uint32_t seq = blockIdx.y;
+  const uint32_t lane = threadIdx.x & 63;
+  // tiles before the sequence, and of all
+  uint32_t before = 0, total = 0;
+  for (uint32_t b = lane; b < a.batch; b += 64) {
+    const uint32_t n = tiles_of(context_of(a, b));
+    total += n;
+    before += b < seq ? n : 0u;
+  }
+  total = __builtin_amdgcn_readfirstlane(wave_sum_u32(total));
+  before = __builtin_amdgcn_readfirstlane(wave_sum_u32(before));
+  const uint32_t tiles = tiles_of(context_of(a, seq));
+  const uint32_t row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), sub = threadIdx.x & 31;
+  const uint32_t per_head = a.rows * a.group;
+  if (row >= a.hkv * per_head) return;
+  const uint32_t kvh = row / per_head, n = row - kvh * per_head;
+  float acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  float inv = 0.f;
+  if (tiles != 0) {
+    const Ranges cut(total, a.ranges);
+    const uint32_t r0 = cut.of(before), r1 = cut.of(before + tiles - 1);
+    if (r0 == r1) return;  // written by its range
+    // range r0 may end with this sequence after others; the rest begin in it
+    const uint32_t which0 = cut.first(r0) < before ? 1u : 0u;
+    auto id = [&](uint32_t r) { return (int64_t(2 * r + (r == r0 ? which0 : 0u)) * a.hkv + kvh) * per_head + n; };
+    float top = kNegInf;
+    for (uint32_t r = r0 + sub; r <= r1; r += 32) top = fmaxf(top, a.ml[id(r)].x);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 32));
+    const float ts = top == kNegInf ? 0.f : top;
+    float sum = 0.f;
+    for (uint32_t b0 = r0; b0 <= r1; b0 += 32) {
+      float2 ml = make_float2(kNegInf, 0.f);
+      if (b0 + sub <= r1) ml = a.ml[id(b0 + sub)];
+      const float f = __builtin_amdgcn_exp2f(ml.x - ts);
+      sum = fmaf(f, ml.y, sum);
+      const uint32_t most = min(32u, r1 - b0 + 1);
+      for (uint32_t i = 0; i < most; ++i) {
+        const float w = __shfl(f, int(i), 32);
+        const float* src = a.o + id(b0 + i) * D + N * sub;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = fmaf(w, src[e], acc[e]);
+      }
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 32);
+    inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (sum == 0.f)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  }
+  const uint32_t r = n / a.group, h = kvh * a.group + n % a.group;
+  const int64_t to = int64_t(seq) * a.out_batch + int64_t(r) * a.out_row + int64_t(h) * a.out_head + N * sub;
+#pragma unroll
+  for (int e = 0; e < N; ++e) store_elem<DT>(a.out, to + e, acc[e] * inv);
+}
+
+// Columns of a workgroup's rows: VT = 2 where 8 rows of a KV head hold them all
+constexpr uint32_t kFewRows = 8;
+
+struct Plan {
+  uint32_t row_tiles, ranges;
+};
+
+int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t max_len, Plan* p) {
+  CBK_REQUIRE(batch >= 0 && batch < (1 << 16), "batch out of range");
+  CBK_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "query heads must be divisible by KV heads");
+  CBK_REQUIRE(rows > 0 && hq < (1 << 16) && rows < (1 << 16), "rows or heads out of range");
+  CBK_REQUIRE(max_len >= 0 && max_len < (int64_t(1) << 31) - kTile, "context out of range");
+  const int64_t n = rows * (hq / hkv);
+  p->row_tiles = n <= kFewRows ? 1 : uint32_t((n + 15) / 16);
+  int cus = 0;
+  if (int rc = device_cus(&cus)) return rc;
+  // two workgroups of each CU at once (LDS); fewer where there are fewer tiles
+  const int64_t most = batch * ((max_len + kTile - 1) / kTile);
+  CBK_REQUIRE(most < (int64_t(1) << 31), "context tiles out of range");
+  const int64_t units = hkv * int64_t(p->row_tiles);
+  int64_t ranges = (2 * int64_t(cus) + units - 1) / units;
+  ranges = ranges < most ? ranges : most;
+  p->ranges = uint32_t(ranges > 1 ? ranges : 1);
+  return CBK_OK;
+}
+
+size_t ml_bytes(const Plan& p, int64_t rows, int64_t hq) {
+  return (size_t(2) * p.ranges * size_t(rows) * size_t(hq) * sizeof(float2) + 255) & ~size_t(255);
+}
+
+size_t plan_bytes(const Plan& p, int64_t rows, int64_t hq, int64_t d) {
+  return ml_bytes(p, rows, hq) + size_t(2) * p.ranges * size_t(rows) * size_t(hq) * size_t(d) * sizeof(float);
+}
+
+template <int DT, int NG>
+int launch(const Int4AttnArgs& a, bool pieces16, hipStream_t s) {
+  const uint64_t groups = uint64_t(a.hkv) * a.row_tiles * ((a.ranges + 7) / 8 * 8);
+  CBK_REQUIRE(groups * kThreads < (uint64_t(1) << 32), "int4 attention: %llu workgroups exceed one launch",
+              (unsigned long long)groups);
+  const dim3 grid(uint32_t(groups), 1, 1), block(kThreads);
+  const bool few = a.rows * a.group <= kFewRows;
+  if (pieces16 && NG % 4 == 0) {
+    constexpr int P = NG % 4 == 0 ? 16 : 4;
+    if (few) hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 2, P>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 1, P>), grid, block, 0, s, a);
+  } else {
+    if (few) hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 2, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 1, 4>), grid, block, 0, s, a);
+  }
+  if (int rc = launch_status("int4 attention")) return rc;
+  const uint64_t rows = uint64_t(a.rows) * a.hq;
+  const dim3 merge(uint32_t((rows + kThreads / 32 - 1) / (kThreads / 32)), a.batch);
+  hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG>), merge, block, 0, s, a);
+  return launch_status("int4 attention merge");
+}
+
+}  // namespace
+}  // namespace cbk
+
+extern "C" {
+
+size_t cbk_paged_attention_int4_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
+                                                int64_t max_len) {
+  using namespace cbk;
+  Plan p;
+  if (batch <= 0 || head_dim <= 0 || plan_of(batch, rows, hq, hkv, max_len, &p)) return 0;
+  return plan_bytes(p, rows, hq, head_dim);
+}
+
+int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+                             int64_t batch, int64_t rows, int64_t hq, const cbk_kv_desc* kv, int64_t hkv,
+                             int64_t head_dim, const int32_t* tables_dev, int64_t table_stride, int64_t table_width,
+                             const int32_t* lens_dev, float scale, int32_t dtype, void* out_dev,
+                             int64_t out_batch_stride, int64_t out_row_stride, int64_t out_head_stride,
+                             void* workspace_dev, size_t workspace_bytes, cbk_stream_t stream) {
+  using namespace cbk;
+  clear_error();
+  if (int rc = validate_desc(kv)) return rc;
+  CBK_REQUIRE(dtype == CBK_DTYPE_F32 || dtype == CBK_DTYPE_BF16 || dtype == CBK_DTYPE_F16, "dtype %d", int(dtype));
+  CBK_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim %lld: 64 or 128 supported", (long long)head_dim);
+  CBK_REQUIRE(hkv > 0 && kv->row_bytes == hkv * int4_row_bytes(head_dim), "a 4-bit row of %lld x %lld is not %lld bytes",
+              (long long)hkv, (long long)head_dim, (long long)kv->row_bytes);
+  CBK_REQUIRE(std::isfinite(scale), "scale must be finite");
+  CBK_REQUIRE(table_width >= 0 && table_width < (int64_t(1) << 31) && table_stride >= 0,
+              "block table width out of range");
+  CBK_REQUIRE(kv->num_blocks < (int64_t(1) << 31), "num_blocks out of range");
+  int64_t max_len = table_width * kv->block_size;
+  Plan p;
+  if (int rc = plan_of(batch, rows, hq, hkv, max_len, &p)) return rc;
+  if (batch == 0) return CBK_OK;
+  CBK_REQUIRE(q_dev && out_dev && lens_dev && (tables_dev || table_width == 0), "NULL pointer");
+  const int64_t words[4] = {int64_t(reinterpret_cast<uintptr_t>(kv->k_base)),
+                            int64_t(reinterpret_cast<uintptr_t>(kv->v_base)), kv->block_stride, kv->token_stride};
+  const int vec = common_vec_bytes(words, 4);
+  CBK_REQUIRE(vec >= 4, "4-bit pages must be 4-byte aligned");
+  const size_t need = plan_bytes(p, rows, hq, head_dim);
+  if (workspace_dev == nullptr || workspace_bytes < need)
+    return set_error(CBK_ERR_WORKSPACE, "int4 attention workspace %zu < %zu bytes", workspace_bytes, need);
+  CBK_REQUIRE((reinterpret_cast<uintptr_t>(workspace_dev) & 255) == 0, "workspace must be 256-byte aligned");
+  Int4AttnArgs a;
+  a.q = q_dev;
+  a.out = out_dev;
+  a.q_batch = q_batch_stride;
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.out_batch = out_batch_stride;
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  a.k_base = static_cast<const char*>(kv->k_base);
+  a.v_base = static_cast<const char*>(kv->v_base);
+  a.block_stride = kv->block_stride;
+  a.token_stride = kv->token_stride;
+  a.tables = tables_dev;
+  a.table_stride = table_stride;
+  a.lens = lens_dev;
+  a.batch = uint32_t(batch);
+  a.rows = uint32_t(rows);
+  a.hq = uint32_t(hq);
+  a.hkv = uint32_t(hkv);
+  a.group = uint32_t(hq / hkv);
+  a.num_blocks = uint32_t(kv->num_blocks);
+  a.max_len = uint32_t(max_len);
+  a.row_tiles = p.row_tiles;
+  a.ranges = p.ranges;
+  a.scale = scale;
+  a.block_div = FastDiv::make(uint32_t(kv->block_size));
+  a.ml = static_cast<float2*>(workspace_dev);
+  a.o = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + ml_bytes(p, rows, hq));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool p16 = vec == 16;
+#define CBK_INT4_ATTN(DT) return head_dim == 128 ? launch<DT, 4>(a, p16, s) : launch<DT, 2>(a, p16, s);
+  switch (dtype) {
+    case CBK_DTYPE_F32: CBK_INT4_ATTN(CBK_DTYPE_F32)
+    case CBK_DTYPE_BF16: CBK_INT4_ATTN(CBK_DTYPE_BF16)
+    default: CBK_INT4_ATTN(CBK_DTYPE_F16)
+  }
+#undef CBK_INT4_ATTN
+}
+
+}  // extern "C"
