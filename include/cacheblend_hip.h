@@ -436,6 +436,32 @@ int cbk_blend_attention_ws(const void* q_dev, int64_t q_row_stride_elems, const 
                            void* workspace_dev, size_t workspace_bytes, cbk_stream_t stream);
 
 /*
+ * Causal attention of packed prompts: sequence s has the queries ends_q[s] ..
+ * ends_q[s + 1] of q [total_q, hq, head_dim] and the keys ends_k[s] ..
+ * ends_k[s + 1] of k, v [total_k, hkv, head_dim] (ends: [batch + 1] int32 on
+ * the device, rising; strides in elements). Its last query is its last key:
+ * query i sees keys k <= i + keys - queries of the sequence, and is zero where
+ * that is none:
+ *   out[i, h] = sum_k softmax_k( scale q[i, h] . key[k, h/G] ) value[k, h/G]
+ * with logits, softmax and sums in float32 (the softmax's terms enter the
+ * second product rounded to the inputs' type). Keys and values that a row does
+ * not see may hold anything. Rows of no sequence become zero (zero_outside) or
+ * stay as they are. head_dim 64 or 128; 16-byte aligned pointers and strides,
+ * K/V token strides below 2^24.
+ * workspace_dev: NULL, or 256-byte aligned scratch of at least what the
+ * _workspace_bytes function gives on the current device: launches whose tiles
+ * do not fill the GPU then split the keys and merge the parts.
+ */
+size_t cbk_prompt_attention_workspace_bytes(int64_t total_q, int64_t total_k, int64_t batch, int64_t hq, int64_t hkv,
+                                            int64_t head_dim, int32_t dtype);
+int cbk_prompt_attention(const void* q_dev, int64_t q_token_stride, int64_t q_head_stride, const void* k_dev,
+                         int64_t k_token_stride, int64_t k_head_stride, const void* v_dev, int64_t v_token_stride,
+                         int64_t v_head_stride, const int32_t* ends_q_dev, const int32_t* ends_k_dev, int64_t batch,
+                         int64_t total_q, int64_t total_k, int64_t hq, int64_t hkv, int64_t head_dim, float scale,
+                         int32_t dtype, void* out_dev, int64_t out_token_stride, int64_t out_head_stride,
+                         int32_t zero_outside, void* workspace_dev, size_t workspace_bytes, cbk_stream_t stream);
+
+/*
  * Attention of each sequence's latest tokens over its context in 4-bit pages
  * (cbk_paged_append's rows): q [batch, rows, hq, head_dim] (strides in
  * elements, dims contiguous), row r of sequence b the token at place len_b -

@@ -1,5 +1,5 @@
-"""Attention on MI355X: of the selected queries, and of single tokens over 4-bit
-pages.
+"""Attention on MI355X: of the selected queries, of packed prompts, and of single
+tokens over 4-bit pages.
 
 ``blend_attention`` keeps the signature of ``Qwen3BlendExecutor._attention``
 (cacheblend_vllm/ascend.py:798-846): queries ``[Nq, Hq, D]`` at absolute
@@ -98,6 +98,110 @@ def _check_out(out: torch.Tensor, query: torch.Tensor) -> None:
         if n > 1 and stride < span:
             raise ValueError("out rows must not overlap")
         span += (n - 1) * stride
+
+
+def _prompt_ends(ends: torch.Tensor, tokens: int, name: str, device: torch.device) -> torch.Tensor:
+    if ends.dim() != 1 or ends.numel() == 0:
+        raise ValueError(f"{name} must be [sequences + 1], got {tuple(ends.shape)}")
+    if ends.device.type == "cpu":
+        if int(ends[0]) < 0 or int(ends[-1]) > tokens or bool((ends[1:] < ends[:-1]).any()):
+            raise IndexError(f"{name} must rise within the {tokens} tokens")
+    return _whole_int32(ends, device).contiguous()
+
+
+def _pieces(t: torch.Tensor, es: int, strided: bool = False) -> bool:
+    """16-byte aligned rows of whole dims; ``strided``: tokens within 2^24 elements."""
+    return (t.stride(2) == 1 and (t.data_ptr() | t.stride(0) * es | t.stride(1) * es) % 16 == 0
+            and not (strided and t.stride(0) >= 1 << 24))
+
+
+def prompt_attention(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    scale: float,
+    cu_seqlens_k: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal attention of packed prompts: a prefill.
+
+    ``query`` ``[tokens, q_heads, head_size]``, ``key`` and ``value`` ``[tokens,
+    kv_heads, head_size]`` hold the sequences one after another, sequence ``s`` from
+    ``cu_seqlens[s]`` to ``cu_seqlens[s + 1]`` (with ``cu_seqlens_k``, keys and values
+    from ``cu_seqlens_k[s]`` to ``cu_seqlens_k[s + 1]``). A sequence's last query is its
+    last key: with more keys than queries the first keys are context from before
+    (a chunk of a longer prompt), with fewer the first queries see nothing and are
+    zero. Head sizes 64 and 128; logits, softmax and sums in float32.
+
+    Tokens before the first sequence and behind the last (padding) are zero in a
+    new output and left as they are in ``out``. What a query does not see may hold
+    anything, infinities and NaN among it. Rows that are not 16-byte aligned are
+    copied first.
+
+    ``cu_seqlens`` on the host is checked (``IndexError``); on the device it is not
+    read back: ends past the tensors are taken as their end.
+    """
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        _native.require_device(t, name)
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [tokens, heads, head_size]")
+    total, hq, d = query.shape
+    total_k, hkv, dk = key.shape
+    if value.shape != key.shape or dk != d:
+        raise ValueError("key/value shapes do not match the query head size")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise ValueError("query, key and value must share a dtype")
+    device = query.device
+    if key.device != device or value.device != device:
+        raise ValueError("query, key and value must share a device")
+    if query.dtype not in _native.DTYPE_CODES:
+        raise ValueError(f"dtype {query.dtype} is not supported")
+    if d not in (64, 128):
+        raise ValueError(f"head size {d}: 64 or 128 supported")
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError(f"query heads ({hq}) must be divisible by KV heads ({hkv})")
+    if cu_seqlens_k is None and total_k != total:
+        raise ValueError(f"{total_k} keys for {total} queries need cu_seqlens_k")
+    ends_q = _prompt_ends(cu_seqlens, total, "cu_seqlens", device)
+    ends_k = ends_q if cu_seqlens_k is None else _prompt_ends(cu_seqlens_k, total_k, "cu_seqlens_k", device)
+    batch = ends_q.numel() - 1
+    if ends_k.numel() != batch + 1:
+        raise ValueError(f"{ends_k.numel()} ends of keys for {batch + 1} of queries")
+    fresh = out is None
+    if fresh:
+        out = torch.empty((total, hq, d), dtype=query.dtype, device=device)
+    else:
+        _check_out(out, query)
+    if total == 0 or batch == 0:
+        return out.zero_() if fresh else out
+    es = query.element_size()
+    copied = {"memory_format": torch.contiguous_format}
+    q = query if _pieces(query, es) else query.clone(**copied)
+    k = key if _pieces(key, es, True) else key.clone(**copied)
+    v = value if _pieces(value, es, True) else value.clone(**copied)
+    o = out if _pieces(out, es) else out.clone(**copied)
+    lib = _native.load()
+    # partial results of the keys' ranges, from torch's allocator on every
+    # call: a captured graph then owns its own
+    code = _native.DTYPE_CODES[query.dtype]
+    nbytes = _native.on_device(device, lib.cbk_prompt_attention_workspace_bytes, total, total_k, batch, hq, hkv, d, code)
+    ws = None
+    if nbytes:
+        try:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        except torch.cuda.OutOfMemoryError:
+            nbytes = 0  # one range, which needs no scratch
+    rc = _native.on_device(
+        device, lib.cbk_prompt_attention, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+        v.data_ptr(), v.stride(0), v.stride(1), ends_q.data_ptr(), ends_k.data_ptr(), batch, total, total_k, hq, hkv, d,
+        float(scale), code, o.data_ptr(), o.stride(0), o.stride(1), int(fresh), _native.ptr(ws), nbytes,
+        _native.stream_handle(device),
+    )
+    _native.check(rc, "prompt_attention")
+    if o is not out:
+        out.copy_(o)
+    return out
 
 
 def paged_attention_int4(

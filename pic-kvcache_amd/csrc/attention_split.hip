@@ -29,7 +29,8 @@ template <> __device__ __forceinline__ __half to_out<__half>(float v) { return _
 template <typename T, int N>
 __global__ __launch_bounds__(kMergeThreads) void attn_merge_kernel(const AttnParts parts, uint32_t nq, uint32_t hq,
                                                                    uint32_t d, const int64_t* pos, T* out,
-                                                                   int64_t out_stride, bool nan_empty) {
+                                                                   int64_t out_stride, int64_t head_stride,
+                                                                   bool nan_empty, const AttnSpan span) {
   constexpr int E = N ? N : 4;  // d <= 128
   constexpr bool F32 = sizeof(T) == 4;
   typedef float VecN __attribute__((ext_vector_type(E)));
@@ -37,7 +38,13 @@ __global__ __launch_bounds__(kMergeThreads) void attn_merge_kernel(const AttnPar
   const uint64_t rows = uint64_t(nq) * hq;
   const uint64_t row = uint64_t(blockIdx.x) * (kMergeThreads / 32) + (threadIdx.x >> 5);
   if (row >= rows) return;  // both halves' exchanges stay within their 32 lanes
-  const uint32_t S = parts.splits;
+  const uint32_t q = uint32_t(row / hq), h = uint32_t(row - uint64_t(q) * hq);
+  bool inside = true;
+  if (span.ends != nullptr) {  // uniform within the row's 32 lanes
+    inside = int64_t(q) >= span.ends[0] && int64_t(q) < span.ends[span.batch];
+    if (!inside && !span.zero_outside) return;
+  }
+  const uint32_t S = inside ? parts.splits : 0u;
   const float2 ml = lane < S ? parts.ml[lane * rows + row] : make_float2(-__builtin_inff(), 0.f);
   float m = ml.x;
 #pragma unroll
@@ -70,10 +77,9 @@ __global__ __launch_bounds__(kMergeThreads) void attn_merge_kernel(const AttnPar
         if (used && lane + 32 * e < d) acc[e] = fmaf(ws, o[s * rows * d + lane + 32 * e], acc[e]);
     }
   }
-  const uint32_t q = uint32_t(row / hq), h = uint32_t(row - uint64_t(q) * hq);
   const float empty = nan_empty && pos[q] >= 0 ? __uint_as_float(0x7fc00000u) : 0.f;
   const float inv = 1.f / l;
-  T* dst = out + int64_t(q) * out_stride + int64_t(h) * d;
+  T* dst = out + int64_t(q) * out_stride + int64_t(h) * head_stride;
   T res[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) res[e] = to_out<T>(l == 0.f ? empty : acc[e] * inv);
@@ -89,13 +95,13 @@ __global__ __launch_bounds__(kMergeThreads) void attn_merge_kernel(const AttnPar
 
 template <typename T>
 int launch_merge_t(const AttnParts& parts, uint32_t nq, uint32_t hq, uint32_t d, const int64_t* pos, T* out,
-                   int64_t out_stride, bool nan_empty, hipStream_t stream) {
+                   int64_t out_stride, int64_t head_stride, bool nan_empty, const AttnSpan& span, hipStream_t stream) {
   constexpr uint64_t kRows = kMergeThreads / 32;
   const dim3 grid(uint32_t((uint64_t(nq) * hq + kRows - 1) / kRows));
-  const bool aligned = out_stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
+  const bool aligned = out_stride % 4 == 0 && head_stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
 #define CBK_MERGE(N)                                                                                             \
   hipLaunchKernelGGL((attn_merge_kernel<T, N>), grid, dim3(kMergeThreads), 0, stream, parts, nq, hq, d, pos, out, \
-                     out_stride, nan_empty)
+                     out_stride, head_stride, nan_empty, span)
   if (d == 128 && aligned) CBK_MERGE(4);
   else if (d == 64 && aligned) CBK_MERGE(2);
   else CBK_MERGE(0);
@@ -157,14 +163,16 @@ AttnParts attn_parts(uint32_t splits, uint64_t rows, void* workspace) {
 }
 
 int launch_attn_merge(const AttnParts& parts, uint32_t nq, uint32_t hq, uint32_t d, const int64_t* pos, void* out,
-                      int64_t out_stride, int32_t dtype, bool nan_empty, hipStream_t stream) {
+                      int64_t out_stride, int32_t dtype, bool nan_empty, hipStream_t stream, int64_t out_head_stride,
+                      AttnSpan span) {
+  const int64_t hs = out_head_stride ? out_head_stride : int64_t(d);
   switch (dtype) {
     case CBK_DTYPE_F32:
-      return launch_merge_t(parts, nq, hq, d, pos, static_cast<float*>(out), out_stride, nan_empty, stream);
+      return launch_merge_t(parts, nq, hq, d, pos, static_cast<float*>(out), out_stride, hs, nan_empty, span, stream);
     case CBK_DTYPE_BF16:
-      return launch_merge_t(parts, nq, hq, d, pos, static_cast<__hip_bfloat16*>(out), out_stride, nan_empty, stream);
+      return launch_merge_t(parts, nq, hq, d, pos, static_cast<__hip_bfloat16*>(out), out_stride, hs, nan_empty, span, stream);
     default:
-      return launch_merge_t(parts, nq, hq, d, pos, static_cast<__half*>(out), out_stride, nan_empty, stream);
+      return launch_merge_t(parts, nq, hq, d, pos, static_cast<__half*>(out), out_stride, hs, nan_empty, span, stream);
   }
 }
 

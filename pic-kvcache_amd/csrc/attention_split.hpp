@@ -52,11 +52,21 @@ uint32_t attn_splits(uint64_t groups, uint64_t rows, int64_t nk, int64_t d);
 size_t attn_parts_bytes(uint32_t splits, uint64_t rows, int64_t d);
 AttnParts attn_parts(uint32_t splits, uint64_t rows, void* workspace);
 
+// Packed sequences: only queries ends[0] .. ends[batch] have partial results;
+// the others' rows become zero, or stay as they are.
+struct AttnSpan {
+  const int32_t* ends;  // NULL: every query has
+  uint32_t batch;
+  bool zero_outside;
+};
+
 // out[r] = the merged rows, in `dtype`; a row without visible keys (position
 // below 0) is zero. nan_empty: a row whose visible keys all have a logit of
-// -inf is NaN, as its softmax is; zero otherwise.
+// -inf is NaN, as its softmax is; zero otherwise (then pos may be NULL).
+// Strides in elements, heads out_head_stride apart (0: d).
 int launch_attn_merge(const AttnParts& parts, uint32_t nq, uint32_t hq, uint32_t d, const int64_t* pos, void* out,
-                      int64_t out_stride, int32_t dtype, bool nan_empty, hipStream_t stream);
+                      int64_t out_stride, int32_t dtype, bool nan_empty, hipStream_t stream,
+                      int64_t out_head_stride = 0, AttnSpan span = AttnSpan{nullptr, 0, false});
 
 struct AttnF32Args {
   const float* q;

@@ -1,0 +1,165 @@
+// Packed prompts: the arguments of their attention, and which sequence and row
+// tile a workgroup has.
+#pragma once
+
+#include "attention_split.hpp"
+
+namespace cbk {
+
+struct PromptArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  // elements
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  const int32_t* ends_q;  // [batch + 1]: sequence s has the queries ends_q[s] .. ends_q[s + 1]
+  const int32_t* ends_k;
+  uint32_t batch, total_q, total_k;
+  uint32_t element;  // bytes
+  uint32_t hq, hkv, group;
+  FastDiv group_div;
+  float scale;
+  bool zero_outside;  // rows of no sequence become zero, instead of staying as they are
+  AttnParts parts;
+};
+
+// Row tiles of `rows` (query, group head) rows that any lengths can need, and
+// one more: past the last tile workgroups have the rows of no sequence.
+inline uint64_t prompt_tiles(const PromptArgs& a, uint32_t rows) {
+  return uint64_t(a.total_q) * a.group / rows + a.batch + 1;
+}
+
+int launch_prompt_f32(const PromptArgs& a, uint32_t d, hipStream_t stream);
+
+struct PromptTile {
+  uint32_t q0, nq, k0, nk;  // of the sequence
+  uint32_t tile;            // of its rows
+  uint32_t beyond;          // > 0: no tile, the beyond-th such rank of `without`
+  uint32_t without;
+};
+
+#ifdef __HIPCC__
+
+struct PromptSeq {
+  uint32_t q0, nq, k0, nk;
+};
+
+// Sequence s; ends that do not rise, or past the tensors, are taken as if they
+// stopped there.
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptArgs& a, uint32_t s) {
+  auto at = [](int32_t x, uint32_t total) { return min(uint32_t(max(x, 0)), total); };
+  PromptSeq r;
+  r.q0 = at(a.ends_q[s], a.total_q);
+  r.nq = max(at(a.ends_q[s + 1], a.total_q), r.q0) - r.q0;
+  r.k0 = at(a.ends_k[s], a.total_k);
+  r.nk = max(at(a.ends_k[s + 1], a.total_k), r.k0) - r.k0;
+  return r;
+}
+
+// The rank-th tile in the order of the tiles' levels, highest first: a
+// tile's level counts the tiles of rows up to its last key, so that tiles with
+// about as many keys share one, whatever their sequences. Within a level the
+// sequences are in their order. By a whole wave, every wave of a workgroup the
+// same.
+template <uint32_t ROWS>
+__device__ PromptTile prompt_tile(const PromptArgs& a, uint32_t rank, uint32_t lane) {
+  // of sequence s (none: no tiles): its lowest level, and one past its highest
+  auto levels = [&](uint32_t s, uint32_t& lo, uint32_t& hi) __attribute__((always_inline)) {
+    lo = hi = 0;
+    if (s >= a.batch) return;
+    const PromptSeq q = prompt_seq(a, s);
+    lo = q.nk > q.nq ? uint32_t(min(uint64_t(q.nk - q.nq) * a.group / ROWS, uint64_t(1) << 30)) : 0u;
+    hi = lo + (q.nq * a.group + ROWS - 1) / ROWS;
+  };
+  auto total = [](uint32_t v) {
+    return uint32_t(__builtin_amdgcn_readlane(int(wave_inclusive_scan(v)), 63));
+  };
+  uint32_t lo0, hi0;  // the first 64 sequences' stay in registers
+  levels(lane, lo0, hi0);
+  const uint32_t rounds = (a.batch + 63) / 64;
+  auto at_least = [&](uint32_t level) __attribute__((always_inline)) {  // tiles of this level or above
+    uint32_t n = hi0 - min(max(level, lo0), hi0);
+    for (uint32_t r = 1; r < rounds; ++r) {
+      uint32_t lo, hi;
+      levels(64 * r + lane, lo, hi);
+      n += hi - min(max(level, lo), hi);
+    }
+    return total(n);
+  };
+  PromptTile t;
+  const uint32_t all = at_least(0);
+  t.beyond = rank >= all ? rank - all + 1 : 0u;
+  t.without = gridDim.x / (a.hkv * a.parts.splits) - all;
+  t.q0 = t.nq = t.k0 = t.nk = t.tile = 0;
+  if (t.beyond) return t;
+  // the highest level with more than `rank` tiles from it on
+  uint32_t low = 0, high = 0;
+  {
+    uint32_t top = hi0;
+    for (uint32_t r = 1; r < rounds; ++r) {
+      uint32_t lo, hi;
+      levels(64 * r + lane, lo, hi);
+      top = max(top, hi);
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), off)));
+    high = __builtin_amdgcn_readfirstlane(top);
+  }
+  if (a.batch == 1) {  // one sequence: the ranks are its levels
+    low = high - 1 - rank;
+  } else {
+    while (high - low > 1) {  // at_least(low) > rank >= at_least(high)
+      const uint32_t mid = (low + high) / 2;
+      if (at_least(mid) > rank) low = mid;
+      else high = mid;
+    }
+  }
+  uint32_t index = rank - (a.batch == 1 ? rank : at_least(low + 1));  // within the level
+  uint32_t seq = 0;
+  for (uint32_t r = 0; r < rounds; ++r) {
+    uint32_t lo = lo0, hi = hi0;
+    if (r > 0) levels(64 * r + lane, lo, hi);
+    const bool has = lo <= low && low < hi;
+    const uint64_t mask = __ballot(has);
+    const uint32_t here = uint32_t(__popcll(mask));
+    if (index < here) {
+      const bool mine = has && uint32_t(__popcll(mask & ((uint64_t(1) << lane) - 1))) == index;
+      const int from = __builtin_ctzll(__ballot(mine));
+      seq = 64 * r + uint32_t(from);
+      t.tile = __builtin_amdgcn_readfirstlane(low - uint32_t(__shfl(int(lo), from)));
+      break;
+    }
+    index -= here;
+  }
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  const PromptSeq q = prompt_seq(a, seq);
+  t.q0 = __builtin_amdgcn_readfirstlane(q.q0);
+  t.nq = __builtin_amdgcn_readfirstlane(q.nq);
+  t.k0 = __builtin_amdgcn_readfirstlane(q.k0);
+  t.nk = __builtin_amdgcn_readfirstlane(q.nk);
+  return t;
+}
+
+// Zeroes the rows of no sequence, before the first and behind the last: the
+// workgroups without a tile share them, each the heads of its KV head. `row`:
+// bytes of a head's row, whole 16-byte pieces.
+__device__ __forceinline__ void prompt_outside(const PromptArgs& a, const PromptTile& t, uint32_t kvh, uint32_t row) {
+  if (!a.zero_outside) return;
+  const uint32_t first = min(uint32_t(max(a.ends_q[0], 0)), a.total_q);
+  const uint32_t behind = max(min(uint32_t(max(a.ends_q[a.batch], 0)), a.total_q), first);
+  const uint32_t per = row / 16, es = a.element;
+  const uint64_t n = uint64_t(first + (a.total_q - behind)) * a.group * per;
+  for (uint64_t i = uint64_t(t.beyond - 1) * blockDim.x + threadIdx.x; i < n; i += uint64_t(t.without) * blockDim.x) {
+    const uint64_t r = i / per;
+    const uint32_t piece = uint32_t(i - r * per), at = uint32_t(r / a.group), h = uint32_t(r - uint64_t(at) * a.group);
+    const uint32_t token = at < first ? at : behind + (at - first);
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    char* dst = static_cast<char*>(a.out) + (int64_t(token) * a.out_token + int64_t(kvh * a.group + h) * a.out_head) * es;
+    reinterpret_cast<u32x4*>(dst)[piece] = u32x4(0u);
+  }
+}
+
+#endif
+
+}  // namespace cbk

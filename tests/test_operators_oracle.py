@@ -166,3 +166,44 @@ def test_int4_gather_entry_refuses(args, word):
     desc = _native.KVDesc(0x10000, 0x20000, 8, 16, 16 * 160, 160, 160)
     assert lib.cbk_paged_gather_int4(desc, *args, None) == _native.CBK_ERR_INVALID
     assert word in lib.cbk_last_error(), lib.cbk_last_error()
+
+
+def _decode(lib, desc, **over):
+    a = dict(q=0x1000, qb=512, qr=512, qh=128, batch=2, rows=1, hq=4, kv=desc, hkv=2, dim=128, tables=0x2000, ts=4, width=4,
+             lens=0x3000, scale=0.1, dtype=1, out=0x4000, ob=512, orow=512, oh=128, ws=0x10000, nbytes=1 << 40, stream=None)
+    a.update(over)
+    return lib.cbk_paged_attention_int4(*a.values())
+
+
+@pytest.mark.parametrize("over,word", [
+    (dict(dtype=4), b"dtype"), (dict(dim=96), b"64 or 128"), (dict(hkv=3), b"4-bit row"), (dict(scale=float("nan")), b"finite"),
+    (dict(width=-1), b"width"), (dict(hq=5), b"divisible"), (dict(rows=0), b"rows"), (dict(batch=-1), b"batch"),
+    (dict(batch=1 << 16), b"batch"), (dict(width=1 << 28, ts=1 << 28), b"context"),
+])
+def test_int4_attention_entry_refuses(over, word):
+    lib = _native.load()
+    desc = _native.KVDesc(0x10000, 0x20000, 8, 16, 16 * 160, 160, 160)
+    assert _decode(lib, desc, **over) == _native.CBK_ERR_INVALID
+    assert word in lib.cbk_last_error(), lib.cbk_last_error()
+
+
+def _prompt(lib, **over):
+    a = dict(q=0x1000, qt=512, qh=128, k=0x2000, kt=256, kh=128, v=0x3000, vt=256, vh=128, ends_q=0x100, ends_k=0x200,
+             batch=2, total_q=10, total_k=10, hq=4, hkv=2, dim=128, scale=0.1, dtype=1, out=0x4000, ot=512, oh=128, zero=1,
+             ws=None, nbytes=0, stream=None)
+    a.update(over)
+    return lib.cbk_prompt_attention(*a.values())
+
+
+@pytest.mark.parametrize("over,word", [
+    (dict(dtype=3), b"dtype"), (dict(dim=80), b"64 or 128"), (dict(hq=3), b"divisible"), (dict(total_q=-1), b"tokens"),
+    (dict(total_k=1 << 30), b"tokens"), (dict(batch=-1), b"batch"), (dict(batch=0), b"without a sequence"),
+    (dict(q=None), b"NULL"), (dict(k=None), b"NULL"), (dict(ends_q=None), b"NULL"), (dict(out=None), b"NULL"),
+    (dict(scale=float("inf")), b"finite"), (dict(q=0x1008), b"16-byte"), (dict(vt=260), b"16-byte"), (dict(oh=132), b"16-byte"),
+    (dict(kt=1 << 24), b"2^24"), (dict(total_q=1 << 29, hq=8, hkv=2), b"too large"),
+])
+def test_prompt_entry_refuses(over, word):
+    lib = _native.load()
+    assert _prompt(lib, **over) == _native.CBK_ERR_INVALID
+    assert word in lib.cbk_last_error(), lib.cbk_last_error()
+    assert _prompt(lib, total_q=0) == _native.CBK_OK
