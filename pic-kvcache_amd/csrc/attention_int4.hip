@@ -15,10 +15,14 @@
 //
 // so the inner sums are v_mfma_f32_16x16x32_bf16 products of small whole
 // numbers, exact in bf16, made from the codes by one and-or per two: 0x4300 | n
-// is 128 + n, and 128 times the other operand's sum is taken off again (for
-// float32 the codes are converted, without the 128). The other operand is cut
-// into bf16 parts: q exactly (one part for bf16, two for f16, three for
-// float32), p step into two (2^-15 of it is lost) or three.
+// is 128 + n, and 128 times the other operand's sum is taken off again: before
+// the first product of q, and by a product with -128 after each of p, so that
+// the running sums stay small. (For float32 the codes are converted, to n - 8
+// for the values: the two sums of out_d then do not cancel.) The other operand
+// is cut into bf16 parts: q exactly (one part for bf16, two for f16, three for
+// float32), p step into two or three, the last rounded to nearest (2^-16, 2^-23
+// of it; cut off instead it would be a bias, which a long context's sums of
+// both signs do not forgive).
 //
 // A wave takes 64 keys of one KV head at a time, K and V rows staged in its own
 // LDS by DMA (K two tiles ahead, V one: no barrier in the loop), and 16 columns of S^T =
@@ -120,13 +124,13 @@ __device__ __forceinline__ void lds_dma(const char* addr, uint32_t lds) {
 }
 
 // 8 codes of a word as the 8 bf16 of an MFMA operand, in the order 0 4 1 5 2 6
-// 3 7: as 128 + n, or (EXACT) as n.
-template <bool EXACT>
+// 3 7: as 128 + n, or (EXACT) as n - LESS.
+template <bool EXACT, int LESS = 0>
 __device__ __forceinline__ s16x8 operand(uint32_t w) {
   u32x4 r;
   if constexpr (EXACT) {
     const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6, 1 3 5 7
-    auto f = [](uint32_t x, int byte) { return __float_as_uint(float((x >> (8 * byte)) & 0xffu)); };
+    auto f = [](uint32_t x, int byte) { return __float_as_uint(float((x >> (8 * byte)) & 0xffu) - float(LESS)); };
     auto pair = [](uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); };
     r[0] = pair(f(even, 0), f(even, 2));
     r[1] = pair(f(odd, 0), f(odd, 2));
@@ -137,6 +141,13 @@ __device__ __forceinline__ s16x8 operand(uint32_t w) {
     for (int i = 0; i < 4; ++i) r[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
   }
   return __builtin_bit_cast(s16x8, r);
+}
+
+// two floats rounded to bf16, x in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x, y}, b2));
 }
 
 template <int DT> __device__ __forceinline__ float load_elem(const void* p, int64_t at);
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
   const float sign = a.scale < 0.f ? -1.f : 1.f, c2 = fabsf(a.scale) * kLog2e;
   const uint32_t lds0 = lds_address(&lds[wave][0]), pages0 = lds_address(&s_pages[wave][0][0]);
   // the selector that puts a float's upper half into the low (tile even) or high half of a word
-  const uint32_t place = v ? 0x03020c0cu : 0x0c0c0302u;
+  const uint32_t place = v ? 0x03020c0cu : 0x0c0c0302u, half = v ? 0xffff0000u : 0x0000ffffu;
 
   for (bool first_seq = true; at < end; first_seq = false) {
     uint32_t len = context_of(a, seq);
@@ -260,11 +271,11 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
     }
 
     float m = kNegInf, l = 0.f, zsum[NG];
-    f32x4 o[2 * NG], ones[NG];
+    f32x4 o[2 * NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       zsum[g] = 0.f;
-      ones[g] = o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
     // The block table's entries of tile i's keys, by DMA; from them where the
@@ -395,7 +406,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
             for (int r = 0; r < 4; ++r) {
               o[2 * g][r] *= ao[r];
               o[2 * g + 1][r] *= ao[r];
-              ones[g][r] *= ao[r];
             }
           }
         }
@@ -415,7 +425,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
         // in bf16 parts, operand word r key r of the first tile in its low half,
         // of the second in its high half
         const uint32_t from = (16 * (c >> 2) + 4 * j + (c & 3)) * RB;  // the row of key 16 j + c
-        const s16x8 one = __builtin_bit_cast(s16x8, u32x4(0x3f803f80u));
+        const s16x8 less = __builtin_bit_cast(s16x8, u32x4(0xc300c300u));  // -128
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           __builtin_amdgcn_sched_barrier(0);
@@ -432,21 +442,23 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
               for (int g = 0; g < NG; ++g) {
                 const uint32_t word = sees ? sw[g] : 0u;  // a masked key's step and offset may be anything
                 y[g][t] = x[u][r] * __uint_as_float(word << 16);
-                zsum[g] = fmaf(x[u][r], __uint_as_float(word & 0xffff0000u), zsum[g]);
+                float z = __uint_as_float(word & 0xffff0000u);
+                if constexpr (EXACT) z = fmaf(8.f, __uint_as_float(word << 16), z);
+                zsum[g] = fmaf(x[u][r], z, zsum[g]);
               }
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
               for (int q = 0; q < PP; ++q) {
-                if constexpr (VT == 1) {
-                  pw[g][q][r] = __builtin_amdgcn_perm(__float_as_uint(y[g][1]), __float_as_uint(y[g][0]), 0x07060302u);
-                } else {
-                  pw[g][q][r] = __builtin_amdgcn_perm(0u, __float_as_uint(y[g][0]), place);
-                }
-                if (q + 1 < PP)
+                if (q + 1 < PP) {  // the upper halves, and what is left
+                  pw[g][q][r] = VT == 1 ? __builtin_amdgcn_perm(__float_as_uint(y[g][2 / VT - 1]), __float_as_uint(y[g][0]), 0x07060302u)
+                                        : __builtin_amdgcn_perm(0u, __float_as_uint(y[g][0]), place);
 #pragma unroll
                   for (int t = 0; t < 2 / VT; ++t) y[g][t] -= __uint_as_float(__float_as_uint(y[g][t]) & 0xffff0000u);
+                } else {
+                  pw[g][q][r] = pack_bf16(y[g][0], y[g][2 / VT - 1]) & (VT == 1 ? 0xffffffffu : half);
+                }
               }
           }
 #pragma unroll
@@ -455,15 +467,15 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
             for (int d = 0; d < 2; ++d) {
               const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
                   (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) const void*)(vb + from + 16 * g + 8 * d)));
-              const s16x8 vf = operand<EXACT>(uint32_t(w[h]));
+              const s16x8 vf = operand<EXACT, 8>(uint32_t(w[h]));
 #pragma unroll
               for (int q = 0; q < PP; ++q)
-                o[2 * g + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(s16x8, pw[g][q]), vf, o[2 * g + d], 0, 0, 0);
+              {
+                const s16x8 pf = __builtin_bit_cast(s16x8, pw[g][q]);
+                o[2 * g + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, vf, o[2 * g + d], 0, 0, 0);
+                if constexpr (!EXACT) o[2 * g + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, less, o[2 * g + d], 0, 0, 0);
+              }
             }
-            if constexpr (!EXACT)
-#pragma unroll
-              for (int q = 0; q < PP; ++q)
-                ones[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(s16x8, pw[g][q]), one, ones[g], 0, 0, 0);
           }
         }
       };
@@ -494,7 +506,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float z = __shfl(zsum[g], int(4 * j + r)) - (EXACT ? 0.f : 128.f * ones[g][r]);
+        const float z = __shfl(zsum[g], int(4 * j + r));
 #pragma unroll
         for (int d = 0; d < 2; ++d) mine[(4 * j + r) * D + 32 * g + 16 * d + c] = o[2 * g + d][r] + z;
       }
