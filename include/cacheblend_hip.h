@@ -476,7 +476,7 @@ int cbk_prompt_attention(const void* q_dev, int64_t q_token_stride, int64_t q_he
  * function gives on the current device, max_len = table_width * block_size.
  */
 size_t cbk_paged_attention_int4_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
-                                                int64_t max_len);
+                                                int64_t max_len, int32_t dtype);
 int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
                              int64_t batch, int64_t rows, int64_t hq, const cbk_kv_desc* kv, int64_t hkv,
                              int64_t head_dim, const int32_t* tables_dev, int64_t table_stride, int64_t table_width,

@@ -172,7 +172,7 @@ _SIGNATURES = {
         [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
          c_i64, ctypes.c_float, c_i32, c_vp, c_i64, c_i64, c_i32, c_vp, ctypes.c_size_t, c_vp],
     ),
-    "cbk_paged_attention_int4_workspace_bytes": (ctypes.c_size_t, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "cbk_paged_attention_int4_workspace_bytes": (ctypes.c_size_t, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i32]),
     "cbk_paged_attention_int4": (
         ctypes.c_int,
         [c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(KVDesc), c_i64, c_i64, c_vp, c_i64, c_i64,

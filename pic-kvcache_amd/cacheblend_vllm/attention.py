@@ -273,7 +273,7 @@ def paged_attention_int4(
     o = out if out.dim() == 4 else out.unsqueeze(1)
     lib = _native.load()
     nbytes = _native.on_device(device, lib.cbk_paged_attention_int4_workspace_bytes, batch, rows, hq, hkv, d,
-                               width * block_size)
+                               width * block_size, _native.DTYPE_CODES[query.dtype])
     # from torch's allocator on every call: a captured graph then owns its own
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     rc = _native.on_device(

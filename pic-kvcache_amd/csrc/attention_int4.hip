@@ -24,21 +24,28 @@
 // of it; cut off instead it would be a bias, which a long context's sums of
 // both signs do not forgive).
 //
-// A wave takes 64 keys of one KV head at a time, K and V rows staged in its own
-// LDS by DMA (K two tiles ahead, V one: no barrier in the loop), and 16 columns of S^T =
-// K . Q^T: VT column groups of 16 / VT rows each, for the rows of the group
-// are often fewer than 16. The Q operand of a 16-key tile is zero outside the
-// tile's column group, so VT tiles share an accumulator and the softmax's work
-// on the VALU is spread over all columns.
-// Tile t's row m is key 16 (m / 4) + 4 t + m % 4 of the 64, so that lane (j =
-// lane / 16, c) holds, over the four tiles, keys 16 j .. 16 j + 15: those whose
-// codes of one dim a ds_read_tr4_b64 hands to lane group j.
+// A wave takes 32 keys of one KV head at a time, their K and V rows staged in
+// its own LDS by DMA two tiles ahead (no barrier in the loop), and 16 columns of
+// S^T = K . Q^T: VT column groups of 16 / VT rows each, for the rows of the
+// group are often fewer than 16. The Q operand of a 16-key half is zero outside
+// the half's column group, so VT 2 gives both halves one accumulator, and the
+// softmax's work on the VALU half the columns. Half t's row m is key 8 (m / 4) +
+// 4 t + m % 4 of the 32, so that lane (j = lane / 16, c) holds, over the two
+// halves, keys 8 j .. 8 j + 7: those of lane group j in the second product, whose
+// codes a ds_read_tr4_b64 hands out, of 16 dims in its first word (from the
+// rows that lanes 0 to 7 address) and of the next 16 in its second (lanes 8 to
+// 15, the same rows, 8 bytes on).
 //
-// The sequences' 64-key tiles, one after another, are cut into as many equal
-// ranges as fill the GPU; a workgroup takes one range of one KV head (and row
-// tile), its four waves every fourth tile, whatever sequences they belong to.
-// A sequence that one range holds whole is written at once, the others'
-// partial results are merged by a second launch.
+// The sequences' 32-key tiles, one after another, are cut into as many equal
+// ranges as fill the GPU, whatever sequences they belong to; a workgroup takes
+// one range and up to 8 KV heads (of one row tile), a wave a head: neighbouring
+// heads' rows share cache lines, and side by side the waves ask for them at the
+// same time. (With a workgroup a head, on one XCD, the heads drifted apart, L2
+// fetched 1.6 GB for 0.83 of pages, and 64 sequences of up to 16K keys took 255
+// us whatever the work per key.) With fewer heads several waves of a head take
+// its tiles in turn. A sequence that one range holds whole is written at once,
+// the others' partial results are merged by a second launch.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -53,9 +60,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kTile = 64;      // keys of a wave's step
+constexpr int kMergeThreads = 256;
+constexpr int kTile = 32;   // keys of a wave's step
+constexpr int kStages = 3;  // tiles in a wave's LDS
+// waves of a workgroup, at most (float32 takes the registers of 8 with 4)
+constexpr int max_waves(int32_t dtype) { return dtype == CBK_DTYPE_F32 ? 4 : 8; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kRescale = 8.f;  // log2 headroom before the reference maximum is raised
@@ -75,7 +84,9 @@ struct Int4AttnArgs {
   uint32_t num_blocks, max_len;
   uint32_t row_tiles;                    // of 16 / VT (row, head of the group) pairs
   uint32_t ranges;
+  uint32_t heads, turns;                 // of a workgroup: KV heads, and waves that share one's tiles
   float scale;
+  bool q_pieces;                         // 16-byte pieces of q are aligned
   FastDiv block_div;
   // partial results of range r's first (0) and last (1) unfinished sequence:
   // entry ((2 r + which) hkv + kv head) * rows * group + row * group + head
@@ -108,27 +119,47 @@ __device__ uint32_t total_tiles(const Int4AttnArgs& a, uint32_t lane) {
 }
 
 // LDS DMA from a 64-bit address per lane (the rows of pages anywhere): lane
-// l's 16 or 4 bytes land at lds + l * size. M0 and its waits as CBK_LDS_DMA's.
-#define CBK_LDS_DMA64(op)                                                                        \
-  "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 4\n\t" op " %1, off\n\ts_nop 0\n\ts_mov_b32 m0, %0"
-template <int PIECE>
-__device__ __forceinline__ void lds_dma(const char* addr, uint32_t lds) {
-  uint32_t saved;
-  if constexpr (PIECE == 16) {
-    asm volatile(CBK_LDS_DMA64("global_load_lds_dwordx4")
-                 : "=&s"(saved) : "v"(addr), "s"(__builtin_amdgcn_readfirstlane(int(lds))) : "memory");
-  } else {
-    asm volatile(CBK_LDS_DMA64("global_load_lds_dword")
-                 : "=&s"(saved) : "v"(addr), "s"(__builtin_amdgcn_readfirstlane(int(lds))) : "memory");
+// l's 16 or 4 bytes land at lds + l * size, N requests' one after another. M0
+// and its waits as CBK_LDS_DMA's; lds wave-uniform.
+#define CBK_LDS_FIRST(op, addr) "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\t" op " " addr ", off\n\t"
+#define CBK_LDS_NEXT(op, step, addr) "s_nop 0\n\ts_add_u32 m0, m0, " step "\n\ts_nop 0\n\t" op " " addr ", off\n\t"
+#define CBK_LDS_LAST "s_nop 0\n\ts_mov_b32 m0, %0"
+template <int PIECE, int N>
+__device__ __forceinline__ void lds_dma(const char* base, const uint64_t (&off)[N], uint32_t lds) {
+  static_assert(N % 5 == 0, "requests in fives");
+#pragma unroll
+  for (int n = 0; n < N; n += 5) {
+    uint32_t saved;
+    const char* const p[5] = {base + off[n], base + off[n + 1], base + off[n + 2], base + off[n + 3], base + off[n + 4]};
+    const uint32_t to = __builtin_amdgcn_readfirstlane(int(lds + n * 64 * PIECE));
+    if constexpr (PIECE == 16) {
+      asm volatile(CBK_LDS_FIRST("global_load_lds_dwordx4", "%2") CBK_LDS_NEXT("global_load_lds_dwordx4", "0x400", "%3")
+                       CBK_LDS_NEXT("global_load_lds_dwordx4", "0x400", "%4") CBK_LDS_NEXT("global_load_lds_dwordx4", "0x400", "%5")
+                           CBK_LDS_NEXT("global_load_lds_dwordx4", "0x400", "%6") CBK_LDS_LAST
+                   : "=&s"(saved) : "s"(to), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]) : "memory", "scc");
+    } else {
+      asm volatile(CBK_LDS_FIRST("global_load_lds_dword", "%2") CBK_LDS_NEXT("global_load_lds_dword", "0x100", "%3")
+                       CBK_LDS_NEXT("global_load_lds_dword", "0x100", "%4") CBK_LDS_NEXT("global_load_lds_dword", "0x100", "%5")
+                           CBK_LDS_NEXT("global_load_lds_dword", "0x100", "%6") CBK_LDS_LAST
+                   : "=&s"(saved) : "s"(to), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]) : "memory", "scc");
+    }
   }
 }
+__device__ __forceinline__ void lds_dma_word(const void* addr, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(CBK_LDS_FIRST("global_load_lds_dword", "%2") CBK_LDS_LAST
+               : "=&s"(saved) : "s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(addr) : "memory");
+}
 
-// 8 codes of a word as the 8 bf16 of an MFMA operand, in the order 0 4 1 5 2 6
-// 3 7: as 128 + n, or (EXACT) as n - LESS.
-template <bool EXACT, int LESS = 0>
+// How codes n become an MFMA operand: as bf16 128 + n, as f16 1024 + n, or
+// converted to bf16 n - LESS.
+enum class Form { kBf16, kF16, kExact };
+
+// 8 codes of a word as 8 operand elements, in the order 0 4 1 5 2 6 3 7.
+template <Form F, int LESS = 0>
 __device__ __forceinline__ s16x8 operand(uint32_t w) {
   u32x4 r;
-  if constexpr (EXACT) {
+  if constexpr (F == Form::kExact) {
     const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6, 1 3 5 7
     auto f = [](uint32_t x, int byte) { return __float_as_uint(float((x >> (8 * byte)) & 0xffu) - float(LESS)); };
     auto pair = [](uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); };
@@ -137,10 +168,23 @@ __device__ __forceinline__ s16x8 operand(uint32_t w) {
     r[2] = pair(f(even, 1), f(even, 3));
     r[3] = pair(f(odd, 1), f(odd, 3));
   } else {
+    const uint32_t mask = 0x000f000fu, one = F == Form::kF16 ? 0x64006400u : 0x43004300u;
+    // (and, or in one instruction: the compiler takes two for two constants.
+    // No inline assembly: the hazards between what it writes and what a matrix
+    // instruction still reads would go unseen)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_bitop3_b32(w >> (4 * i), mask, one, 0xea);
   }
   return __builtin_bit_cast(s16x8, r);
+}
+
+template <Form F>
+__device__ __forceinline__ f32x4 mma(const s16x8& a, const s16x8& b, const f32x4& c) {
+  typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+  if constexpr (F == Form::kF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
 // two floats rounded to bf16, x in the low half
@@ -160,41 +204,72 @@ template <> __device__ __forceinline__ float load_elem<CBK_DTYPE_BF16>(const voi
 template <> __device__ __forceinline__ float load_elem<CBK_DTYPE_F16>(const void* p, int64_t at) {
   return float(static_cast<const _Float16*>(p)[at]);
 }
+// 8 neighbouring elements, in 16-byte pieces where they are aligned; zeros if not `live`
+template <int DT>
+__device__ __forceinline__ void load_elems(const void* p, int64_t at, bool pieces, bool live, float (&x)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  if (!live) return;
+  if (!pieces) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = load_elem<DT>(p, at + e);
+  } else if constexpr (DT == CBK_DTYPE_F32) {
+    const f32x4* w = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
+    const f32x4 lo = w[0], hi = w[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = lo[e];
+      x[e + 4] = hi[e];
+    }
+  } else {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t bits = uint16_t(w[e / 2] >> (16 * (e & 1)));
+      x[e] = DT == CBK_DTYPE_BF16 ? bf16_bits_to_float(bits) : float(__builtin_bit_cast(_Float16, bits));
+    }
+  }
+}
 template <int DT> __device__ __forceinline__ void store_elem(void* p, int64_t at, float x) {
   if constexpr (DT == CBK_DTYPE_F32) static_cast<float*>(p)[at] = x;
   else if constexpr (DT == CBK_DTYPE_BF16) static_cast<__bf16*>(p)[at] = __bf16(x);
   else static_cast<_Float16*>(p)[at] = _Float16(x);
 }
 
+// The operands' parts, the form of the codes beside q and beside p step.
 template <int DT> struct Parts;
-template <> struct Parts<CBK_DTYPE_BF16> { static constexpr int q = 1, p = 2; };
-template <> struct Parts<CBK_DTYPE_F16> { static constexpr int q = 2, p = 2; };
-template <> struct Parts<CBK_DTYPE_F32> { static constexpr int q = 3, p = 3; };
+template <> struct Parts<CBK_DTYPE_BF16> { static constexpr int q = 1, p = 2; static constexpr Form k = Form::kBf16, v = Form::kBf16; };
+template <> struct Parts<CBK_DTYPE_F16> { static constexpr int q = 1, p = 2; static constexpr Form k = Form::kF16, v = Form::kBf16; };
+template <> struct Parts<CBK_DTYPE_F32> { static constexpr int q = 3, p = 3; static constexpr Form k = Form::kExact, v = Form::kExact; };
 
 template <int DT, int NG, int VT, int PIECE>
-__global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnArgs a) {
-  constexpr bool EXACT = DT == CBK_DTYPE_F32;
+__global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const Int4AttnArgs a) {
+  constexpr int kMax = max_waves(DT);
   constexpr int QP = Parts<DT>::q, PP = Parts<DT>::p;
+  constexpr Form KF = Parts<DT>::k, VF = Parts<DT>::v;
+  constexpr float kLess = KF == Form::kF16 ? 1024.f : KF == Form::kBf16 ? 128.f : 0.f;  // in the codes beside q
   constexpr int D = 32 * NG, RB = kInt4GroupBytes * NG;  // dims and bytes of a head's row
-  constexpr int U = 4 / VT, COLS = 16 / VT;
-  constexpr uint32_t kBuf = kTile * RB;                  // one of K or V
-  constexpr uint32_t kPieces = RB / PIECE, kInsts = kTile * kPieces / 64;
-  constexpr uint32_t kWaveLds = 3 * kBuf;                // two K buffers, one of V: two workgroups per CU
-  static_assert(16 * D * 4 + 128 <= int(kWaveLds), "the wave's results fit its buffers");
-  // per wave: K buffers, V buffer; then the results of a sequence
-  __shared__ __attribute__((aligned(16))) char lds[kWaves][kWaveLds];
-  __shared__ uint32_t s_pages[kWaves][2][kTile];  // block table entries of two tiles' keys
+  constexpr int U = 2 / VT, COLS = 16 / VT;
+  constexpr uint32_t kBuf = kTile * RB;                      // K or V rows of a tile
+  constexpr uint32_t kPieces = RB / PIECE, kInsts = 2 * kTile * kPieces / 64;
+  constexpr uint32_t kWaveLds = kStages * 2 * kBuf;
+  static_assert(2 * kTile * kPieces % 64 == 0 && 16 * D * 4 + 128 <= int(kWaveLds), "whole requests; the wave's results fit its buffers");
+  // per wave: tiles of K rows, then V rows; then the results of a sequence
+  __shared__ __attribute__((aligned(16))) char lds[kMax][kWaveLds];
+  __shared__ uint32_t s_pages[kMax][2][64];  // block table entries of two tiles' keys
 
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t j = lane >> 4, c = lane & 15;
-  // workgroups of one range (all KV heads and row tiles) on one XCD, one after
-  // another: a token's row is one piece of memory for all heads
-  const uint32_t units = a.hkv * a.row_tiles;
-  const uint32_t turn = blockIdx.x >> 3;
-  const uint32_t range = __builtin_amdgcn_readfirstlane((turn / units) * 8 + (blockIdx.x & 7));
+  // workgroups of one range on one XCD, one after another: a token's row is
+  // one piece of memory for all heads
+  const uint32_t units = a.hkv / a.heads * a.row_tiles;
+  const uint32_t place_in = blockIdx.x >> 3;
+  const uint32_t range = __builtin_amdgcn_readfirstlane((place_in / units) * 8 + (blockIdx.x & 7));
   if (range >= a.ranges) return;
-  const uint32_t unit = __builtin_amdgcn_readfirstlane(turn % units);
-  const uint32_t kvh = unit / a.row_tiles, row_tile = unit - kvh * a.row_tiles;
+  const uint32_t unit = __builtin_amdgcn_readfirstlane(place_in % units);
+  const uint32_t head0 = unit / a.row_tiles * a.heads, row_tile = unit % a.row_tiles;  // the workgroup's
+  const uint32_t turn = __builtin_amdgcn_readfirstlane(wave / a.heads), turns = a.turns;
+  const uint32_t kvh = head0 + (wave - turn * a.heads);
 
   const Ranges cut(total_tiles(a, lane), a.ranges);
   uint32_t at = cut.first(range);
@@ -223,7 +298,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
   // a negative scale goes into the queries
   const float sign = a.scale < 0.f ? -1.f : 1.f, c2 = fabsf(a.scale) * kLog2e;
   const uint32_t lds0 = lds_address(&lds[wave][0]), pages0 = lds_address(&s_pages[wave][0][0]);
-  // the selector that puts a float's upper half into the low (tile even) or high half of a word
+  // the selector that puts a float's upper half into the low (first 16 keys) or high half of a word
   const uint32_t place = v ? 0x03020c0cu : 0x0c0c0302u, half = v ? 0xffff0000u : 0x0000ffffu;
 
   for (bool first_seq = true; at < end; first_seq = false) {
@@ -238,8 +313,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
     const uint32_t seq_end = before + tiles_of(len);
     const uint32_t stop = min(end, seq_end);
     const bool whole = at == before && stop == seq_end;
-    const int32_t tile0 = int32_t(at - before + wave);           // the wave's first tile of the sequence
-    const int32_t count = max(0, (int32_t(stop - at) - int32_t(wave) + kWaves - 1) / kWaves);
+    const int32_t tile0 = int32_t(at - before + turn);           // the wave's first tile of the sequence
+    const int32_t count = int32_t((stop - at + turns - 1 - turn) / turns);
     const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
     const int32_t last_key = live ? int32_t(len) - int32_t(a.rows) + int32_t(qr) : -1;  // the row sees keys up to it
 
@@ -250,9 +325,10 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
     for (int g = 0; g < NG; ++g) {
       const int64_t from = int64_t(seq) * a.q_batch + int64_t(qr) * a.q_row + int64_t(qh) * a.q_head + 32 * g + 8 * j;
       float x[8], sum = 0.f;
+      load_elems<DT>(a.q, from, a.q_pieces, live, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = live ? sign * load_elem<DT>(a.q, from + e) : 0.f;
+        x[e] *= sign;
         sum += x[e];
       }
       sum += __shfl_xor(sum, 16);
@@ -262,7 +338,14 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
       for (int p = 0; p < QP; ++p) {
         u32x4 w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(__float_as_uint(x[i + 4]), __float_as_uint(x[i]), 0x07060302u);
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (KF == Form::kF16) {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            w[i] = __builtin_bit_cast(uint32_t, h2{_Float16(x[i]), _Float16(x[i + 4])});
+          } else {
+            w[i] = __builtin_amdgcn_perm(__float_as_uint(x[i + 4]), __float_as_uint(x[i]), 0x07060302u);
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] -= __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
 #pragma unroll
@@ -278,86 +361,84 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
       o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // The block table's entries of tile i's keys, by DMA; from them where the
-    // tile's rows are; and K or V of those rows, by DMA. Keys past the context,
-    // or in a page out of range, are read from the first page and masked: their
-    // bits of the result are clear.
+    // The block table's entries of tile i's keys, by DMA; and, from them, the
+    // tile's rows, by DMA. Keys past the context, or in a page out of range, are
+    // read from the first page and masked: their bits of the result are clear.
     auto entries = [&](int32_t i) __attribute__((always_inline)) {
-      const uint32_t key = min(uint32_t(tile0 + kWaves * i) * kTile + lane, len - 1);
-      lds_dma<4>(reinterpret_cast<const char*>(table + a.block_div.div(key)), pages0 + uint32_t(i & 1) * kTile * 4);
+      const uint32_t key = min(uint32_t(tile0 + turns * i) * kTile + lane, len - 1);
+      lds_dma_word(table + a.block_div.div(key), pages0 + uint32_t(i & 1) * 256);
     };
-    int64_t row = 0;  // of key `lane` of the tile located last, from the planes' bases
-    auto locate = [&](int32_t i) __attribute__((always_inline)) {
-      const uint32_t key = uint32_t(tile0 + kWaves * i) * kTile + lane;
+    const char* const k_base = a.k_base + int64_t(kvh) * RB;
+    const int64_t v_minus_k = a.v_base - a.k_base;
+    auto request = [&](int32_t i, uint32_t buf) __attribute__((always_inline)) {
+      const uint32_t key = uint32_t(tile0 + turns * i) * kTile + lane;
       const uint32_t page = s_pages[wave][i & 1][lane];
       const bool held = key < len && page < a.num_blocks;
-      row = 0;
+      uint64_t row = 0;
       if (held) {
         const uint32_t blk = a.block_div.div(key);
-        row = int64_t(page) * a.block_stride + int64_t(key - blk * a.block_div.d) * a.token_stride;
+        row = uint64_t(page) * uint64_t(a.block_stride) + uint64_t(key - blk * a.block_div.d) * uint64_t(a.token_stride);
       }
-      return __ballot(held);
-    };
-    auto request = [&](const char* base, uint32_t buf) __attribute__((always_inline)) {
-      const int lo = int(uint32_t(row)), hi = int(uint32_t(uint64_t(row) >> 32));
-      base += int64_t(kvh) * RB;
+      uint64_t off[kInsts];
 #pragma unroll
       for (uint32_t n = 0; n < kInsts; ++n) {
-        // piece 64 n + lane: of the buffer's row R, which is key 16 (R % 16 / 4) + 4 (R / 16) + R % 4
-        const uint32_t piece = 64 * n + lane, R = piece / kPieces, part = piece - R * kPieces;
-        const int from = int(16 * ((R >> 2) & 3) + 4 * (R >> 4) + (R & 3));
-        uint64_t off = uint64_t(uint32_t(__shfl(lo, from))) | (uint64_t(uint32_t(__shfl(hi, from))) << 32);
-        off += part * PIECE;
-        asm volatile("" : "+v"(off));  // (base + part would be kept in registers for every n)
-        lds_dma<PIECE>(base + int64_t(off), buf + n * 64 * PIECE);
+        // piece 64 n + lane of the buffer: of row R of the K rows, then the V
+        // rows; that is key 8 (R % 16 / 4) + 4 (R / 16) + R % 4
+        const uint32_t piece = 64 * n + lane, line = piece / kPieces, part = piece - line * kPieces, R = line % kTile;
+        const int from = int(8 * ((R >> 2) & 3) + 4 * (R >> 4) + (R & 3));
+        off[n] = (uint64_t(uint32_t(__shfl(int(uint32_t(row)), from))) |
+                  (uint64_t(uint32_t(__shfl(int(uint32_t(row >> 32)), from))) << 32)) + part * PIECE;
+        if (64 * n >= uint32_t(kTile) * kPieces) off[n] += uint64_t(v_minus_k);
+        else if (64 * n + 63 >= uint32_t(kTile) * kPieces) off[n] += line >= uint32_t(kTile) ? uint64_t(v_minus_k) : 0u;
       }
+      lds_dma<PIECE>(k_base, off, lds0 + buf * 2 * kBuf);
+      return uint32_t(__ballot(held));
     };
 
-    uint64_t held = 0, held_next = 0;
-    CBK_WAIT_VM_LGKM0(0);  // nothing of the compiler's own in flight
+    uint32_t held[2] = {0, 0};  // of tiles i and i + 1
+    CBK_WAIT_VM_LGKM0(0);       // nothing of the compiler's own in flight
     if (count > 0) {
       entries(0);
       if (count > 1) entries(1);
       CBK_WAIT_VM_LGKM0(0);
-      held = locate(0);
-      request(a.k_base, lds0);
-      request(a.v_base, lds0 + 2 * kBuf);
+      held[0] = request(0, 0);
       if (count > 2) entries(2);
-      if (count > 1) {
-        held_next = locate(1);
-        request(a.k_base, lds0 + kBuf);
-      }
+      if (count > 1) held[1] = request(1, 1);
     }
+    uint32_t buf = 0;  // of tile i: i % kStages
     for (int32_t i = 0; i < count; ++i) {
-      // requested in this order: K(i), V(i), the entries of tile i + 2, K(i + 1);
-      // K(i) has landed
-      if (i + 1 < count) CBK_WAIT_VM_LGKM0(2 * kInsts);
-      else CBK_WAIT_VM_LGKM0(kInsts);
+      // requested in this order: tile i, the entries of tile i + 2, tile i + 1;
+      // all but the last have landed
+      if (i + 1 < count) CBK_WAIT_VM_LGKM0(kInsts);
+      else CBK_WAIT_VM_LGKM0(0);
       asm volatile("" ::: "memory");
-      const char* kb = &lds[wave][(i & 1) * kBuf];
-      const char* vb = &lds[wave][2 * kBuf];
-      const int32_t key0 = (tile0 + kWaves * i) * kTile;
-      const uint64_t here = held;
-      const bool masked = here != ~uint64_t(0) || key0 + kTile > int32_t(len - a.rows + 1);
+      const uint32_t here = held[0];
+      held[0] = held[1];
+      if (i + 3 < count) entries(i + 3);
+      if (i + 2 < count) held[1] = request(i + 2, buf == 0 ? 2 : buf - 1);  // the buffer of tile i - 1
+      const char* kb = &lds[wave][buf * 2 * kBuf];
+      const char* vb = kb + kBuf;
+      buf = buf == kStages - 1 ? 0 : buf + 1;
+      const int32_t key0 = int32_t(tile0 + turns * i) * kTile;
+      const bool masked = here != ~0u || key0 + kTile > int32_t(len - a.rows + 1);
 
       auto step = [&](auto mask) __attribute__((always_inline)) {
         constexpr bool MASK = decltype(mask)::value;
-        // S^T: x[u][i] is the logit (log2 units) of key 16 j + 4 (u VT + v) + i and column c's row
+        // S^T: x[u][i] is the logit (log2 units) of key 8 j + 4 (u VT + v) + i and column c's row
         f32x4 x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          __builtin_amdgcn_sched_barrier(0);
           f32x4 acc[NG];
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const float init = EXACT ? 0.f : -128.f * qs[g];
+            const float init = -kLess * qs[g];
             acc[g] = f32x4{init, init, init, init};
 #pragma unroll
             for (int t = 0; t < VT; ++t) {
               const uint32_t w = *reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + t) + c) * RB + 16 * g + 4 * j);
-              const s16x8 kf = operand<EXACT>(w);
+              const s16x8 kf = operand<KF>(w);
 #pragma unroll
-              for (int p = 0; p < QP; ++p) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[p][t][g], acc[g], 0, 0, 0);
+              for (int p = 0; p < QP; ++p) acc[g] = mma<KF>(kf, qf[p][t][g], acc[g]);
             }
           }
 #pragma unroll
@@ -373,11 +454,11 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
           }
         }
         // which of the lane's keys its row sees: bit 4 t + i of `seen`
-        uint32_t seen = 0xffffu;
+        uint32_t seen = 0xffu;
         if constexpr (MASK) {
-          const int32_t left = last_key - key0 - int32_t(16 * j) + 1;  // of the lane's 16 keys
-          seen = uint32_t(here >> (16 * j)) & 0xffffu;
-          seen &= left <= 0 ? 0u : left >= 16 ? 0xffffu : (1u << left) - 1u;
+          const int32_t left = last_key - key0 - int32_t(8 * j) + 1;  // of the lane's 8 keys
+          seen = (here >> (8 * j)) & 0xffu;
+          seen &= left <= 0 ? 0u : left >= 8 ? 0xffu : (1u << left) - 1u;
 #pragma unroll
           for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -417,80 +498,61 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
             x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - ms);  // p from here on
             l += x[u][r];
           }
-        // V(i) and the entries have landed
-        if (i + 1 < count) CBK_WAIT_VM_LGKM0(kInsts);
-        else CBK_WAIT_VM_LGKM0(0);
-        asm volatile("" ::: "memory");
-        // O += (p step) . n, the 32 keys of tiles 2 h and 2 h + 1 at a time: p step
-        // in bf16 parts, operand word r key r of the first tile in its low half,
-        // of the second in its high half
-        const uint32_t from = (16 * (c >> 2) + 4 * j + (c & 3)) * RB;  // the row of key 16 j + c
-        const s16x8 less = __builtin_bit_cast(s16x8, u32x4(0xc300c300u));  // -128
+        // O += (p step) . n: p step in bf16 parts, operand word r key r of the
+        // first half in its low half, of the second in its high half
+        u32x4 pw[NG][PP];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          __builtin_amdgcn_sched_barrier(0);
-          u32x4 pw[NG][PP];
+        for (int r = 0; r < 4; ++r) {
+          float y[NG][U];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float y[NG][2 / VT];
+          for (int u = 0; u < U; ++u) {
+            const uint32_t* sw = reinterpret_cast<const uint32_t*>(vb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
+            const bool sees = !MASK || ((seen >> (4 * (u * VT + v) + r)) & 1u);
 #pragma unroll
-            for (int t = 0; t < 2 / VT; ++t) {
-              const int u = h * (2 / VT) + t;
-              const uint32_t* sw = reinterpret_cast<const uint32_t*>(vb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
-              const bool sees = !MASK || ((seen >> (4 * (u * VT + v) + r)) & 1u);
-#pragma unroll
-              for (int g = 0; g < NG; ++g) {
-                const uint32_t word = sees ? sw[g] : 0u;  // a masked key's step and offset may be anything
-                y[g][t] = x[u][r] * __uint_as_float(word << 16);
-                float z = __uint_as_float(word & 0xffff0000u);
-                if constexpr (EXACT) z = fmaf(8.f, __uint_as_float(word << 16), z);
-                zsum[g] = fmaf(x[u][r], z, zsum[g]);
-              }
+            for (int g = 0; g < NG; ++g) {
+              const uint32_t word = sees ? sw[g] : 0u;  // a masked key's step and offset may be anything
+              y[g][u] = x[u][r] * __uint_as_float(word << 16);
+              float z = __uint_as_float(word & 0xffff0000u);
+              if constexpr (VF == Form::kExact) z = fmaf(8.f, __uint_as_float(word << 16), z);
+              zsum[g] = fmaf(x[u][r], z, zsum[g]);
             }
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-              for (int q = 0; q < PP; ++q) {
-                if (q + 1 < PP) {  // the upper halves, and what is left
-                  pw[g][q][r] = VT == 1 ? __builtin_amdgcn_perm(__float_as_uint(y[g][2 / VT - 1]), __float_as_uint(y[g][0]), 0x07060302u)
-                                        : __builtin_amdgcn_perm(0u, __float_as_uint(y[g][0]), place);
-#pragma unroll
-                  for (int t = 0; t < 2 / VT; ++t) y[g][t] -= __uint_as_float(__float_as_uint(y[g][t]) & 0xffff0000u);
-                } else {
-                  pw[g][q][r] = pack_bf16(y[g][0], y[g][2 / VT - 1]) & (VT == 1 ? 0xffffffffu : half);
-                }
-              }
           }
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
+          for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-              const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                  (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) const void*)(vb + from + 16 * g + 8 * d)));
-              const s16x8 vf = operand<EXACT, 8>(uint32_t(w[h]));
+            for (int q = 0; q < PP; ++q) {
+              if (q + 1 < PP) {  // the upper halves, and what is left
+                pw[g][q][r] = VT == 1 ? __builtin_amdgcn_perm(__float_as_uint(y[g][U - 1]), __float_as_uint(y[g][0]), 0x07060302u)
+                                      : __builtin_amdgcn_perm(0u, __float_as_uint(y[g][0]), place);
 #pragma unroll
-              for (int q = 0; q < PP; ++q)
-              {
-                const s16x8 pf = __builtin_bit_cast(s16x8, pw[g][q]);
-                o[2 * g + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, vf, o[2 * g + d], 0, 0, 0);
-                if constexpr (!EXACT) o[2 * g + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf, less, o[2 * g + d], 0, 0, 0);
+                for (int u = 0; u < U; ++u) y[g][u] -= __uint_as_float(__float_as_uint(y[g][u]) & 0xffff0000u);
+              } else {
+                pw[g][q][r] = pack_bf16(y[g][0], y[g][U - 1]) & (VT == 1 ? 0xffffffffu : half);
               }
             }
+        }
+        const uint32_t from = (16 * ((c >> 2) & 1) + 4 * j + (c & 3)) * RB + (c >> 3) * 8;  // the row of key 8 j + c % 8
+        const s16x8 less = __builtin_bit_cast(s16x8, u32x4(0xc300c300u));  // -128
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+              (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) const void*)(vb + from + 16 * g)));
+          const s16x8 vf[2] = {operand<VF, 8>(uint32_t(w[0])), operand<VF, 8>(uint32_t(w[1]))};
+#pragma unroll
+          for (int q = 0; q < PP; ++q) {
+            const s16x8 pf = __builtin_bit_cast(s16x8, pw[g][q]);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, vf[d], o[2 * g + d]);
+            if constexpr (VF != Form::kExact)
+#pragma unroll
+              for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, less, o[2 * g + d]);
           }
         }
       };
       if (masked) step(std::true_type());
       else step(std::false_type());
-
-      // the reads of this tile's buffers are done before the next requests into them
+      // the reads of this tile's buffer are done before the next requests into it
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      held = held_next;
-      if (i + 1 < count) request(a.v_base, lds0 + 2 * kBuf);
-      if (i + 3 < count) entries(i + 3);
-      if (i + 2 < count) {
-        held_next = locate(i + 2);
-        request(a.k_base, lds0 + uint32_t(i & 1) * kBuf);
-      }
     }
 
     // the wave's results, then all waves' and column groups' together
@@ -515,17 +577,16 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
       mine[16 * D + 2 * c + 1] = l;
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < uint32_t(COLS * D); e += kThreads) {
-      const uint32_t row = e / D, dim = e - row * D, n = row_tile * COLS + row;
-      if (n >= a.rows * a.group) break;
+    for (uint32_t e = threadIdx.x; e < a.heads * uint32_t(COLS * D); e += blockDim.x) {
+      const uint32_t line = e / D, dim = e - line * D, head = line / COLS, row = line - head * COLS;
+      const uint32_t n = row_tile * COLS + row;
+      if (n >= a.rows * a.group) continue;
       float top = kNegInf, sum = 0.f, acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w)
+      for (uint32_t w = head; w < a.heads * turns; w += a.heads)
 #pragma unroll
         for (int t = 0; t < VT; ++t) top = fmaxf(top, reinterpret_cast<const float*>(&lds[w][0])[16 * D + 2 * (t * COLS + row)]);
       const float ts = top == kNegInf ? 0.f : top;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w)
+      for (uint32_t w = head; w < a.heads * turns; w += a.heads)
 #pragma unroll
         for (int t = 0; t < VT; ++t) {
           const float* res = reinterpret_cast<const float*>(&lds[w][0]);
@@ -534,12 +595,12 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
           sum = fmaf(f, res[16 * D + 2 * col + 1], sum);
           acc = fmaf(f, res[col * D + dim], acc);
         }
-      const uint32_t r = n / a.group, h = kvh * a.group + n % a.group;
+      const uint32_t r = n / a.group, h = (head0 + head) * a.group + n % a.group;
       if (whole) {
         store_elem<DT>(a.out, int64_t(seq) * a.out_batch + int64_t(r) * a.out_row + int64_t(h) * a.out_head + dim,
                        sum == 0.f ? 0.f : acc / sum);
       } else {
-        const int64_t id = (int64_t(2 * range + (first_seq ? 0 : 1)) * a.hkv + kvh) * (a.rows * a.group) + n;
+        const int64_t id = (int64_t(2 * range + (first_seq ? 0 : 1)) * a.hkv + head0 + head) * (a.rows * a.group) + n;
         a.o[id * D + dim] = acc;
         if (dim == 0) a.ml[id] = make_float2(top, sum);
       }
@@ -549,92 +610,97 @@ __global__ __launch_bounds__(kThreads, 2) void int4_attn_kernel(const Int4AttnAr
   }
 }
 
-// The sequences that more than one range holds, and those without keys: 32
-// lanes a row, each D / 32 dims.
+// The sequences that more than one range holds, and those without keys: a
+// workgroup per row, every 32 lanes each eighth range of it (one 32 lanes for
+// all of 128 ranges took 46 us), each lane D / 32 dims.
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void int4_attn_merge_kernel(const Int4AttnArgs a) {
-  constexpr int N = D / 32;
+__global__ __launch_bounds__(kMergeThreads) void int4_attn_merge_kernel(const Int4AttnArgs a) {
+  constexpr int N = D / 32, SUBS = kMergeThreads / 32;
+  typedef float VecN __attribute__((ext_vector_type(N)));
+  __shared__ float s_o[SUBS][D], s_l[SUBS], s_m[SUBS];
   const uint32_t seq = blockIdx.y;
-  const uint32_t lane = threadIdx.x & 63;
-  // tiles before the sequence, and of all
-  uint32_t before = 0, total = 0;
-  for (uint32_t b = lane; b < a.batch; b += 64) {
-    const uint32_t n = tiles_of(context_of(a, b));
-    total += n;
-    before += b < seq ? n : 0u;
-  }
-  total = __builtin_amdgcn_readfirstlane(wave_sum_u32(total));
-  before = __builtin_amdgcn_readfirstlane(wave_sum_u32(before));
+  const uint32_t lane = threadIdx.x & 63, dim = threadIdx.x & 31, sub = threadIdx.x >> 5;
   const uint32_t tiles = tiles_of(context_of(a, seq));
-  const uint32_t row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), sub = threadIdx.x & 31;
   const uint32_t per_head = a.rows * a.group;
-  if (row >= a.hkv * per_head) return;
-  const uint32_t kvh = row / per_head, n = row - kvh * per_head;
-  float acc[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  float inv = 0.f;
+  const uint32_t kvh = blockIdx.x / per_head, n = blockIdx.x - kvh * per_head;
+  float top = kNegInf, sum = 0.f;
+  VecN acc = VecN(0.f);
   if (tiles != 0) {
+    // tiles before the sequence, and of all
+    uint32_t before = 0, total = 0;
+    for (uint32_t b = lane; b < a.batch; b += 64) {
+      const uint32_t t = tiles_of(context_of(a, b));
+      total += t;
+      before += b < seq ? t : 0u;
+    }
+    total = __builtin_amdgcn_readlane(wave_inclusive_scan(total), 63);
+    before = __builtin_amdgcn_readlane(wave_inclusive_scan(before), 63);
     const Ranges cut(total, a.ranges);
     const uint32_t r0 = cut.of(before), r1 = cut.of(before + tiles - 1);
     if (r0 == r1) return;  // written by its range
     // range r0 may end with this sequence after others; the rest begin in it
     const uint32_t which0 = cut.first(r0) < before ? 1u : 0u;
-    auto id = [&](uint32_t r) { return (int64_t(2 * r + (r == r0 ? which0 : 0u)) * a.hkv + kvh) * per_head + n; };
-    float top = kNegInf;
-    for (uint32_t r = r0 + sub; r <= r1; r += 32) top = fmaxf(top, a.ml[id(r)].x);
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 32));
-    const float ts = top == kNegInf ? 0.f : top;
-    float sum = 0.f;
-    for (uint32_t b0 = r0; b0 <= r1; b0 += 32) {
-      float2 ml = make_float2(kNegInf, 0.f);
-      if (b0 + sub <= r1) ml = a.ml[id(b0 + sub)];
-      const float f = __builtin_amdgcn_exp2f(ml.x - ts);
-      sum = fmaf(f, ml.y, sum);
-      const uint32_t most = min(32u, r1 - b0 + 1);
-      for (uint32_t i = 0; i < most; ++i) {
-        const float w = __shfl(f, int(i), 32);
-        const float* src = a.o + id(b0 + i) * D + N * sub;
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = fmaf(w, src[e], acc[e]);
-      }
+#pragma unroll 4
+    for (uint32_t r = r0 + sub; r <= r1; r += SUBS) {
+      const int64_t id = (int64_t(2 * r + (r == r0 ? which0 : 0u)) * a.hkv + kvh) * per_head + n;
+      const float2 ml = a.ml[id];
+      const VecN part = *reinterpret_cast<const VecN*>(a.o + id * D + N * dim);
+      const float mn = fmaxf(top, ml.x), ms = mn == kNegInf ? 0.f : mn;
+      const float f = __builtin_amdgcn_exp2f(top - ms), w = __builtin_amdgcn_exp2f(ml.x - ms);
+      sum = f * sum + w * ml.y;
+      acc = f * acc + w * part;
+      top = mn;
     }
+  }
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 32);
-    inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (sum == 0.f)
+  for (int e = 0; e < N; ++e) s_o[sub][N * dim + e] = acc[e];
+  if (dim == 0) {
+    s_m[sub] = top;
+    s_l[sub] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x >= uint32_t(D)) return;
+  float all = kNegInf, l = 0.f, o = 0.f;
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  for (int i = 0; i < SUBS; ++i) all = fmaxf(all, s_m[i]);
+  const float ms = all == kNegInf ? 0.f : all;
+#pragma unroll
+  for (int i = 0; i < SUBS; ++i) {
+    const float w = __builtin_amdgcn_exp2f(s_m[i] - ms);
+    l = fmaf(w, s_l[i], l);
+    o = fmaf(w, s_o[i][threadIdx.x], o);
   }
   const uint32_t r = n / a.group, h = kvh * a.group + n % a.group;
-  const int64_t to = int64_t(seq) * a.out_batch + int64_t(r) * a.out_row + int64_t(h) * a.out_head + N * sub;
-#pragma unroll
-  for (int e = 0; e < N; ++e) store_elem<DT>(a.out, to + e, acc[e] * inv);
+  store_elem<DT>(a.out, int64_t(seq) * a.out_batch + int64_t(r) * a.out_row + int64_t(h) * a.out_head + threadIdx.x,
+                 l == 0.f ? 0.f : o / l);
 }
 
-// Columns of a workgroup's rows: VT = 2 where 8 rows of a KV head hold them all
-constexpr uint32_t kFewRows = 8;
+// Column groups for the rows of a KV head.
+constexpr int column_groups(uint64_t rows) { return rows <= 8 ? 2 : 1; }
 
 struct Plan {
-  uint32_t row_tiles, ranges;
+  uint32_t row_tiles, ranges, heads, turns;
 };
 
-int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t max_len, Plan* p) {
+int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t max_len, int32_t dtype, Plan* p) {
   CBK_REQUIRE(batch >= 0 && batch < (1 << 16), "batch out of range");
   CBK_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "query heads must be divisible by KV heads");
   CBK_REQUIRE(rows > 0 && hq < (1 << 16) && rows < (1 << 16), "rows or heads out of range");
   CBK_REQUIRE(max_len >= 0 && max_len < (int64_t(1) << 31) - kTile, "context out of range");
   const int64_t n = rows * (hq / hkv);
-  p->row_tiles = n <= kFewRows ? 1 : uint32_t((n + 15) / 16);
+  p->row_tiles = uint32_t((n + 15) / 16);
+  const uint32_t waves = uint32_t(max_waves(dtype));
+  for (p->heads = waves; hkv % p->heads != 0;) --p->heads;
+  p->turns = waves / p->heads;
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
-  // two workgroups of each CU at once (LDS); fewer where there are fewer tiles
+  // a workgroup of each CU (LDS, registers); fewer where its waves would have
+  // less than a tile or two each
   const int64_t most = batch * ((max_len + kTile - 1) / kTile);
   CBK_REQUIRE(most < (int64_t(1) << 31), "context tiles out of range");
-  const int64_t units = hkv * int64_t(p->row_tiles);
-  int64_t ranges = (2 * int64_t(cus) + units - 1) / units;
-  ranges = ranges < most ? ranges : most;
+  const int64_t units = hkv / p->heads * int64_t(p->row_tiles);
+  int64_t ranges = (int64_t(cus) + units - 1) / units;
+  ranges = std::min(ranges, (most + p->turns - 1) / p->turns);
   p->ranges = uint32_t(ranges > 1 ? ranges : 1);
   return CBK_OK;
 }
@@ -647,25 +713,26 @@ size_t plan_bytes(const Plan& p, int64_t rows, int64_t hq, int64_t d) {
   return ml_bytes(p, rows, hq) + size_t(2) * p.ranges * size_t(rows) * size_t(hq) * size_t(d) * sizeof(float);
 }
 
+template <int DT, int NG, int P>
+int launch_pieces(const Int4AttnArgs& a, hipStream_t s) {
+  const uint64_t groups = uint64_t(a.hkv / a.heads) * a.row_tiles * ((a.ranges + 7) / 8 * 8);
+  const uint32_t threads = 64 * a.heads * a.turns;
+  CBK_REQUIRE(groups * threads < (uint64_t(1) << 32), "int4 attention: %llu workgroups exceed one launch",
+              (unsigned long long)groups);
+  const dim3 grid(uint32_t(groups), 1, 1), block(threads);
+  if (column_groups(uint64_t(a.rows) * a.group) == 2)
+    hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 2, P>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 1, P>), grid, block, 0, s, a);
+  return launch_status("int4 attention");
+}
+
 template <int DT, int NG>
 int launch(const Int4AttnArgs& a, bool pieces16, hipStream_t s) {
-  const uint64_t groups = uint64_t(a.hkv) * a.row_tiles * ((a.ranges + 7) / 8 * 8);
-  CBK_REQUIRE(groups * kThreads < (uint64_t(1) << 32), "int4 attention: %llu workgroups exceed one launch",
-              (unsigned long long)groups);
-  const dim3 grid(uint32_t(groups), 1, 1), block(kThreads);
-  const bool few = a.rows * a.group <= kFewRows;
-  if (pieces16 && NG % 4 == 0) {
-    constexpr int P = NG % 4 == 0 ? 16 : 4;
-    if (few) hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 2, P>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 1, P>), grid, block, 0, s, a);
-  } else {
-    if (few) hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 2, 4>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((int4_attn_kernel<DT, NG, 1, 4>), grid, block, 0, s, a);
-  }
-  if (int rc = launch_status("int4 attention")) return rc;
-  const uint64_t rows = uint64_t(a.rows) * a.hq;
-  const dim3 merge(uint32_t((rows + kThreads / 32 - 1) / (kThreads / 32)), a.batch);
-  hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG>), merge, block, 0, s, a);
+  // 16-byte pieces of a row: whole ones, where the pages are aligned to them
+  constexpr int P = kInt4GroupBytes * NG % 16 == 0 ? 16 : 4;
+  if (int rc = pieces16 ? launch_pieces<DT, NG, P>(a, s) : launch_pieces<DT, NG, 4>(a, s)) return rc;
+  hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG>), dim3(a.rows * a.hq, a.batch), dim3(kMergeThreads), 0, s, a);
   return launch_status("int4 attention merge");
 }
 
@@ -675,10 +742,10 @@ int launch(const Int4AttnArgs& a, bool pieces16, hipStream_t s) {
 extern "C" {
 
 size_t cbk_paged_attention_int4_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
-                                                int64_t max_len) {
+                                                int64_t max_len, int32_t dtype) {
   using namespace cbk;
   Plan p;
-  if (batch <= 0 || head_dim <= 0 || plan_of(batch, rows, hq, hkv, max_len, &p)) return 0;
+  if (batch <= 0 || head_dim <= 0 || plan_of(batch, rows, hq, hkv, max_len, dtype, &p)) return 0;
   return plan_bytes(p, rows, hq, head_dim);
 }
 
@@ -701,7 +768,7 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
   CBK_REQUIRE(kv->num_blocks < (int64_t(1) << 31), "num_blocks out of range");
   int64_t max_len = table_width * kv->block_size;
   Plan p;
-  if (int rc = plan_of(batch, rows, hq, hkv, max_len, &p)) return rc;
+  if (int rc = plan_of(batch, rows, hq, hkv, max_len, dtype, &p)) return rc;
   if (batch == 0) return CBK_OK;
   CBK_REQUIRE(q_dev && out_dev && lens_dev && (tables_dev || table_width == 0), "NULL pointer");
   const int64_t words[4] = {int64_t(reinterpret_cast<uintptr_t>(kv->k_base)),
@@ -737,7 +804,12 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
   a.max_len = uint32_t(max_len);
   a.row_tiles = p.row_tiles;
   a.ranges = p.ranges;
+  a.heads = p.heads;
+  a.turns = p.turns;
   a.scale = scale;
+  const int64_t es = dtype == CBK_DTYPE_F32 ? 4 : 2;
+  const int64_t pieces[4] = {int64_t(reinterpret_cast<uintptr_t>(q_dev)), q_batch_stride * es, q_row_stride * es, q_head_stride * es};
+  a.q_pieces = common_vec_bytes(pieces, 4) == 16;
   a.block_div = FastDiv::make(uint32_t(kv->block_size));
   a.ml = static_cast<float2*>(workspace_dev);
   a.o = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + ml_bytes(p, rows, hq));
