@@ -24,8 +24,10 @@
 // of it; cut off instead it would be a bias, which a long context's sums of
 // both signs do not forgive).
 //
-// A wave takes 32 keys of one KV head at a time, their K and V rows staged in
-// its own LDS by DMA two tiles ahead (no barrier in the loop), and 16 columns of
+// A wave takes 32 keys of one KV head at a time, their rows staged in its own
+// LDS by DMA two steps ahead (no barrier in the loop): a step's buffer holds V
+// of its tile and K of the next, for it takes S^T of the next tile beside P . V
+// of its own, two chains of dependent work in turns. And a wave takes 16 columns of
 // S^T = K . Q^T: VT column groups of 16 / VT rows each, for the rows of the
 // group are often fewer than 16. The Q operand of a 16-key half is zero outside
 // the half's column group, so VT 2 gives both halves one accumulator, and the
@@ -361,197 +363,230 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
       o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // The block table's entries of tile i's keys, by DMA; and, from them, the
-    // tile's rows, by DMA. Keys past the context, or in a page out of range, are
-    // read from the first page and masked: their bits of the result are clear.
+    // The block table's entries of step i's rows -- K of tile i + 1, lanes 0 to
+    // 31, and V of tile i, the others -- by DMA; and, from them, the rows, by DMA.
+    // Keys past the context, or in a page out of range, are read from the first
+    // page and masked: their bits of the result, K's, are clear.
+    auto key_of = [&](int32_t i) __attribute__((always_inline)) {  // of this lane; < 0 before the first tile
+      return int32_t(tile0 + turns * (i + (lane < 32u ? 1 : 0))) * kTile + int32_t(lane & 31u);
+    };
     auto entries = [&](int32_t i) __attribute__((always_inline)) {
-      const uint32_t key = min(uint32_t(tile0 + turns * i) * kTile + lane, len - 1);
+      const uint32_t key = uint32_t(min(max(key_of(i), 0), int32_t(len) - 1));
       lds_dma_word(table + a.block_div.div(key), pages0 + uint32_t(i & 1) * 256);
     };
     const char* const k_base = a.k_base + int64_t(kvh) * RB;
     const int64_t v_minus_k = a.v_base - a.k_base;
     auto request = [&](int32_t i, uint32_t buf) __attribute__((always_inline)) {
-      const uint32_t key = uint32_t(tile0 + turns * i) * kTile + lane;
+      const int32_t key = key_of(i);
       const uint32_t page = s_pages[wave][i & 1][lane];
-      const bool held = key < len && page < a.num_blocks;
+      const bool held = key >= 0 && key < int32_t(len) && page < a.num_blocks;
       uint64_t row = 0;
       if (held) {
-        const uint32_t blk = a.block_div.div(key);
-        row = uint64_t(page) * uint64_t(a.block_stride) + uint64_t(key - blk * a.block_div.d) * uint64_t(a.token_stride);
+        const uint32_t blk = a.block_div.div(uint32_t(key));
+        row = uint64_t(page) * uint64_t(a.block_stride) +
+              uint64_t(uint32_t(key) - blk * a.block_div.d) * uint64_t(a.token_stride);
       }
+      if (lane >= 32u) row += uint64_t(v_minus_k);
       uint64_t off[kInsts];
 #pragma unroll
       for (uint32_t n = 0; n < kInsts; ++n) {
         // piece 64 n + lane of the buffer: of row R of the K rows, then the V
         // rows; that is key 8 (R % 16 / 4) + 4 (R / 16) + R % 4
         const uint32_t piece = 64 * n + lane, line = piece / kPieces, part = piece - line * kPieces, R = line % kTile;
-        const int from = int(8 * ((R >> 2) & 3) + 4 * (R >> 4) + (R & 3));
+        const int from = int((line & 32u) + 8 * ((R >> 2) & 3) + 4 * (R >> 4) + (R & 3));
         off[n] = (uint64_t(uint32_t(__shfl(int(uint32_t(row)), from))) |
                   (uint64_t(uint32_t(__shfl(int(uint32_t(row >> 32)), from))) << 32)) + part * PIECE;
-        if (64 * n >= uint32_t(kTile) * kPieces) off[n] += uint64_t(v_minus_k);
-        else if (64 * n + 63 >= uint32_t(kTile) * kPieces) off[n] += line >= uint32_t(kTile) ? uint64_t(v_minus_k) : 0u;
       }
       lds_dma<PIECE>(k_base, off, lds0 + buf * 2 * kBuf);
       return uint32_t(__ballot(held));
     };
 
-    uint32_t held[2] = {0, 0};  // of tiles i and i + 1
-    CBK_WAIT_VM_LGKM0(0);       // nothing of the compiler's own in flight
-    if (count > 0) {
+    f32x4 x[U];  // logits (log2 units), then weights, of key 8 j + 4 (u VT + v) + r and column c's row
+    uint32_t seen = 0xffu;  // which of the lane's keys its row sees: bit 4 t + r
+    bool masked = false;    // uniform: not all keys of the tile, for all rows
+
+    // S^T of a tile
+    auto logits = [&](const char* kb, f32x4 (&s)[U]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        f32x4 acc[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float init = -kLess * qs[g];
+          acc[g] = f32x4{init, init, init, init};
+#pragma unroll
+          for (int t = 0; t < VT; ++t) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + t) + c) * RB + 16 * g + 4 * j);
+            const s16x8 kf = operand<KF>(w);
+#pragma unroll
+            for (int p = 0; p < QP; ++p) acc[g] = mma<KF>(kf, qf[p][t][g], acc[g]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t* sw = reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
+          float sum = 0.f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            sum = fmaf(__uint_as_float(sw[g] << 16), acc[g][r], sum);
+            sum = fmaf(__uint_as_float(sw[g] & 0xffff0000u), qs[g], sum);
+          }
+          s[u][r] = sum * c2;
+        }
+      }
+    };
+    // the tile's mask, from its keys' bits, and the reference maximum
+    auto settle = [&](int32_t key0, uint32_t here) __attribute__((always_inline)) {
+      masked = here != ~0u || key0 + kTile > int32_t(len - a.rows + 1);
+      seen = 0xffu;
+      if (masked) {
+        const int32_t left = last_key - key0 - int32_t(8 * j) + 1;  // of the lane's 8 keys
+        seen = (here >> (8 * j)) & 0xffu;
+        seen &= left <= 0 ? 0u : left >= 8 ? 0xffu : (1u << left) - 1u;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!((seen >> (4 * (u * VT + v) + r)) & 1u)) x[u][r] = kNegInf;
+      }
+      float lm = x[0][0];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lm = fmaxf(lm, x[u][r]);
+      if (__any(lm > m + kRescale)) {  // rare: raise the reference of the columns that need it
+        float bm = fmaxf(lm, __shfl_xor(lm, 16));
+        bm = fmaxf(bm, __shfl_xor(bm, 32));
+        const float mn = fmaxf(m, bm);
+        const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= alpha;
+        float ao[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ao[r] = __shfl(alpha, int(4 * j + r));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          zsum[g] *= alpha;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            o[2 * g][r] *= ao[r];
+            o[2 * g + 1][r] *= ao[r];
+          }
+        }
+      }
+    };
+    // O += P . V of the settled tile
+    auto sums = [&](const char* vb, auto mask) __attribute__((always_inline)) {
+      constexpr bool MASK = decltype(mask)::value;
+      const float ms = m == kNegInf ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - ms);
+          l += x[u][r];
+        }
+      // p step in bf16 parts, operand word r key r of the first half in its low
+      // half, of the second in its high half
+      u32x4 pw[NG][PP];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float y[NG][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t* sw = reinterpret_cast<const uint32_t*>(vb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
+          const bool sees = !MASK || ((seen >> (4 * (u * VT + v) + r)) & 1u);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const uint32_t word = sees ? sw[g] : 0u;  // a masked key's step and offset may be anything
+            y[g][u] = x[u][r] * __uint_as_float(word << 16);
+            float z = __uint_as_float(word & 0xffff0000u);
+            if constexpr (VF == Form::kExact) z = fmaf(8.f, __uint_as_float(word << 16), z);
+            zsum[g] = fmaf(x[u][r], z, zsum[g]);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int q = 0; q < PP; ++q) {
+            if (q + 1 < PP) {  // the upper halves, and what is left
+              pw[g][q][r] = VT == 1 ? __builtin_amdgcn_perm(__float_as_uint(y[g][U - 1]), __float_as_uint(y[g][0]), 0x07060302u)
+                                    : __builtin_amdgcn_perm(0u, __float_as_uint(y[g][0]), place);
+#pragma unroll
+              for (int u = 0; u < U; ++u) y[g][u] -= __uint_as_float(__float_as_uint(y[g][u]) & 0xffff0000u);
+            } else {
+              pw[g][q][r] = pack_bf16(y[g][0], y[g][U - 1]) & (VT == 1 ? 0xffffffffu : half);
+            }
+          }
+      }
+      const uint32_t from = (16 * ((c >> 2) & 1) + 4 * j + (c & 3)) * RB + (c >> 3) * 8;  // the row of key 8 j + c % 8
+      const s16x8 less = __builtin_bit_cast(s16x8, u32x4(0xc300c300u));  // -128
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) const void*)(vb + from + 16 * g)));
+        const s16x8 vf[2] = {operand<VF, 8>(uint32_t(w[0])), operand<VF, 8>(uint32_t(w[1]))};
+#pragma unroll
+        for (int q = 0; q < PP; ++q) {
+          const s16x8 pf = __builtin_bit_cast(s16x8, pw[g][q]);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, vf[d], o[2 * g + d]);
+          if constexpr (VF != Form::kExact)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, less, o[2 * g + d]);
+        }
+      }
+    };
+
+    uint32_t held = 0, held_next = 0;  // of the K rows of steps i and i + 1
+    CBK_WAIT_VM_LGKM0(0);              // nothing of the compiler's own in flight
+    if (count > 0) {  // step -1: S^T of tile 0 alone
+      entries(-1);
       entries(0);
-      if (count > 1) entries(1);
       CBK_WAIT_VM_LGKM0(0);
-      held[0] = request(0, 0);
+      held = request(-1, 2);
+      if (count > 1) entries(1);
+      held_next = request(0, 0);
+      CBK_WAIT_VM_LGKM0(kInsts);
+      asm volatile("" ::: "memory");
+      const uint32_t here = held;
+      held = held_next;
       if (count > 2) entries(2);
-      if (count > 1) held[1] = request(1, 1);
+      if (count > 1) held_next = request(1, 1);
+      logits(&lds[wave][2 * 2 * kBuf], x);
+      settle(int32_t(tile0) * kTile, here);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    uint32_t buf = 0;  // of tile i: i % kStages
+    uint32_t buf = 0;  // of step i: i % kStages
     for (int32_t i = 0; i < count; ++i) {
-      // requested in this order: tile i, the entries of tile i + 2, tile i + 1;
+      // requested in this order: step i, the entries of step i + 2, step i + 1;
       // all but the last have landed
       if (i + 1 < count) CBK_WAIT_VM_LGKM0(kInsts);
       else CBK_WAIT_VM_LGKM0(0);
       asm volatile("" ::: "memory");
-      const uint32_t here = held[0];
-      held[0] = held[1];
+      const uint32_t here = held;
+      held = held_next;
       if (i + 3 < count) entries(i + 3);
-      if (i + 2 < count) held[1] = request(i + 2, buf == 0 ? 2 : buf - 1);  // the buffer of tile i - 1
+      if (i + 2 < count) held_next = request(i + 2, buf == 0 ? 2 : buf - 1);  // the buffer of step i - 1
       const char* kb = &lds[wave][buf * 2 * kBuf];
       const char* vb = kb + kBuf;
       buf = buf == kStages - 1 ? 0 : buf + 1;
-      const int32_t key0 = int32_t(tile0 + turns * i) * kTile;
-      const bool masked = here != ~0u || key0 + kTile > int32_t(len - a.rows + 1);
-
-      auto step = [&](auto mask) __attribute__((always_inline)) {
-        constexpr bool MASK = decltype(mask)::value;
-        // S^T: x[u][i] is the logit (log2 units) of key 8 j + 4 (u VT + v) + i and column c's row
-        f32x4 x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          f32x4 acc[NG];
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const float init = -kLess * qs[g];
-            acc[g] = f32x4{init, init, init, init};
-#pragma unroll
-            for (int t = 0; t < VT; ++t) {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + t) + c) * RB + 16 * g + 4 * j);
-              const s16x8 kf = operand<KF>(w);
-#pragma unroll
-              for (int p = 0; p < QP; ++p) acc[g] = mma<KF>(kf, qf[p][t][g], acc[g]);
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t* sw = reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
-            float s = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              s = fmaf(__uint_as_float(sw[g] << 16), acc[g][r], s);
-              s = fmaf(__uint_as_float(sw[g] & 0xffff0000u), qs[g], s);
-            }
-            x[u][r] = s * c2;
-          }
+      if (i + 1 < count) {
+        f32x4 next[U];
+        if (masked) {
+          logits(kb, next);
+          sums(vb, std::true_type());
+        } else {
+          logits(kb, next);
+          sums(vb, std::false_type());
         }
-        // which of the lane's keys its row sees: bit 4 t + i of `seen`
-        uint32_t seen = 0xffu;
-        if constexpr (MASK) {
-          const int32_t left = last_key - key0 - int32_t(8 * j) + 1;  // of the lane's 8 keys
-          seen = (here >> (8 * j)) & 0xffu;
-          seen &= left <= 0 ? 0u : left >= 8 ? 0xffu : (1u << left) - 1u;
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (!((seen >> (4 * (u * VT + v) + r)) & 1u)) x[u][r] = kNegInf;
-        }
-        float lm = x[0][0];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) lm = fmaxf(lm, x[u][r]);
-        if (__any(lm > m + kRescale)) {  // rare: raise the reference of the columns that need it
-          float bm = fmaxf(lm, __shfl_xor(lm, 16));
-          bm = fmaxf(bm, __shfl_xor(bm, 32));
-          const float mn = fmaxf(m, bm);
-          const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-          m = mn;
-          l *= alpha;
-          float ao[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) ao[r] = __shfl(alpha, int(4 * j + r));
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            zsum[g] *= alpha;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              o[2 * g][r] *= ao[r];
-              o[2 * g + 1][r] *= ao[r];
-            }
-          }
-        }
-        const float ms = m == kNegInf ? 0.f : m;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - ms);  // p from here on
-            l += x[u][r];
-          }
-        // O += (p step) . n: p step in bf16 parts, operand word r key r of the
-        // first half in its low half, of the second in its high half
-        u32x4 pw[NG][PP];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float y[NG][U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const uint32_t* sw = reinterpret_cast<const uint32_t*>(vb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
-            const bool sees = !MASK || ((seen >> (4 * (u * VT + v) + r)) & 1u);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              const uint32_t word = sees ? sw[g] : 0u;  // a masked key's step and offset may be anything
-              y[g][u] = x[u][r] * __uint_as_float(word << 16);
-              float z = __uint_as_float(word & 0xffff0000u);
-              if constexpr (VF == Form::kExact) z = fmaf(8.f, __uint_as_float(word << 16), z);
-              zsum[g] = fmaf(x[u][r], z, zsum[g]);
-            }
-          }
-#pragma unroll
-          for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int q = 0; q < PP; ++q) {
-              if (q + 1 < PP) {  // the upper halves, and what is left
-                pw[g][q][r] = VT == 1 ? __builtin_amdgcn_perm(__float_as_uint(y[g][U - 1]), __float_as_uint(y[g][0]), 0x07060302u)
-                                      : __builtin_amdgcn_perm(0u, __float_as_uint(y[g][0]), place);
-#pragma unroll
-                for (int u = 0; u < U; ++u) y[g][u] -= __uint_as_float(__float_as_uint(y[g][u]) & 0xffff0000u);
-              } else {
-                pw[g][q][r] = pack_bf16(y[g][0], y[g][U - 1]) & (VT == 1 ? 0xffffffffu : half);
-              }
-            }
-        }
-        const uint32_t from = (16 * ((c >> 2) & 1) + 4 * j + (c & 3)) * RB + (c >> 3) * 8;  // the row of key 8 j + c % 8
-        const s16x8 less = __builtin_bit_cast(s16x8, u32x4(0xc300c300u));  // -128
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-              (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) const void*)(vb + from + 16 * g)));
-          const s16x8 vf[2] = {operand<VF, 8>(uint32_t(w[0])), operand<VF, 8>(uint32_t(w[1]))};
-#pragma unroll
-          for (int q = 0; q < PP; ++q) {
-            const s16x8 pf = __builtin_bit_cast(s16x8, pw[g][q]);
-#pragma unroll
-            for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, vf[d], o[2 * g + d]);
-            if constexpr (VF != Form::kExact)
-#pragma unroll
-              for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, less, o[2 * g + d]);
-          }
-        }
-      };
-      if (masked) step(std::true_type());
-      else step(std::false_type());
-      // the reads of this tile's buffer are done before the next requests into it
+        for (int u = 0; u < U; ++u) x[u] = next[u];
+        settle(int32_t(tile0 + turns * (i + 1)) * kTile, here);
+      } else {
+        sums(vb, std::true_type());
+      }
+      // the reads of this step's buffer are done before the next requests into it
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 
