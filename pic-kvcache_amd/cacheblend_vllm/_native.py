@@ -246,8 +246,14 @@ def check(rc: int, what: str) -> None:
     raise RuntimeError(f"{text} ({load().cbk_error_string(rc).decode()})")
 
 
+# the current stream's handle without a Stream object around it (1.8 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
     """hipStream_t of torch's current stream on ``device``."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .kv_layout import KVLayer, int4_geometry, kv_desc
+from .kv_layout import KVLayer, int4_geometry, paged_layer
 
 
 def blend_attention(
@@ -84,7 +84,7 @@ def _whole_int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
             raise ValueError(f"whole numbers expected, got {t.dtype}")
         if t.dtype in (torch.int64, torch.uint32, torch.uint64):
             t = t.to(torch.int64).clamp(-1, (1 << 31) - 1)
-    return t.to(device=device, dtype=torch.int32, non_blocking=True)
+    return t if t.dtype == torch.int32 and t.device == device else t.to(device=device, dtype=torch.int32)
 
 
 def _check_out(out: torch.Tensor, query: torch.Tensor) -> None:
@@ -233,8 +233,8 @@ def paged_attention_int4(
         raise ValueError("query must be [batch, q_heads, head_size] or [batch, rows, q_heads, head_size]")
     if query.dtype not in _native.DTYPE_CODES:
         raise ValueError(f"dtype {query.dtype} is not supported")
-    desc, plane = kv_desc(kv_layer, block_size)
-    hkv, d = int4_geometry(plane)
+    desc, row, plane = paged_layer(kv_layer, block_size)
+    hkv, d = int4_geometry(plane.dtype, row)
     device = query.device
     if plane.device != device:
         raise ValueError(f"query is on {device}, the cache on {plane.device}")
@@ -269,7 +269,9 @@ def paged_attention_int4(
     tables = _whole_int32(block_tables, device)
     if width and tables.stride(1) != 1:
         tables = tables.contiguous()
-    lens = _whole_int32(context_lens.reshape(-1), device).contiguous()
+    lens = _whole_int32(context_lens, device)
+    if not lens.is_contiguous():
+        lens = lens.contiguous()
     o = out if out.dim() == 4 else out.unsqueeze(1)
     lib = _native.load()
     nbytes = _native.on_device(device, lib.cbk_paged_attention_int4_workspace_bytes, batch, rows, hq, hkv, d,

@@ -97,6 +97,29 @@ def kv_desc(kv_layer: KVLayer, block_size: int) -> tuple[_native.KVDesc, torch.T
     return desc, key
 
 
+def paged_layer(kv_layer: KVLayer, block_size: int) -> tuple[_native.KVDesc, tuple, torch.Tensor]:
+    """``kv_desc`` without making the planes' views where one tensor holds both
+    (3 of the 20 us that a call of one token takes): (desc, row shape, the tensor
+    or K)."""
+    if isinstance(kv_layer, torch.Tensor) and kv_layer.is_cuda and kv_layer.ndim >= 4:
+        shape, strides = kv_layer.shape, kv_layer.stride()
+        at = 0 if shape[0] == 2 else 1  # where K and V are
+        if shape[at] == 2:
+            blocks, row, tokens = shape[1 - at], shape[3:], shape[2]
+            if len(row) and 0 < block_size <= tokens:
+                es, expected = kv_layer.element_size(), 1
+                for n, stride in zip(reversed(row), reversed(strides[3:])):
+                    if n != 1 and stride != expected:
+                        break
+                    expected *= n
+                else:
+                    base = kv_layer.data_ptr()
+                    return _native.KVDesc(base, base + strides[at] * es, blocks, block_size, strides[1 - at] * es,
+                                          strides[2] * es, expected * es), row, kv_layer
+    desc, key = kv_desc(kv_layer, block_size)
+    return desc, key.shape[2:], key
+
+
 def _device_slots(slot_mapping: torch.Tensor, device: torch.device, num_slots: int) -> torch.Tensor:
     """Reference kv_layout.py:23-24, plus a host-side range check."""
     if slot_mapping.device.type == "cpu" and slot_mapping.numel():
@@ -204,6 +227,16 @@ def scatter_paged_kv(
     _native.check(rc, "scatter_paged_kv")
 
 
+def _device_list(t: torch.Tensor, device: torch.device, num_slots: int | None = None) -> torch.Tensor:
+    """One int64 entry a token on ``device`` (as it is, where it is that), slots checked if on the host."""
+    if t.dtype == torch.int64 and t.device == device and t.is_contiguous():
+        return t
+    t = t.reshape(-1)
+    if num_slots is not None:
+        return _device_slots(t, device, num_slots)
+    return t.to(device=device, dtype=torch.int64).contiguous()
+
+
 INT4_GROUP = 32  # dims of a 4-bit row that share a step and an offset
 
 
@@ -218,21 +251,19 @@ def int4_row_bytes(head_size: int) -> int:
     return head_size // INT4_GROUP * (INT4_GROUP // 2 + 4)
 
 
-def int4_geometry(plane: torch.Tensor) -> tuple[int, int]:
-    """(kv_heads, head_size) of a 4-bit plane ``[num_blocks, block_size, kv_heads, bytes]``."""
+def int4_geometry(dtype: torch.dtype, row: tuple) -> tuple[int, int]:
+    """(kv_heads, head_size) of 4-bit pages with rows ``[kv_heads, bytes]``."""
     per_group = INT4_GROUP // 2 + 4
-    if plane.dtype != torch.uint8 or plane.ndim != 4 or plane.shape[3] == 0 or plane.shape[3] % per_group:
-        raise ValueError(
-            f"4-bit pages must be uint8 [num_blocks, block_size, kv_heads, a multiple of {per_group}], "
-            f"got {plane.dtype} {tuple(plane.shape)}"
-        )
-    return plane.shape[2], plane.shape[3] // per_group * INT4_GROUP
+    if dtype != torch.uint8 or len(row) != 2 or row[1] == 0 or row[1] % per_group:
+        raise ValueError(f"4-bit pages must be uint8 with rows [kv_heads, a multiple of {per_group}], "
+                         f"got {dtype} {tuple(row)}")
+    return row[0], row[1] // per_group * INT4_GROUP
 
 
 def _check_rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, out: bool = False) -> None:
     """[tokens, heads, head_size] with contiguous dims, of ``like``'s type and device; rows apart if written."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must match the keys' dtype and device")
     if t.stride(2) != 1 and shape[2] > 1:
@@ -277,24 +308,24 @@ def append_paged_kv(
     rows in the outputs. The slots that are written must differ from each other:
     of two tokens with one slot, either's values may stay.
     """
-    desc, plane = kv_desc(kv_layer, block_size)
+    desc, row, plane = paged_layer(kv_layer, block_size)
     if key.dim() != 3:
         raise ValueError("key must be [tokens, kv_heads, head_size]")
     if key.dtype not in _native.DTYPE_CODES:
         raise ValueError(f"dtype {key.dtype} is not supported")
     if key.device != plane.device:
         raise ValueError(f"key is on {key.device}, the cache on {plane.device}")
-    shape = tuple(key.shape)
+    shape = key.shape
     tokens, heads, head_size = shape
     _check_rows(key, "key", shape, key)
     _check_rows(value, "value", shape, key)
     int4 = plane.dtype == torch.uint8
     if int4:
-        if int4_geometry(plane) != (heads, head_size):
-            raise ValueError(f"4-bit pages of {tuple(plane.shape[2:])} bytes a token do not hold rows of {shape[1:]}")
-    elif plane.dtype != key.dtype or tuple(plane.shape[2:]) != shape[1:]:
+        if int4_geometry(plane.dtype, row) != (heads, head_size):
+            raise ValueError(f"4-bit pages of {tuple(row)} bytes a token do not hold rows of {tuple(shape[1:])}")
+    elif plane.dtype != key.dtype or row != shape[1:]:
         raise ValueError(
-            f"the pages hold {plane.dtype} rows {tuple(plane.shape[2:])}, the keys are {key.dtype} {shape[1:]}"
+            f"the pages hold {plane.dtype} rows {tuple(row)}, the keys are {key.dtype} {tuple(shape[1:])}"
         )
     q_heads = 0
     if query is not None:
@@ -337,13 +368,14 @@ def append_paged_kv(
     if heads == 0 or head_size == 0:
         raise ValueError("key must have heads and dims")
     device = key.device
-    slots = _device_slots(slot_mapping.reshape(-1), device, desc.num_blocks * block_size)
+    slots = _device_list(slot_mapping, device, desc.num_blocks * block_size)
     pos = None
     if table is not None:
-        pos = positions.reshape(-1).to(device=device, dtype=torch.int64).contiguous()
+        pos = _device_list(positions, device)
         if table.dtype not in _native.DTYPE_CODES:
             table = table.float()
-        table = table.to(device)
+        if table.device != device:
+            table = table.to(device)
         if table.stride(1) != 1:
             table = table.contiguous()
     q = (query.data_ptr(), query.stride(0), query.stride(1)) if q_heads else (None, 0, 0)
@@ -370,35 +402,36 @@ def gather_paged_kv_int4(
     """:func:`gather_paged_kv` of a 4-bit layer (:func:`int4_row_bytes`) as values
     ``[2, tokens, kv_heads, head_size]`` of ``dtype`` (or ``out``'s): one launch
     (cbk_paged_gather_int4). Slots as there."""
-    desc, plane = kv_desc(kv_layer, block_size)
-    heads, head_size = int4_geometry(plane)
-    tokens = int(slot_mapping.numel())
+    desc, row, plane = paged_layer(kv_layer, block_size)
+    heads, head_size = int4_geometry(plane.dtype, row)
+    device = plane.device
+    tokens = slot_mapping.numel()
     shape = (2, tokens, heads, head_size)
     if out is not None:
-        if tuple(out.shape) != shape:
+        if out.shape != shape:
             raise ValueError(f"gather output has shape {tuple(out.shape)}, expected {shape}")
-        if out.device != plane.device:
+        if out.device != device:
             raise ValueError("gather output must be on the KV cache's device")
         dtype = out.dtype
     if dtype not in _native.DTYPE_CODES:
         raise ValueError(f"dtype {dtype} is not supported")
-    target = torch.empty(shape, dtype=dtype, device=plane.device) if out is None else out
+    target = torch.empty(shape, dtype=dtype, device=device) if out is None else out
     if tokens == 0 or heads == 0:
         return target
     es = target.element_size()
-    direct = (
-        _plane_rows_ok(target[0])
-        and target.stride(0) != 0
-        and (tokens == 1 or target.stride(1) >= heads * head_size)
-        and (target.data_ptr() | target.stride(0) * es | target.stride(1) * es) % 16 == 0
+    direct = out is None or (
+        _rows_contiguous(out, 2)
+        and out.stride(0) != 0
+        and (tokens == 1 or out.stride(1) >= heads * head_size)
+        and (out.data_ptr() | out.stride(0) * es | out.stride(1) * es) % 16 == 0
     )
-    dst = target if direct else torch.empty(shape, dtype=dtype, device=plane.device)
-    row = dst.stride(1) if tokens > 1 else heads * head_size
-    slots = _device_slots(slot_mapping.reshape(-1), plane.device, desc.num_blocks * block_size)
+    dst = target if direct else torch.empty(shape, dtype=dtype, device=device)
+    slots = _device_list(slot_mapping, device, desc.num_blocks * block_size)
+    plane_stride, token_stride = dst.stride(0), dst.stride(1) if tokens > 1 else heads * head_size
+    base = dst.data_ptr()
     rc = _native.on_device(
-        plane.device, _native.load().cbk_paged_gather_int4, desc, slots.data_ptr(), tokens, heads, head_size,
-        _native.DTYPE_CODES[dtype], dst[0].data_ptr(), dst[1].data_ptr(), row * es,
-        _native.stream_handle(plane.device),
+        device, _native.load().cbk_paged_gather_int4, desc, slots.data_ptr(), tokens, heads, head_size,
+        _native.DTYPE_CODES[dtype], base, base + plane_stride * es, token_stride * es, _native.stream_handle(device),
     )
     _native.check(rc, "gather_paged_kv_int4")
     if dst is not target:

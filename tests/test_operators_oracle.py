@@ -100,11 +100,10 @@ def test_4_bit_geometry():
     for d in (0, -32, 33, 48):
         with pytest.raises(ValueError, match="multiple of 32"):
             int4_row_bytes(d)
-    assert int4_geometry(torch.empty(4, 16, 2, 80, dtype=torch.uint8)) == (2, 128)
-    for bad in (torch.empty(4, 16, 2, 80), torch.empty(4, 16, 160, dtype=torch.uint8),
-                torch.empty(4, 16, 2, 72, dtype=torch.uint8), torch.empty(4, 16, 2, 0, dtype=torch.uint8)):
+    assert int4_geometry(torch.uint8, (2, 80)) == (2, 128)
+    for bad in ((torch.float32, (2, 80)), (torch.uint8, (160,)), (torch.uint8, (2, 72)), (torch.uint8, (2, 0))):
         with pytest.raises(ValueError, match="4-bit pages"):
-            int4_geometry(bad)
+            int4_geometry(*bad)
 
 
 def test_cpu_tensors_are_refused():
