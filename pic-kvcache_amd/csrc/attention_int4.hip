@@ -13,16 +13,23 @@
 //   q . key   = sum_g step_g (sum_{d in g} q_d n_d) + offset_g (sum_{d in g} q_d)
 //   out_d     = sum_k (p_k step_g) n_d + sum_k p_k offset_g
 //
-// so the inner sums are v_mfma_f32_16x16x32_bf16 products of small whole
-// numbers, exact in bf16, made from the codes by one and-or per two: 0x4300 | n
-// is 128 + n, and 128 times the other operand's sum is taken off again: before
-// the first product of q, and by a product with -128 after each of p, so that
-// the running sums stay small. (For float32 the codes are converted, to n - 8
-// for the values: the two sums of out_d then do not cancel.) The other operand
-// is cut into bf16 parts: q exactly (one part for bf16, two for f16, three for
-// float32), p step into two or three, the last rounded to nearest (2^-16, 2^-23
-// of it; cut off instead it would be a bias, which a long context's sums of
-// both signs do not forgive).
+// so the inner sums are products of small whole numbers on the matrix cores, the
+// codes in a form that takes little work:
+//  - beside q (16 bits) a byte 0000nnnn is the e4m3 value n 2^-9, for n below 8
+//    as below 16 (the subnormal numbers and the first binade are evenly spaced):
+//    two masks make 8 codes an operand. q, divided by a power of two of its row
+//    that leaves its largest element at 128 to 256, is cut into two (bf16) or
+//    three (f16) e4m3 parts, which hold it to 2^-18 of that element.
+//  - beside p step a halfword 0x4300 | n is the bf16 value 128 + n, one and-or
+//    for two codes; a product with -128 follows, so that the running sums stay
+//    small.
+//  - float32 converts the codes, to n - 8 for the values: the two sums of out_d
+//    then do not cancel; q is three bf16 parts.
+// sum_g offset_g (sum q_d) is one more product: a row's steps and offsets, as
+// they are stored, with the sums of q in three bf16 parts. p step is cut into
+// two bf16 parts (float32: three), the last rounded to nearest (2^-16, 2^-23 of
+// it; cut off instead it would be a bias, which a long context's sums of both
+// signs do not forgive).
 //
 // A wave takes 32 keys of one KV head at a time, their rows staged in its own
 // LDS by DMA two steps ahead (no barrier in the loop): a step's buffer holds V
@@ -62,7 +69,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kMergeThreads = 256;
 constexpr int kTile = 32;   // keys of a wave's step
 constexpr int kStages = 3;  // tiles in a wave's LDS
 // waves of a workgroup, at most (float32 takes the registers of 8 with 4)
@@ -153,9 +159,9 @@ __device__ __forceinline__ void lds_dma_word(const void* addr, uint32_t lds) {
                : "=&s"(saved) : "s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(addr) : "memory");
 }
 
-// How codes n become an MFMA operand: as bf16 128 + n, as f16 1024 + n, or
-// converted to bf16 n - LESS.
-enum class Form { kBf16, kF16, kExact };
+// How codes n become an MFMA operand: as bf16 128 + n, or converted to bf16 n -
+// LESS (beside q of 16 bits: as e4m3 n 2^-9).
+enum class Form { kBf16, kExact, kFp8 };
 
 // 8 codes of a word as 8 operand elements, in the order 0 4 1 5 2 6 3 7.
 template <Form F, int LESS = 0>
@@ -170,7 +176,7 @@ __device__ __forceinline__ s16x8 operand(uint32_t w) {
     r[2] = pair(f(even, 1), f(even, 3));
     r[3] = pair(f(odd, 1), f(odd, 3));
   } else {
-    const uint32_t mask = 0x000f000fu, one = F == Form::kF16 ? 0x64006400u : 0x43004300u;
+    const uint32_t mask = 0x000f000fu, one = 0x43004300u;
     // (and, or in one instruction: the compiler takes two for two constants.
     // No inline assembly: the hazards between what it writes and what a matrix
     // instruction still reads would go unseen)
@@ -180,14 +186,48 @@ __device__ __forceinline__ s16x8 operand(uint32_t w) {
   return __builtin_bit_cast(s16x8, r);
 }
 
-template <Form F>
 __device__ __forceinline__ f32x4 mma(const s16x8& a, const s16x8& b, const f32x4& c) {
-  typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-  if constexpr (F == Form::kF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+
+// The operands of q . n: QParts of q, and the codes' words.
+template <Form F> struct QOperand;
+template <> struct QOperand<Form::kExact> {
+  typedef s16x8 Q;
+  static __device__ __forceinline__ s16x8 codes(uint32_t w) { return operand<Form::kExact>(w); }
+  static __device__ __forceinline__ f32x4 mul(const s16x8& k, const Q& q, const f32x4& c) { return mma(k, q, c); }
+  // 8 elements' upper 8 bits, in the codes' order; x: what is left
+  static __device__ __forceinline__ Q cut(float (&x)[8]) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(__float_as_uint(x[i + 4]), __float_as_uint(x[i]), 0x07060302u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] -= __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
+    return __builtin_bit_cast(s16x8, w);
+  }
+};
+template <> struct QOperand<Form::kFp8> {
+  typedef u32x2 Q;
+  // in the order 0 2 4 6 1 3 5 7
+  static __device__ __forceinline__ u32x2 codes(uint32_t w) { return u32x2{w & 0x0f0f0f0fu, (w >> 4) & 0x0f0f0f0fu}; }
+  static __device__ __forceinline__ f32x4 mul(const u32x2& k, const Q& q, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(__builtin_bit_cast(long, k), __builtin_bit_cast(long, q), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ Q cut(float (&x)[8]) {
+    Q r;
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[odd], x[odd + 2], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[odd + 4], x[odd + 6], w, true);
+      r[odd] = uint32_t(w);
+      x[odd] -= __builtin_amdgcn_cvt_f32_fp8(w, 0);
+      x[odd + 2] -= __builtin_amdgcn_cvt_f32_fp8(w, 1);
+      x[odd + 4] -= __builtin_amdgcn_cvt_f32_fp8(w, 2);
+      x[odd + 6] -= __builtin_amdgcn_cvt_f32_fp8(w, 3);
+    }
+    return r;
+  }
+};
 
 // two floats rounded to bf16, x in the low half
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
@@ -240,8 +280,8 @@ template <int DT> __device__ __forceinline__ void store_elem(void* p, int64_t at
 
 // The operands' parts, the form of the codes beside q and beside p step.
 template <int DT> struct Parts;
-template <> struct Parts<CBK_DTYPE_BF16> { static constexpr int q = 1, p = 2; static constexpr Form k = Form::kBf16, v = Form::kBf16; };
-template <> struct Parts<CBK_DTYPE_F16> { static constexpr int q = 1, p = 2; static constexpr Form k = Form::kF16, v = Form::kBf16; };
+template <> struct Parts<CBK_DTYPE_BF16> { static constexpr int q = 2, p = 2; static constexpr Form k = Form::kFp8, v = Form::kBf16; };
+template <> struct Parts<CBK_DTYPE_F16> { static constexpr int q = 3, p = 2; static constexpr Form k = Form::kFp8, v = Form::kBf16; };
 template <> struct Parts<CBK_DTYPE_F32> { static constexpr int q = 3, p = 3; static constexpr Form k = Form::kExact, v = Form::kExact; };
 
 template <int DT, int NG, int VT, int PIECE>
@@ -249,7 +289,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
   constexpr int kMax = max_waves(DT);
   constexpr int QP = Parts<DT>::q, PP = Parts<DT>::p;
   constexpr Form KF = Parts<DT>::k, VF = Parts<DT>::v;
-  constexpr float kLess = KF == Form::kF16 ? 1024.f : KF == Form::kBf16 ? 128.f : 0.f;  // in the codes beside q
+  using QO = QOperand<KF>;
   constexpr int D = 32 * NG, RB = kInt4GroupBytes * NG;  // dims and bytes of a head's row
   constexpr int U = 2 / VT, COLS = 16 / VT;
   constexpr uint32_t kBuf = kTile * RB;                      // K or V rows of a tile
@@ -320,39 +360,58 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
     const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
     const int32_t last_key = live ? int32_t(len) - int32_t(a.rows) + int32_t(qr) : -1;  // the row sees keys up to it
 
-    // Q operands and the sums of their groups
-    s16x8 qf[QP][VT][NG];
-    float qs[NG];
+    // Q operands (zero outside a half's column group), and the sums of their
+    // groups as the operand beside the steps and offsets: lane group j has part j
+    typename QO::Q qf[QP][VT][NG];
+    s16x8 qsum;
+    float unit = c2;  // of S^T, in log2 units
+    {
+      float x[NG][8], top = 0.f;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int64_t from = int64_t(seq) * a.q_batch + int64_t(qr) * a.q_row + int64_t(qh) * a.q_head + 32 * g + 8 * j;
-      float x[8], sum = 0.f;
-      load_elems<DT>(a.q, from, a.q_pieces, live, x);
+      for (int g = 0; g < NG; ++g) {
+        const int64_t from = int64_t(seq) * a.q_batch + int64_t(qr) * a.q_row + int64_t(qh) * a.q_head + 32 * g + 8 * j;
+        load_elems<DT>(a.q, from, a.q_pieces, live, x[g]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] *= sign;
-        sum += x[e];
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[g][e]));
       }
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      qs[g] = sum;
+      float down = sign, inverse = 1.f;  // 1 / the row's unit
+      if constexpr (KF == Form::kFp8) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // the exponent of the largest element, within what keeps both powers normal
+        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -115), 115);
+        down *= __uint_as_float(uint32_t(127 + 7 - e) << 23);
+        unit *= 512.f * __uint_as_float(uint32_t(127 - 7 + e) << 23);  // and the codes' 2^9
+        inverse = 1.f / 512.f;
+      }
+      uint32_t part[NG];
 #pragma unroll
-      for (int p = 0; p < QP; ++p) {
-        u32x4 w;
+      for (int g = 0; g < NG; ++g) {
+        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (KF == Form::kF16) {
-            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-            w[i] = __builtin_bit_cast(uint32_t, h2{_Float16(x[i]), _Float16(x[i + 4])});
-          } else {
-            w[i] = __builtin_amdgcn_perm(__float_as_uint(x[i + 4]), __float_as_uint(x[i]), 0x07060302u);
-          }
+        for (int e = 0; e < 8; ++e) {
+          x[g][e] *= down;
+          sum += x[g][e];
         }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        sum *= inverse;
+        const uint32_t hi = __float_as_uint(sum) & 0xffff0000u;
+        const float rest = sum - __uint_as_float(hi);
+        const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
+        const uint32_t low = __float_as_uint(rest - __uint_as_float(mid)) & 0xffff0000u;
+        part[g] = j == 0 ? hi : j == 1 ? mid : j == 2 ? low : 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] -= __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
+        for (int p = 0; p < QP; ++p) {
+          const typename QO::Q w = QO::cut(x[g]);
 #pragma unroll
-        for (int t = 0; t < VT; ++t) qf[p][t][g] = __builtin_bit_cast(s16x8, VT == 1 || v == uint32_t(t) ? w : u32x4(0u));
+          for (int t = 0; t < VT; ++t) qf[p][t][g] = VT == 1 || v == uint32_t(t) ? w : typename QO::Q(0);
+        }
       }
+      u32x4 w = u32x4(0u);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) w[g] = part[g];
+      qsum = __builtin_bit_cast(s16x8, w);
     }
 
     float m = kNegInf, l = 0.f, zsum[NG];
@@ -409,29 +468,35 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
     auto logits = [&](const char* kb, f32x4 (&s)[U]) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        // the offsets' part: of each half by itself, for a masked key's offset may
+        // be NaN, which the other half's zeros would not keep out
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+          const uint32_t* sw = reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + t) + c) * RB + 16 * NG);
+          u32x4 w = u32x4(0u);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) w[g] = sw[g];
+          const f32x4 part = mma(__builtin_bit_cast(s16x8, w), qsum, f32x4{0.f, 0.f, 0.f, 0.f});
+          s[u] = t == 0 || v == uint32_t(t) ? part : s[u];
+        }
         f32x4 acc[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const float init = -kLess * qs[g];
-          acc[g] = f32x4{init, init, init, init};
+          acc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int t = 0; t < VT; ++t) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + t) + c) * RB + 16 * g + 4 * j);
-            const s16x8 kf = operand<KF>(w);
+            const auto kf = QO::codes(*reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + t) + c) * RB + 16 * g + 4 * j));
 #pragma unroll
-            for (int p = 0; p < QP; ++p) acc[g] = mma<KF>(kf, qf[p][t][g], acc[g]);
+            for (int p = 0; p < QP; ++p) acc[g] = QO::mul(kf, qf[p][t][g], acc[g]);
           }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint32_t* sw = reinterpret_cast<const uint32_t*>(kb + (16 * (u * VT + v) + 4 * j + r) * RB + 16 * NG);
-          float sum = 0.f;
+          float sum = s[u][r];
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            sum = fmaf(__uint_as_float(sw[g] << 16), acc[g][r], sum);
-            sum = fmaf(__uint_as_float(sw[g] & 0xffff0000u), qs[g], sum);
-          }
-          s[u][r] = sum * c2;
+          for (int g = 0; g < NG; ++g) sum = fmaf(__uint_as_float(sw[g] << 16), acc[g][r], sum);
+          s[u][r] = sum * unit;
         }
       }
     };
@@ -530,10 +595,10 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
         for (int q = 0; q < PP; ++q) {
           const s16x8 pf = __builtin_bit_cast(s16x8, pw[g][q]);
 #pragma unroll
-          for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, vf[d], o[2 * g + d]);
+          for (int d = 0; d < 2; ++d) o[2 * g + d] = mma(pf, vf[d], o[2 * g + d]);
           if constexpr (VF != Form::kExact)
 #pragma unroll
-            for (int d = 0; d < 2; ++d) o[2 * g + d] = mma<VF>(pf, less, o[2 * g + d]);
+            for (int d = 0; d < 2; ++d) o[2 * g + d] = mma(pf, less, o[2 * g + d]);
         }
       }
     };
@@ -646,11 +711,12 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
 }
 
 // The sequences that more than one range holds, and those without keys: a
-// workgroup per row, every 32 lanes each eighth range of it (one 32 lanes for
-// all of 128 ranges took 46 us), each lane D / 32 dims.
-template <int DT, int D>
-__global__ __launch_bounds__(kMergeThreads) void int4_attn_merge_kernel(const Int4AttnArgs a) {
-  constexpr int N = D / 32, SUBS = kMergeThreads / 32;
+// workgroup per row, every 32 lanes each SUBS-th range of it, each lane D / 32
+// dims. 256 ranges of 32 rows: 46 us with one 32 lanes a row, 14 with 8, and
+// see launch() for 32.
+template <int DT, int D, int SUBS>
+__global__ __launch_bounds__(32 * SUBS) void int4_attn_merge_kernel(const Int4AttnArgs a) {
+  constexpr int N = D / 32;
   typedef float VecN __attribute__((ext_vector_type(N)));
   __shared__ float s_o[SUBS][D], s_l[SUBS], s_m[SUBS];
   const uint32_t seq = blockIdx.y;
@@ -767,7 +833,10 @@ int launch(const Int4AttnArgs& a, bool pieces16, hipStream_t s) {
   // 16-byte pieces of a row: whole ones, where the pages are aligned to them
   constexpr int P = kInt4GroupBytes * NG % 16 == 0 ? 16 : 4;
   if (int rc = pieces16 ? launch_pieces<DT, NG, P>(a, s) : launch_pieces<DT, NG, 4>(a, s)) return rc;
-  hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG>), dim3(a.rows * a.hq, a.batch), dim3(kMergeThreads), 0, s, a);
+  // a sequence of many ranges: more lanes for each of its rows
+  const dim3 grid(a.rows * a.hq, a.batch);
+  if (a.ranges > 16 * a.batch) hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG, 32>), grid, dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG, 8>), grid, dim3(256), 0, s, a);
   return launch_status("int4 attention merge");
 }
 

@@ -1,15 +1,17 @@
 """GPU: attention of single tokens over 4-bit pages, against 64 bits.
 
 Tolerance of a row. A logit sums, per 32 dims, products of a query element
-with a whole number below 144 (float32: 16), exact, and then step times that
-sum and offset times the query's sum: fewer than 64 float32 roundings on the
-way, of at most 2^-24 of the sum of the absolute terms each; taking it to log2
-units and the reference maximum off rounds it three times more. The weights
-then lose 2^-15 (two bf16 parts, cut; float32: three, 2^-23), their sums at
-most one rounding a key of a lane and the merges'. A relative change e of every
-weight moves an output by at most 2 e sum p |v|; last comes the type's own
-half step. With codes, |v| is replaced by what a value's two products hold:
-step * 144 + |offset|, rounded as often."""
+with a whole number below 16, exact, and then step times that sum and offset
+times the query's sum: fewer than 64 float32 roundings on the way, of at most
+2^-24 of the sum of the absolute terms each; taking it to log2 units and the
+reference maximum off rounds it three times more. 16-bit queries are cut into
+parts that hold an element to 2^-10 where the row's largest is 128 to 256, so to
+2^-17 of that one. The weights then lose 2^-16 (two bf16 parts, the second
+rounded; float32: three, 2^-23), their sums at most one rounding a key of a lane
+and the merges'. A relative change e of every weight moves an output by at most
+2 e sum p |v|; last comes the type's own half step. With codes, |v| is replaced
+by what a value's products hold: step * 144 (the codes are 128 to 143 there,
+and 128 is taken off; float32: step * 16) + |offset|, rounded as often."""
 
 import numpy as np
 import pytest
@@ -50,12 +52,13 @@ def _bound(q, pages, tables, lens, scale, dtype, want, mass):
     k_pages, v_pages = (p.cpu().numpy() for p in KL.kv_planes(pages))
     size, heads, d = k_pages.shape[1], k_pages.shape[2], q.shape[3]
     exact = dtype == F32
-    top = 16 if exact else 144
-    # per head: the largest sum of absolute terms of a group's logit part, and of a value
+
+    # steps and offsets [.., groups]
     def held(p):
         words = np.ascontiguousarray(p[..., d // 2:]).view(np.uint16).astype(np.uint32) << 16
         both = words.view(np.float32).reshape(*p.shape[:-1], d // 32, 2)
-        return np.abs(both[..., 0]) * top + np.abs(both[..., 1])
+        return np.abs(both[..., 0]), np.abs(both[..., 1])
+
     tol = np.zeros(want.shape)
     for b, n in enumerate(lens):
         if n == 0:
@@ -65,11 +68,15 @@ def _bound(q, pages, tables, lens, scale, dtype, want, mass):
         ok = (page >= 0) & (page < k_pages.shape[0])
         if not ok.any():
             continue
-        hk, hv = (held(p[page[ok], at[ok] % size]) for p in (k_pages, v_pages))  # [n, heads, groups]
+        (ks, ko), (vs, vo) = (held(p[page[ok], at[ok] % size]) for p in (k_pages, v_pages))  # [n, heads, groups]
+        hk, hv = 16 * ks + ko, (16 if exact else 144) * vs + vo
         qs = np.abs(q[b]).reshape(q.shape[1], q.shape[2], d // 32, 32).sum(axis=-1)  # [rows, hq, groups]
         group = q.shape[2] // heads
         terms = np.einsum("rhg,nhg->rhn", qs, hk.repeat(group, axis=1)).max(axis=-1) * abs(scale)
         e = 67 * 2.0 ** -24 * terms + (2.0 ** -22 if exact else 2.0 ** -15) + (n / 16 + 64) * 2.0 ** -24
+        if not exact:  # the queries' parts
+            cut = 2.0 ** -17 * np.abs(q[b]).max(axis=-1) * 32 * 15 * ks.sum(axis=-1).max(axis=0).repeat(group)
+            e = e + abs(scale) * cut
         values = hv.max(axis=0).repeat(group, axis=0).repeat(32, axis=1)  # [hq, d]
         tol[b] = 2 * e[..., None] * mass[b] + (n / 16 + 64) * 2.0 ** -24 * values
     return tol + torch.finfo(dtype).eps / 2 * np.abs(want) + (2.0 ** -25 if dtype == F16 else 1e-30)
