@@ -10,14 +10,13 @@
 // the table; products and differences in float32, each rounded, then once to
 // the type (4-bit keys: in 64 bits).
 //
-// Bound by HBM: every row is read once and written once. A thread takes 16
-// dims of one head as two 16-byte pieces, the two halves of 8 pairs, so that
-// no pair is read twice and in-place outputs are safe; the threads of a wave
-// cover whole heads of one token after another.
+// Bound by HBM: every row is read once and written once (8192 tokens of 32 + 2 x
+// 8 heads x 128 bf16: 37 us, 5.6 TB/s). A thread takes 16 dims of one head as
+// two 16-byte pieces, the two halves of 8 pairs, so that no pair is read twice
+// and in-place outputs are safe; the threads of a wave cover whole heads of one
+// token after another.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
-
-#include <type_traits>
 
 #include "int4_rows.hpp"
 
@@ -31,6 +30,11 @@ struct Rows {  // [tokens, heads, head_dim], strides in elements
   const void* base;
   int64_t token_stride, head_stride;
 };
+
+// field by field: a choice of addresses would put the kernel's arguments into scratch memory
+__device__ __forceinline__ Rows choose(bool first, const Rows& a, const Rows& b) {
+  return Rows{first ? a.base : b.base, first ? a.token_stride : b.token_stride, first ? a.head_stride : b.head_stride};
+}
 
 struct AppendArgs {
   Rows query, key, value;
@@ -54,9 +58,7 @@ struct AppendArgs {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef double f64x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 // element conversions of the three types, one at a time (the general kernel)
 // and eight at a time
@@ -92,16 +94,24 @@ __device__ __forceinline__ f32x8 load8(const void* base, int64_t at) {
   }
 }
 
-template <int DT>
+template <int DT, bool STREAM = false>
 __device__ __forceinline__ void store8(void* base, int64_t at, const f32x8& x) {
   typedef typename Elem<DT>::T T8 __attribute__((ext_vector_type(8)));
   typename Elem<DT>::T* p = static_cast<typename Elem<DT>::T*>(base) + at;
   if constexpr (DT == CBK_DTYPE_F32) {
     f32x4* w = reinterpret_cast<f32x4*>(p);
-    w[0] = __builtin_shufflevector(x, x, 0, 1, 2, 3);
-    w[1] = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+    const f32x4 lo = __builtin_shufflevector(x, x, 0, 1, 2, 3), hi = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+    if constexpr (STREAM) {
+      __builtin_nontemporal_store(lo, w);
+      __builtin_nontemporal_store(hi, w + 1);
+    } else {
+      w[0] = lo;
+      w[1] = hi;
+    }
   } else {
-    *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, __builtin_convertvector(x, T8));
+    const u32x4 bits = __builtin_bit_cast(u32x4, __builtin_convertvector(x, T8));
+    if constexpr (STREAM) __builtin_nontemporal_store(bits, reinterpret_cast<u32x4*>(p));
+    else *reinterpret_cast<u32x4*>(p) = bits;
   }
 }
 
@@ -160,59 +170,92 @@ __device__ __forceinline__ void group_extremes(double& low, double& high, bool& 
   }
 }
 
-// 8 values of a 32-dim group held by 4 neighbouring lanes (NEOX), or 16 by 2:
-// the codes as one or two words, and the group's scale word.
-template <int N, typename V>
-__device__ __forceinline__ uint32_t codes(const V (&x)[N], uint32_t (&word)[N]) {
-  double low = __builtin_inf(), high = -__builtin_inf();
-  bool finite = true;
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double v = double(x[n][e]);
-      low = fmin(low, v);
-      high = fmax(high, v);
-      finite = finite && fabs(v) < __builtin_inf();
-    }
-  group_extremes<4 / N>(low, high, finite);
-  const Int4Scale s = int4_scale(low, high, finite);
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    word[n] = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) word[n] |= int4_code(double(x[n][e]), s) << (4 * e);
+struct Extremes {
+  double low, high;
+  bool finite;
+  __device__ __forceinline__ void add(double v) {
+    low = fmin(low, v);
+    high = fmax(high, v);
+    finite = finite && fabs(v) < __builtin_inf();
   }
-  return int4_scale_word(s);
-}
+  __device__ __forceinline__ void join(const Extremes& o) {
+    low = fmin(low, o.low);
+    high = fmax(high, o.high);
+    finite = finite && o.finite;
+  }
+  // of a group in 4 lanes (quarters) or in 2
+  __device__ __forceinline__ Int4Scale scale(bool quarters) {
+    group_extremes<2>(low, high, finite);
+    const Extremes other{__shfl_xor(low, 2), __shfl_xor(high, 2), __shfl_xor(int(finite), 2) != 0};
+    if (quarters) join(other);
+    return int4_scale(low, high, finite);
+  }
+};
 
-// The 16 dims of a thread: [d0, d0 + 8) and [d1, d1 + 8).
-template <typename V>
-__device__ __forceinline__ void store_codes(char* row, uint32_t head_dim, bool halves, uint32_t d0, uint32_t d1, V (&x)[2]) {
-  auto scale_at = [&](uint32_t d) { return reinterpret_cast<uint32_t*>(row + head_dim / 2 + d / kInt4Group * 4); };
-  if (halves) {  // each 8 are a quarter of a group of their own
+// A thread's 8 pairs (x, y), turned by (c, s) if TURN, to 4 bits. With `halves`
+// the x are [d0, d0 + 8), a quarter of a group of their own (the rest in the
+// neighbouring lanes), the y [d1, d1 + 8); otherwise x and y alternate over the
+// 16 dims from d0, half a group. The 64-bit values are computed twice, for the
+// extremes and for the codes, and never held: 96 registers instead of 148, so
+// that the queries' rows of the launch, bound by HBM, have five waves per SIMD
+// instead of three (8192 tokens of 32 + 2 x 8 heads x 128 bf16: 64.9 -> 51.7 us;
+// at six waves registers spill). `row` NULL: nothing is written.
+template <bool TURN>
+__device__ __forceinline__ void store_codes(char* row, uint32_t head_dim, bool halves, uint32_t d0, uint32_t d1, f32x8 xv,
+                                            f32x8 yv, f32x8 cv, f32x8 sv) {
+#pragma clang fp contract(off)
+  float x[8], y[8];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const uint32_t d = n ? d1 : d0;
-      const V one[1] = {x[n]};
-      uint32_t word[1];
-      const uint32_t sw = codes<1>(one, word);
-      *reinterpret_cast<uint32_t*>(row + d / 2) = word[0];
-      if (d % kInt4Group == 0) *scale_at(d) = sw;
-    }
-  } else {  // 16 neighbouring dims are half a group
-    uint32_t word[2];
-    const uint32_t sw = codes<2>(x, word);
-    reinterpret_cast<uint32_t*>(row + d0 / 2)[0] = word[0];
-    reinterpret_cast<uint32_t*>(row + d0 / 2)[1] = word[1];
-    if (d0 % kInt4Group == 0) *scale_at(d0) = sw;
+  for (int i = 0; i < 8; ++i) {
+    x[i] = xv[i];
+    y[i] = yv[i];
   }
+#define CBK_FIRST(i) (TURN ? double(x[i]) * double(cv[i]) - double(y[i]) * double(sv[i]) : double(x[i]))
+#define CBK_SECOND(i) (TURN ? double(y[i]) * double(cv[i]) + double(x[i]) * double(sv[i]) : double(y[i]))
+  Extremes ex{__builtin_inf(), -__builtin_inf(), true}, ey = ex;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    ex.add(CBK_FIRST(i));
+    ey.add(CBK_SECOND(i));
+  }
+  if (!halves) {
+    ex.join(ey);
+    ey = ex;
+  }
+  const Int4Scale sx = ex.scale(halves), sy = ey.scale(halves);
+  // (the values are not to be kept until here)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(x[i]), "+v"(y[i]));
+  uint32_t even = 0, odd = 0;  // codes of the x, of the y
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    even |= int4_code(CBK_FIRST(i), sx) << (4 * i);
+    odd |= int4_code(CBK_SECOND(i), sy) << (4 * i);
+  }
+#undef CBK_FIRST
+#undef CBK_SECOND
+  if (row == nullptr) return;
+  if (!halves) {  // x and y in turn: each half's four pairs of codes are a word
+    auto spread = [](uint32_t w) {  // 4 codes to the low halves of 4 bytes
+      w = (w | (w << 8)) & 0x00ff00ffu;
+      return (w | (w << 4)) & 0x0f0f0f0fu;
+    };
+    const uint32_t lo = spread(even & 0xffffu) | spread(odd & 0xffffu) << 4;
+    const uint32_t hi = spread(even >> 16) | spread(odd >> 16) << 4;
+    even = lo;
+    odd = hi;
+  }
+  *reinterpret_cast<uint32_t*>(row + d0 / 2) = even;
+  *reinterpret_cast<uint32_t*>(row + d1 / 2) = odd;
+  uint32_t* const words = reinterpret_cast<uint32_t*>(row + head_dim / 2);
+  if (d0 % kInt4Group == 0) words[d0 / kInt4Group] = int4_scale_word(sx);
+  if (halves && d1 % kInt4Group == 0) words[d1 / kInt4Group] = int4_scale_word(sy);
 }
 
 // One thread per 16 dims of a (token, head): rotary_dim is head_dim or 0,
 // everything 16-byte aligned, head_dim a multiple of 16 (4-bit pages: 64).
 template <int DT, bool INT4>
-__global__ __launch_bounds__(kThreads) void append_pieces_kernel(const AppendArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(INT4 ? 5 : 8))) void append_pieces_kernel(const AppendArgs a) {
   const uint32_t units = a.unit_div.d, per = kThreads / units;  // threads of a head, heads of a block
   const uint32_t local = a.unit_div.div(threadIdx.x), u = threadIdx.x - local * units;
   if (local >= per) return;
@@ -225,7 +268,7 @@ __global__ __launch_bounds__(kThreads) void append_pieces_kernel(const AppendArg
   const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.heads;
   if (!is_q) h -= a.q_heads;
   if (is_v) h -= a.heads;
-  const Rows& in = is_q ? a.query : is_v ? a.value : a.key;
+  const Rows in = choose(is_q, a.query, choose(is_v, a.value, a.key));
   const bool rotate = a.positions != nullptr && !is_v;
   // neox pairs lie half a head apart; the others, and rows not rotated, side by side
   const bool halves = a.neox && a.positions != nullptr;
@@ -238,32 +281,29 @@ __global__ __launch_bounds__(kThreads) void append_pieces_kernel(const AppendArg
     c = table8(a.table, a.table_dtype, tab);
     s = table8(a.table, a.table_dtype, tab + a.head_dim / 2);
   }
-  auto turned = [&](auto& y) {
-    if (!rotate) return;
-    using V = std::remove_reference_t<decltype(y[0])>;
-    const V cv = __builtin_convertvector(c, V), sv = __builtin_convertvector(s, V);
-    if (halves) {
-      turn(y[0], y[1], cv, sv);
-    } else {
-      V p = __builtin_shufflevector(y[0], y[1], 0, 2, 4, 6, 8, 10, 12, 14);
-      V q = __builtin_shufflevector(y[0], y[1], 1, 3, 5, 7, 9, 11, 13, 15);
-      turn(p, q, cv, sv);
-      y[0] = __builtin_shufflevector(p, q, 0, 8, 1, 9, 2, 10, 3, 11);
-      y[1] = __builtin_shufflevector(p, q, 4, 12, 5, 13, 6, 14, 7, 15);
-    }
-  };
+  // as pairs: the pieces themselves, or their even and odd dims
+  if (!halves) {
+    const f32x8 even = __builtin_shufflevector(x[0], x[1], 0, 2, 4, 6, 8, 10, 12, 14);
+    x[1] = __builtin_shufflevector(x[0], x[1], 1, 3, 5, 7, 9, 11, 13, 15);
+    x[0] = even;
+  }
   char* const page = tok.page < 0 ? nullptr : (is_v ? a.v_base : a.k_base) + tok.page;
   if constexpr (INT4) {
     if (!is_q) {  // whole heads: the lanes of a group are here together
-      f64x8 y[2] = {__builtin_convertvector(x[0], f64x8), __builtin_convertvector(x[1], f64x8)};
-      turned(y);
-      if (page) store_codes(page + int64_t(h) * int4_row_bytes(a.head_dim), a.head_dim, halves, d0, d1, y);
+      char* const row = page ? page + int64_t(h) * int4_row_bytes(a.head_dim) : nullptr;
+      if (rotate) store_codes<true>(row, a.head_dim, halves, d0, d1, x[0], x[1], c, s);
+      else store_codes<false>(row, a.head_dim, halves, d0, d1, x[0], x[1], c, s);
     }
   }
-  const Rows& out = is_q ? a.query_out : a.key_out;
+  const Rows out = choose(is_q, a.query_out, a.key_out);
   const bool copy = !is_v && out.base != nullptr;
-  if (INT4 ? !copy : false) return;
-  turned(x);
+  if (INT4 && !copy) return;
+  if (rotate) turn(x[0], x[1], c, s);
+  if (!halves) {
+    const f32x8 front = __builtin_shufflevector(x[0], x[1], 0, 8, 1, 9, 2, 10, 3, 11);
+    x[1] = __builtin_shufflevector(x[0], x[1], 4, 12, 5, 13, 6, 14, 7, 15);
+    x[0] = front;
+  }
   if constexpr (!INT4) {
     if (!is_q && page) {
       store8<DT>(page, int64_t(h) * a.head_dim + d0, x[0]);
@@ -296,7 +336,7 @@ __global__ __launch_bounds__(kThreads) void append_rows_kernel(const AppendArgs 
   const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.heads;
   if (!is_q) h -= a.q_heads;
   if (is_v) h -= a.heads;
-  const Rows& in = is_q ? a.query : is_v ? a.value : a.key;
+  const Rows in = choose(is_q, a.query, choose(is_v, a.value, a.key));
   const bool rotate = a.positions != nullptr && !is_v;
   const T* src = static_cast<const T*>(in.base) + int64_t(t) * in.token_stride + int64_t(h) * in.head_stride;
   const uint32_t half = a.rotary_dim / 2;
@@ -351,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void append_rows_kernel(const AppendArgs 
         if (lane + 64 * i < a.head_dim) dst[lane + 64 * i] = E::put(x[i]);
     }
   }
-  const Rows& out = is_q ? a.query_out : a.key_out;
+  const Rows out = choose(is_q, a.query_out, a.key_out);
   if (is_v || out.base == nullptr) return;
   T* dst = static_cast<T*>(const_cast<void*>(out.base)) + int64_t(t) * out.token_stride + int64_t(h) * out.head_stride;
   const bool zero = rotate && !tok.placed;
@@ -361,8 +401,9 @@ __global__ __launch_bounds__(kThreads) void append_rows_kernel(const AppendArgs 
 }
 
 // Rows of 4-bit pages as values: a thread reads one word of codes and its
-// group's scale word and writes 8 values. Bound by HBM, mostly the values
-// written; a slot out of range gives a zero row.
+// group's scale word and writes 8 values, past the caches (65,531 tokens of 4 x
+// 128 bf16: 28.7 us, 6.1 TB/s; 40.3 through them). Bound by HBM, mostly the
+// values written; a slot out of range gives a zero row.
 struct GatherArgs {
   const char* k_base;
   const char* v_base;
@@ -397,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void gather_int4_kernel(const GatherArgs 
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = int4_value((word >> (4 * e)) & 15u, sw);
   }
-  store8<DT>(a.out_k + (is_v ? a.out_plane : 0) + int64_t(t) * a.out_token, int64_t(w) * 8, x);
+  store8<DT, true>(a.out_k + (is_v ? a.out_plane : 0) + int64_t(t) * a.out_token, int64_t(w) * 8, x);
 }
 
 template <bool INT4>
