@@ -119,11 +119,8 @@ __device__ __forceinline__ uint32_t context_of(const Int4AttnArgs& a, uint32_t b
 
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + kTile - 1) / kTile; }
 
-// All sequences' tiles, by a whole wave.
-__device__ uint32_t total_tiles(const Int4AttnArgs& a, uint32_t lane) {
-  uint32_t n = 0;
-  for (uint32_t b = lane; b < a.batch; b += 64) n += tiles_of(context_of(a, b));
-  return __builtin_amdgcn_readfirstlane(wave_sum_u32(n));
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_readlane(int(wave_inclusive_scan(v)), 63));
 }
 
 // LDS DMA from a 64-bit address per lane (the rows of pages anywhere): lane
@@ -313,23 +310,28 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
   const uint32_t turn = __builtin_amdgcn_readfirstlane(wave / a.heads), turns = a.turns;
   const uint32_t kvh = head0 + (wave - turn * a.heads);
 
-  const Ranges cut(total_tiles(a, lane), a.ranges);
+  // the tiles of 64 sequences, a lane each (the first 64 are read once), and of all
+  const uint32_t tiles0 = lane < a.batch ? tiles_of(context_of(a, lane)) : 0u;
+  uint32_t all = tiles0;
+  for (uint32_t b = lane + 64; b < a.batch; b += 64) all += tiles_of(context_of(a, b));
+  const Ranges cut(wave_total(all), a.ranges);
   uint32_t at = cut.first(range);
   const uint32_t end = cut.first(range + 1);
   if (at == end) return;
   // the sequence that holds tile `at`, and the tiles before it
   uint32_t seq = 0, before = 0;
   for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-    const uint32_t n = b0 + lane < a.batch ? tiles_of(context_of(a, b0 + lane)) : 0u;
+    uint32_t n = tiles0;
+    if (b0 > 0) n = b0 + lane < a.batch ? tiles_of(context_of(a, b0 + lane)) : 0u;
     const uint32_t upto = before + wave_inclusive_scan(n);
     const uint64_t past = __ballot(upto > at);
     if (past) {
       const int first = __builtin_ctzll(past);
       seq = b0 + uint32_t(first);
-      before = __builtin_amdgcn_readfirstlane(__shfl(int(upto - n), first));
+      before = uint32_t(__builtin_amdgcn_readlane(int(upto - n), first));
       break;
     }
-    before = __builtin_amdgcn_readfirstlane(__shfl(int(upto), 63));
+    before = uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
   }
   seq = __builtin_amdgcn_readfirstlane(seq);
 
@@ -360,67 +362,11 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
     const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
     const int32_t last_key = live ? int32_t(len) - int32_t(a.rows) + int32_t(qr) : -1;  // the row sees keys up to it
 
-    // Q operands (zero outside a half's column group), and the sums of their
-    // groups as the operand beside the steps and offsets: lane group j has part j
-    typename QO::Q qf[QP][VT][NG];
-    s16x8 qsum;
-    float unit = c2;  // of S^T, in log2 units
-    {
-      float x[NG][8], top = 0.f;
+    float x_q[NG][8];  // the row's elements 32 g + 8 j ..
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const int64_t from = int64_t(seq) * a.q_batch + int64_t(qr) * a.q_row + int64_t(qh) * a.q_head + 32 * g + 8 * j;
-        load_elems<DT>(a.q, from, a.q_pieces, live, x[g]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[g][e]));
-      }
-      float down = sign, inverse = 1.f;  // 1 / the row's unit
-      if constexpr (KF == Form::kFp8) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        // the exponent of the largest element, within what keeps both powers normal
-        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -115), 115);
-        down *= __uint_as_float(uint32_t(127 + 7 - e) << 23);
-        unit *= 512.f * __uint_as_float(uint32_t(127 - 7 + e) << 23);  // and the codes' 2^9
-        inverse = 1.f / 512.f;
-      }
-      uint32_t part[NG];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[g][e] *= down;
-          sum += x[g][e];
-        }
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        sum *= inverse;
-        const uint32_t hi = __float_as_uint(sum) & 0xffff0000u;
-        const float rest = sum - __uint_as_float(hi);
-        const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
-        const uint32_t low = __float_as_uint(rest - __uint_as_float(mid)) & 0xffff0000u;
-        part[g] = j == 0 ? hi : j == 1 ? mid : j == 2 ? low : 0u;
-#pragma unroll
-        for (int p = 0; p < QP; ++p) {
-          const typename QO::Q w = QO::cut(x[g]);
-#pragma unroll
-          for (int t = 0; t < VT; ++t) qf[p][t][g] = VT == 1 || v == uint32_t(t) ? w : typename QO::Q(0);
-        }
-      }
-      u32x4 w = u32x4(0u);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) w[g] = part[g];
-      qsum = __builtin_bit_cast(s16x8, w);
-    }
-
-    float m = kNegInf, l = 0.f, zsum[NG];
-    f32x4 o[2 * NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      zsum[g] = 0.f;
-      o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int g = 0; g < NG; ++g)
+      load_elems<DT>(a.q, int64_t(seq) * a.q_batch + int64_t(qr) * a.q_row + int64_t(qh) * a.q_head + 32 * g + 8 * j,
+                     a.q_pieces, live, x_q[g]);
 
     // The block table's entries of step i's rows -- K of tile i + 1, lanes 0 to
     // 31, and V of tile i, the others -- by DMA; and, from them, the rows, by DMA.
@@ -459,6 +405,78 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
       lds_dma<PIECE>(k_base, off, lds0 + buf * 2 * kBuf);
       return uint32_t(__ballot(held));
     };
+
+    uint32_t held = 0, held_next = 0;  // of the K rows of steps i and i + 1
+    if (count > 0) {
+      entries(-1);
+      entries(0);
+    }
+    CBK_WAIT_VM_LGKM0(0);  // nothing of the compiler's own in flight from here on
+    if (count > 0) {
+      held = request(-1, 2);
+      if (count > 1) entries(1);
+      held_next = request(0, 0);
+    }
+
+    // Q operands (zero outside a half's column group), and the sums of their
+    // groups as the operand beside the steps and offsets: lane group j has part j;
+    // made while the first rows are on their way
+    typename QO::Q qf[QP][VT][NG];
+    s16x8 qsum;
+    float unit = c2;  // of S^T, in log2 units
+    {
+      float top = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x_q[g][e]));
+      float down = sign, inverse = 1.f;  // 1 / the row's unit
+      if constexpr (KF == Form::kFp8) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // the exponent of the largest element, within what keeps both powers normal
+        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -115), 115);
+        down *= __uint_as_float(uint32_t(127 + 7 - e) << 23);
+        unit *= 512.f * __uint_as_float(uint32_t(127 - 7 + e) << 23);  // and the codes' 2^9
+        inverse = 1.f / 512.f;
+      }
+      uint32_t part[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x_q[g][e] *= down;
+          sum += x_q[g][e];
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        sum *= inverse;
+        const uint32_t hi = __float_as_uint(sum) & 0xffff0000u;
+        const float rest = sum - __uint_as_float(hi);
+        const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
+        const uint32_t low = __float_as_uint(rest - __uint_as_float(mid)) & 0xffff0000u;
+        part[g] = j == 0 ? hi : j == 1 ? mid : j == 2 ? low : 0u;
+#pragma unroll
+        for (int p = 0; p < QP; ++p) {
+          const typename QO::Q w = QO::cut(x_q[g]);
+#pragma unroll
+          for (int t = 0; t < VT; ++t) qf[p][t][g] = VT == 1 || v == uint32_t(t) ? w : typename QO::Q(0);
+        }
+      }
+      u32x4 w = u32x4(0u);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) w[g] = part[g];
+      qsum = __builtin_bit_cast(s16x8, w);
+    }
+
+    float m = kNegInf, l = 0.f, zsum[NG];
+    f32x4 o[2 * NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      zsum[g] = 0.f;
+      o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 
     f32x4 x[U];  // logits (log2 units), then weights, of key 8 j + 4 (u VT + v) + r and column c's row
     uint32_t seen = 0xffu;  // which of the lane's keys its row sees: bit 4 t + r
@@ -603,15 +621,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
       }
     };
 
-    uint32_t held = 0, held_next = 0;  // of the K rows of steps i and i + 1
-    CBK_WAIT_VM_LGKM0(0);              // nothing of the compiler's own in flight
     if (count > 0) {  // step -1: S^T of tile 0 alone
-      entries(-1);
-      entries(0);
-      CBK_WAIT_VM_LGKM0(0);
-      held = request(-1, 2);
-      if (count > 1) entries(1);
-      held_next = request(0, 0);
       CBK_WAIT_VM_LGKM0(kInsts);
       asm volatile("" ::: "memory");
       const uint32_t here = held;
@@ -734,8 +744,8 @@ __global__ __launch_bounds__(32 * SUBS) void int4_attn_merge_kernel(const Int4At
       total += t;
       before += b < seq ? t : 0u;
     }
-    total = __builtin_amdgcn_readlane(wave_inclusive_scan(total), 63);
-    before = __builtin_amdgcn_readlane(wave_inclusive_scan(before), 63);
+    total = wave_total(total);
+    before = wave_total(before);
     const Ranges cut(total, a.ranges);
     const uint32_t r0 = cut.of(before), r1 = cut.of(before + tiles - 1);
     if (r0 == r1) return;  // written by its range
