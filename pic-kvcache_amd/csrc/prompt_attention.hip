@@ -22,8 +22,7 @@
 // float32 inputs: prompt_attention_f32.hip.
 //
 // Which sequence and tile a workgroup has is found on the device (the lengths
-// stay there): tiles are taken in the order of their key counts, longest
-// first, over all sequences.
+// stay there).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -112,6 +111,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     if (S == 1) prompt_outside(a, tl, kvh, D * 2);
     return;
   }
+  if (tl.none) return;
   const uint32_t nrows = tl.nq * a.group;
   const uint32_t r_wave = tl.tile * kRows + wave * 16 * RT;
   const int32_t shift = int32_t(tl.nk) - int32_t(tl.nq);  // a query's position minus its index

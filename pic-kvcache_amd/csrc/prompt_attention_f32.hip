@@ -106,6 +106,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(3, 3))
     if (S == 1) prompt_outside(a, tl, kvh, D * 4);
     return;
   }
+  if (tl.none) return;
   const uint32_t nrows = tl.nq * a.group;
   const uint32_t r0 = tl.tile * kRows + wave * 16;  // the wave's first row
   const uint32_t r = r0 + row;

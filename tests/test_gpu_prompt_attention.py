@@ -115,6 +115,21 @@ def test_rows_around_the_sequences(dtype):
     _check(dtype, 8, 2, 64, [20], [1500], seed=4, before=7, behind=50)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_hundreds_of_sequences(dtype):
+    g = torch.Generator().manual_seed(20)
+    lens = torch.randint(0, 9, (600,), generator=g).tolist()
+    lens[37], lens[599] = 150, 70
+    _check(dtype, 4, 2, 64, lens, seed=20, before=3, behind=40)
+    _check(dtype, 4, 2, 128, lens, [n + 5 for n in lens], seed=21)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_large_launch_of_few_sequences(dtype):
+    # more than 2048 workgroups: the tiles sequence after sequence
+    _check(dtype, 128, 128, 64, [300, 0, 1100], seed=22, before=300, behind=200)
+
+
 def test_long_sequences():
     _check(BF16, 4, 1, 128, [3500, 100], seed=5)
     _check(F16, 2, 2, 64, [4100], seed=6)
