@@ -556,9 +556,10 @@ int check_sizes(int64_t total_q, int64_t total_k, int64_t batch, int64_t hq, int
 
 uint32_t splits_of(int64_t total_q, int64_t total_k, int64_t batch, int64_t hq, int64_t hkv, int64_t head_dim,
                    int32_t dtype) {
-  const uint64_t per = dtype == CBK_DTYPE_F32 ? kAttnF32Rows : kRows;
+  const uint64_t group = uint64_t(hq / hkv);
+  const uint64_t per = dtype == CBK_DTYPE_F32 ? prompt_f32_rows(uint64_t(total_q) * group, uint64_t(hkv)) : kRows;
   // what the lengths, which stay on the device, are on average
-  const uint64_t tiles = (uint64_t(total_q) * uint64_t(hq / hkv) / uint64_t(batch) + per - 1) / per * uint64_t(batch);
+  const uint64_t tiles = (uint64_t(total_q) * group / uint64_t(batch) + per - 1) / per * uint64_t(batch);
   const int64_t nk = (total_k + batch - 1) / batch;
   if (dtype == CBK_DTYPE_F32) return attn_f32_splits(tiles * uint64_t(hkv), nk);
   return attn_splits(tiles * uint64_t(hkv), uint64_t(total_q) * uint64_t(hq), nk, head_dim);

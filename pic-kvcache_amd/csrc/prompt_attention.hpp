@@ -30,6 +30,12 @@ inline uint64_t prompt_tiles(const PromptArgs& a, uint32_t rows) {
   return uint64_t(a.total_q) * a.group / rows + a.batch + 1;
 }
 
+// Rows of a workgroup of the float32 kernel, for rows of (query, group head): 128,
+// which share each K/V block's cutting and LDS reads, from two rounds of 64-row
+// workgroups (three a CU) on; below that more and shorter workgroups fill the
+// GPU better. us with 64 / 128: 8000 tokens of 32 / 8 heads x 128 2824 / 2506,
+// 3000 469 / 404, 2200 237 / 245; 4 of 1000, 16 / 8 heads, 112 / 142.
+inline uint32_t prompt_f32_rows(uint64_t rows, uint64_t hkv) { return rows * hkv >= 1536 * 64 ? 128 : 64; }
 int launch_prompt_f32(const PromptArgs& a, uint32_t d, hipStream_t stream);
 
 struct PromptTile {

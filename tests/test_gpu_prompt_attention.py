@@ -177,6 +177,35 @@ def test_what_a_row_does_not_see_may_be_anything(dtype, value):
         assert bool(got[60, 1].isnan().any())
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_float32_workgroups_of_128_rows(d):
+    # rows x KV heads from 1536 x 64 on
+    _check(F32, 64, 64, d, [700, 1, 0, 95, 850], seed=23, behind=10)
+    _check(F32, 96, 32, d, [400, 129, 600], [500, 100, 601], seed=24, before=5)
+    g = torch.Generator().manual_seed(25)
+    q, k, v = (t.to(DEV) for t in _make(g, 1600, 1600, 64, 64, d, F32))
+    ends = torch.tensor([0, 150, 1560], device=DEV)
+    want = prompt_attention(q, k, v, ends, 0.1)
+    k2, v2 = k.clone(), v.clone()
+    k2[149], v2[149] = float("nan"), float("inf")  # the first sequence's last token: its own row alone
+    k2[1560:], v2[1560:] = float("nan"), float("nan")
+    got = prompt_attention(q, k2, v2, ends, 0.1)
+    same = torch.ones(1600, dtype=torch.bool, device=DEV)
+    same[149] = False
+    # Rows of a masked block with such a value are summed one by one, in another
+    # order: both results hold to _bound (a dot product of d terms in 24 bits is off
+    # by up to (d + 8) 2^-24 of its absolute terms' sum, 1e-5 and more of a logit
+    # here, and the weights by that relative to themselves), so that they are apart by
+    # twice that at most. 4 eps (1 + |want|), as first written, leaves that out.
+    ends = [0, 150, 1560]
+    qn, kn, vn = (t.double().cpu().numpy() for t in (q, k, v))
+    clean, mass = R.prompt_attention(qn, kn, vn, ends, ends, 0.1)
+    tol = 2 * torch.from_numpy(_bound(qn, kn, vn, ends, ends, 0.1, F32, clean, mass)).to(DEV)[same]
+    assert bool(((got[same] - want[same]).abs() <= tol).all())
+    assert bool(((got[same] - torch.from_numpy(clean).to(DEV)[same]).abs() <= tol).all())
+    assert not bool(got[149].isfinite().any())
+
+
 def test_strides_and_alignment():
     g = torch.Generator().manual_seed(10)
     qkv = torch.randn(200, 8 + 2 + 2, 128, generator=g).to(BF16).to(DEV)
