@@ -51,7 +51,9 @@
 // heads' rows share cache lines, and side by side the waves ask for them at the
 // same time. (With a workgroup a head, on one XCD, the heads drifted apart, L2
 // fetched 1.6 GB for 0.83 of pages, and 64 sequences of up to 16K keys took 255
-// us whatever the work per key.) With fewer heads several waves of a head take
+// us whatever the work per key; now 208, 3.9 TB/s. Without the work 157 to 190,
+// without the transfers 154 to 173: what is left is their dependences, at the
+// two waves a SIMD that the registers allow.) With fewer heads several waves of a head take
 // its tiles in turn. A sequence that one range holds whole is written at once,
 // the others' partial results are merged by a second launch.
 #include <algorithm>
@@ -722,8 +724,8 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
 
 // The sequences that more than one range holds, and those without keys: a
 // workgroup per row, every 32 lanes each SUBS-th range of it, each lane D / 32
-// dims. 256 ranges of 32 rows: 46 us with one 32 lanes a row, 14 with 8, and
-// see launch() for 32.
+// dims. 256 ranges of 32 rows: 46 us with one 32 lanes a row, 14 with 8, 6.9
+// with 32.
 template <int DT, int D, int SUBS>
 __global__ __launch_bounds__(32 * SUBS) void int4_attn_merge_kernel(const Int4AttnArgs a) {
   constexpr int N = D / 32;
@@ -843,7 +845,9 @@ int launch(const Int4AttnArgs& a, bool pieces16, hipStream_t s) {
   // 16-byte pieces of a row: whole ones, where the pages are aligned to them
   constexpr int P = kInt4GroupBytes * NG % 16 == 0 ? 16 : 4;
   if (int rc = pieces16 ? launch_pieces<DT, NG, P>(a, s) : launch_pieces<DT, NG, 4>(a, s)) return rc;
-  // a sequence of many ranges: more lanes for each of its rows
+  // a sequence of many ranges: more lanes for each of its rows (a call in us with
+  // 8 / 32 sets of them, 32 over 8 heads x 128: 256 ranges a sequence 32.3 /
+  // 25.1, 64 35.4 / 34.0, 16 42.1 / 42.3, 8 62.1 / 65.1)
   const dim3 grid(a.rows * a.hq, a.batch);
   if (a.ranges > 16 * a.batch) hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG, 32>), grid, dim3(1024), 0, s, a);
   else hipLaunchKernelGGL((int4_attn_merge_kernel<DT, 32 * NG, 8>), grid, dim3(256), 0, s, a);
