@@ -18,6 +18,9 @@
 // - 1 issued beside the softmax of block b, exponents against a fixed
 // reference. It differs in what it does not do: no logit is rounded to the
 // inputs' type, positions and sequences follow from the lengths.
+// The weights, as the second product's operand, are rounded to the inputs' type
+// (half a step each, as the output itself); their sums are of the rounded ones,
+// in float32, so that equal values come out as they are.
 //
 // float32 inputs: prompt_attention_f32.hip.
 //

@@ -124,6 +124,21 @@ def test_hundreds_of_sequences(dtype):
     _check(dtype, 4, 2, 128, lens, [n + 5 for n in lens], seed=21)
 
 
+def test_thousands_of_sequences_and_ends_that_do_not_rise():
+    g = torch.Generator().manual_seed(26)
+    lens = torch.randint(0, 3, (5000,), generator=g).tolist()
+    q, k, v, got = _check(BF16, 2, 1, 64, lens, seed=26, before=1, behind=2)
+    # out of order: taken as they stand, within the tensors
+    ends = torch.tensor(_ends(lens, 1))
+    ends[2000:3000] = ends[2000:3000].flip(0)
+    ends[4000] = -5
+    ends[4500] = 1 << 30
+    for dtype in (BF16, F32):
+        out = prompt_attention(q.to(DEV, dtype), k.to(DEV, dtype), v.to(DEV, dtype), ends.to(DEV), 0.1)
+        torch.cuda.synchronize()
+        assert out.shape == q.shape
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_a_large_launch_of_few_sequences(dtype):
     # more than 2048 workgroups: the tiles sequence after sequence
