@@ -467,7 +467,9 @@ int cbk_prompt_attention(const void* q_dev, int64_t q_token_stride, int64_t q_he
  * elements, dims contiguous), row r of sequence b the token at place len_b -
  * rows + r of its context, which sees the keys up to its own:
  *   out[b, r, h] = sum_k softmax_k( scale q[b, r, h] . key[k, h/G] ) value[k, h/G]
- * with the logits, the softmax and the sums in float32. lens [batch] int32
+ * with the logits, the softmax and the sums in float32 (16-bit queries enter the
+ * first product exactly, or to 2^-36 of their row's largest element; the
+ * softmax's terms the second to 2^-16 of themselves, float32 2^-23). lens [batch] int32
  * (clamped to 0 .. table_width * block_size); tables [batch, table_width] int32,
  * row stride in entries: key k of a sequence is in page tables[k / block_size].
  * A page out of range holds no keys; a row that sees none is zero. head_dim 64

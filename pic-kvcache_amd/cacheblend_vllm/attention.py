@@ -221,7 +221,9 @@ def paged_attention_int4(
     keys up to its own. Key ``k`` of sequence ``b`` is in page ``block_tables[b, k //
     block_size]``; ``context_lens[b]`` counts the keys, those of ``query``'s tokens
     among them (append before attending). Head sizes 64 and 128; logits, softmax
-    and sums in float32, whatever the queries' type.
+    and sums in float32, whatever the queries' type: 16-bit queries enter the first
+    product exactly, or to 2^-36 of their row's largest element, the softmax's terms
+    the second to 2^-16 of themselves (float32: 2^-23).
 
     Lengths on the host are checked, and the tables where both are there
     (``IndexError``). On the device they are not read back: lengths are clamped

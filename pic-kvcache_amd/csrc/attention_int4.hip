@@ -15,11 +15,13 @@
 //
 // so the inner sums are products of small whole numbers on the matrix cores, the
 // codes in a form that takes little work:
-//  - beside q (16 bits) a byte 0000nnnn is the e4m3 value n 2^-9, for n below 8
-//    as below 16 (the subnormal numbers and the first binade are evenly spaced):
-//    two masks make 8 codes an operand. q, divided by a power of two of its row
-//    that leaves its largest element at 128 to 256, is cut into two (bf16) or
-//    three (f16) e4m3 parts, which hold it to 2^-18 of that element.
+//  - beside q (16 bits) a halfword 000n or 00n0 (hex) is the float16 subnormal
+//    number n 2^-24 or n 2^-20: four masks and a shift make 8 codes an operand. q,
+//    times a power of two of its row that brings its largest element to 2^15 ..
+//    2^16, and every second element times 2^-4 more, is a float16 operand: float16
+//    and bf16 elements as they are, down to where float16 ends, 2^-36 of the row's
+//    largest. (One product a code word. e4m3 parts of q, two or three products, held
+//    it to 2^-17 of that element only.)
 //  - beside p step a halfword 0x4300 | n is the bf16 value 128 + n, one and-or
 //    for two codes; a product with -128 follows, so that the running sums stay
 //    small.
@@ -66,6 +68,7 @@ namespace cbk {
 namespace {
 
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -159,8 +162,8 @@ __device__ __forceinline__ void lds_dma_word(const void* addr, uint32_t lds) {
 }
 
 // How codes n become an MFMA operand: as bf16 128 + n, or converted to bf16 n -
-// LESS (beside q of 16 bits: as e4m3 n 2^-9).
-enum class Form { kBf16, kExact, kFp8 };
+// LESS (beside q of 16 bits: as float16 n 2^-24 and n 2^-20 in turns).
+enum class Form { kBf16, kExact, kHalf };
 
 // 8 codes of a word as 8 operand elements, in the order 0 4 1 5 2 6 3 7.
 template <Form F, int LESS = 0>
@@ -189,7 +192,7 @@ __device__ __forceinline__ f32x4 mma(const s16x8& a, const s16x8& b, const f32x4
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// The operands of q . n: QParts of q, and the codes' words.
+// The operands of q . n: parts of q, and the codes' words.
 template <Form F> struct QOperand;
 template <> struct QOperand<Form::kExact> {
   typedef s16x8 Q;
@@ -205,26 +208,20 @@ template <> struct QOperand<Form::kExact> {
     return __builtin_bit_cast(s16x8, w);
   }
 };
-template <> struct QOperand<Form::kFp8> {
-  typedef u32x2 Q;
-  // in the order 0 2 4 6 1 3 5 7
-  static __device__ __forceinline__ u32x2 codes(uint32_t w) { return u32x2{w & 0x0f0f0f0fu, (w >> 4) & 0x0f0f0f0fu}; }
-  static __device__ __forceinline__ f32x4 mul(const u32x2& k, const Q& q, const f32x4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(__builtin_bit_cast(long, k), __builtin_bit_cast(long, q), c, 0, 0, 0);
+template <> struct QOperand<Form::kHalf> {
+  typedef h16x8 Q;
+  static __device__ __forceinline__ h16x8 codes(uint32_t w) {
+    const uint32_t low = 0x000f000fu, high = 0x00f000f0u;
+    return __builtin_bit_cast(h16x8, u32x4{w & low, w & high, (w >> 8) & low, (w >> 8) & high});
   }
+  static __device__ __forceinline__ f32x4 mul(const h16x8& k, const Q& q, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q, c, 0, 0, 0);
+  }
+  // 8 elements in the codes' order, those beside n 2^-20 times 2^-4
   static __device__ __forceinline__ Q cut(float (&x)[8]) {
-    Q r;
-#pragma unroll
-    for (int odd = 0; odd < 2; ++odd) {
-      int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[odd], x[odd + 2], 0, false);
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[odd + 4], x[odd + 6], w, true);
-      r[odd] = uint32_t(w);
-      x[odd] -= __builtin_amdgcn_cvt_f32_fp8(w, 0);
-      x[odd + 2] -= __builtin_amdgcn_cvt_f32_fp8(w, 1);
-      x[odd + 4] -= __builtin_amdgcn_cvt_f32_fp8(w, 2);
-      x[odd + 6] -= __builtin_amdgcn_cvt_f32_fp8(w, 3);
-    }
-    return r;
+    constexpr float less = 1.f / 16.f;
+    return Q{_Float16(x[0]), _Float16(x[4]), _Float16(x[1] * less), _Float16(x[5] * less),
+             _Float16(x[2]), _Float16(x[6]), _Float16(x[3] * less), _Float16(x[7] * less)};
   }
 };
 
@@ -279,8 +276,8 @@ template <int DT> __device__ __forceinline__ void store_elem(void* p, int64_t at
 
 // The operands' parts, the form of the codes beside q and beside p step.
 template <int DT> struct Parts;
-template <> struct Parts<CBK_DTYPE_BF16> { static constexpr int q = 2, p = 2; static constexpr Form k = Form::kFp8, v = Form::kBf16; };
-template <> struct Parts<CBK_DTYPE_F16> { static constexpr int q = 3, p = 2; static constexpr Form k = Form::kFp8, v = Form::kBf16; };
+template <> struct Parts<CBK_DTYPE_BF16> { static constexpr int q = 1, p = 2; static constexpr Form k = Form::kHalf, v = Form::kBf16; };
+template <> struct Parts<CBK_DTYPE_F16> { static constexpr int q = 1, p = 2; static constexpr Form k = Form::kHalf, v = Form::kBf16; };
 template <> struct Parts<CBK_DTYPE_F32> { static constexpr int q = 3, p = 3; static constexpr Form k = Form::kExact, v = Form::kExact; };
 
 template <int DT, int NG, int VT, int PIECE>
@@ -433,14 +430,14 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x_q[g][e]));
       float down = sign, inverse = 1.f;  // 1 / the row's unit
-      if constexpr (KF == Form::kFp8) {
+      if constexpr (KF == Form::kHalf) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         // the exponent of the largest element, within what keeps both powers normal
-        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -115), 115);
-        down *= __uint_as_float(uint32_t(127 + 7 - e) << 23);
-        unit *= 512.f * __uint_as_float(uint32_t(127 - 7 + e) << 23);  // and the codes' 2^9
-        inverse = 1.f / 512.f;
+        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -112), 115);
+        down *= __uint_as_float(uint32_t(127 + 15 - e) << 23);
+        unit *= __uint_as_float(uint32_t(127 + 24 - 15 + e) << 23);  // and the codes' 2^24
+        inverse = 0x1p-24f;
       }
       uint32_t part[NG];
 #pragma unroll

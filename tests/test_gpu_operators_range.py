@@ -1,0 +1,91 @@
+"""GPU: decode attention where magnitudes lie far apart or near
+the ends of float32's range, against 64 bits.
+
+Tolerance over 4-bit pages. A logit sums, per 32 dims, a query element times a
+whole number below 16, then step times that sum and offset times the query's sum:
+fewer than 67 float32 roundings of at most 2^-24 of the sum of the absolute terms
+OF EACH GROUP of 32 dims, whatever the other groups hold. Beside that a 16-bit
+query element may be off by 2^-36 of its row's largest, and, where products lie
+below float32's normal range, by an absolute 2^-149 that the row's unit scales
+up (`tiny`, given by the test that goes there). Weights: 2^-15 (two bf16 parts,
+and their sum's roundings; float32 2^-22); a relative change e of every weight
+moves an output by at most 2 e sum p |v|. The values' products hold step * 144 (float32: step * 16) +
+|offset| and round at most once a key of a lane; last comes the type's half step."""
+
+import numpy as np
+import pytest
+import torch
+
+from cacheblend_vllm import kv_layout as KL
+from cacheblend_vllm.attention import paged_attention_int4
+from oracle import operators as R
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _held(rows, d):
+    """|steps| and |offsets| [.., groups] of 4-bit rows."""
+    words = np.ascontiguousarray(rows[..., d // 2:]).view(np.uint16).astype(np.uint32) << 16
+    both = np.abs(words.view(np.float32).astype(np.float64)).reshape(*rows.shape[:-1], d // 32, 2)
+    return both[..., 0], both[..., 1]
+
+
+def _decode(dtype, q, k, v, scale, tiny=0.0, size=16):
+    """One sequence whose pages hold k, v [tokens, heads, d] (64 bits); q [rows, hq, d]."""
+    n, heads, d = k.shape
+    rows, hq = q.shape[:2]
+    blocks = (n + size - 1) // size
+    held = np.zeros((2, blocks * size, heads, KL.int4_row_bytes(d)), dtype=np.uint8)
+    held[:, :n] = R.int4_encode(np.stack([k, v]))
+    pages = torch.from_numpy(held).reshape(2, blocks, size, heads, -1).to(DEV)
+    tables = torch.arange(blocks, dtype=torch.int32)[None]
+    got = paged_attention_int4(q[None].to(DEV), pages, tables.to(DEV), torch.tensor([n], device=DEV), size, scale)
+    torch.cuda.synchronize()
+    qn = q.double().numpy()
+    want, mass = R.paged_attention_int4(qn[None], *pages.cpu().numpy(), tables.numpy(), [n], scale)
+    (ks, ko), (vs, vo) = (_held(p[:n], d) for p in held)
+    group = hq // heads
+    qg = np.abs(qn).reshape(rows, hq, d // 32, 32)
+    # [rows, hq, keys, groups] -> the largest sum over the groups of any key
+    terms = np.einsum("rhg,nhg->rhn", qg.sum(-1), (16 * ks + ko).repeat(group, axis=1)).max(-1)
+    exact = dtype == F32
+    e = 67 * 2.0 ** -24 * abs(scale) * terms + tiny + (2.0 ** -22 if exact else 2.0 ** -15) + (n / 16 + 64) * 2.0 ** -24
+    if not exact:
+        e = e + abs(scale) * 2.0 ** -36 * np.abs(qn).max(-1) * 32 * 15 * ks.sum(-1).max(0).repeat(group)
+    values = ((16 if exact else 144) * vs + vo).max(0).repeat(group, axis=0).repeat(32, axis=1)
+    tol = 2 * e[..., None] * mass[0] + (n / 16 + 64) * 2.0 ** -24 * values
+    tol = tol + torch.finfo(dtype).eps / 2 * np.abs(want[0]) + (2.0 ** -25 if dtype == F16 else 1e-38)
+    err = np.abs(got[0].double().cpu().numpy() - want[0])
+    print(f"decode {dtype} {hq}/{heads}x{d} of {n}: worst {float((err / tol).max()):.3f} of the bound", flush=True)
+    assert np.all(err <= tol)
+    return got[0]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("outlier,rest,step", [(200.0, 0.1, 5.0), (200.0, 0.03, 15.0), (1000.0, 0.1, 5.0)])
+def test_an_outlier_of_the_query_beside_small_elements(outlier, rest, step, dtype):
+    # a large element of q over keys that are small there: the other groups' elements
+    # keep their bits
+    g = np.random.default_rng(int(outlier + step))
+    for d, hq, heads, n in ((128, 8, 2, 300), (64, 4, 4, 90), (128, 32, 2, 700)):
+        q = g.standard_normal((1, hq, d)) * rest
+        q[..., 5] = outlier
+        k = g.standard_normal((n, heads, d)) * step
+        k[..., :32] *= 0.004 / step
+        v = g.standard_normal((n, heads, d))
+        _decode(dtype, torch.from_numpy(q).to(dtype), k, v, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_an_outlier_within_a_group_of_the_query(dtype):
+    # its keys are the group's lowest: code 0, all in the offset
+    g = np.random.default_rng(3)
+    for d, hq, heads, n in ((128, 8, 2, 300), (64, 4, 4, 90)):
+        q = g.standard_normal((1, hq, d)) * 0.1
+        q[..., 5] = 200.0
+        k = g.standard_normal((n, heads, d)) * 5
+        k[..., 5] = -32.0
+        v = g.standard_normal((n, heads, d))
+        _decode(dtype, torch.from_numpy(q).to(dtype), k, v, d ** -0.5)
