@@ -18,7 +18,8 @@
 //  - beside q (16 bits) a halfword 000n or 00n0 (hex) is the float16 subnormal
 //    number n 2^-24 or n 2^-20: four masks and a shift make 8 codes an operand. q,
 //    times a power of two of its row that brings its largest element to 2^15 ..
-//    2^16, and every second element times 2^-4 more, is a float16 operand: float16
+//    2^16 (its exponent is put back last, the range of q and of keys is float32's),
+//    and every second element times 2^-4 more, is a float16 operand: float16
 //    and bf16 elements as they are, down to where float16 ends, 2^-36 of the row's
 //    largest. (One product a code word. e4m3 parts of q, two or three products, held
 //    it to 2^-17 of that element only.)
@@ -339,7 +340,9 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
   const bool live = n_row < a.rows * a.group;
   const uint32_t qr = live ? n_row / a.group : 0, qh = kvh * a.group + (live ? n_row % a.group : 0);
   // a negative scale goes into the queries
-  const float sign = a.scale < 0.f ? -1.f : 1.f, c2 = fabsf(a.scale) * kLog2e;
+  const float sign = a.scale < 0.f ? -1.f : 1.f;
+  int c2_exponent;
+  const float c2 = frexpf(fabsf(a.scale) * kLog2e, &c2_exponent);  // 0.5 .. 1, its exponent in the rows' units
   const uint32_t lds0 = lds_address(&lds[wave][0]), pages0 = lds_address(&s_pages[wave][0][0]);
   // the selector that puts a float's upper half into the low (first 16 keys) or high half of a word
   const uint32_t place = v ? 0x03020c0cu : 0x0c0c0302u, half = v ? 0xffff0000u : 0x0000ffffu;
@@ -422,35 +425,31 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
     // made while the first rows are on their way
     typename QO::Q qf[QP][VT][NG];
     s16x8 qsum;
-    float unit = c2;  // of S^T, in log2 units
+    int unit;  // the exponent of S^T's unit
     {
       float top = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x_q[g][e]));
-      float down = sign, inverse = 1.f;  // 1 / the row's unit
-      if constexpr (KF == Form::kHalf) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        // the exponent of the largest element, within what keeps both powers normal
-        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -112), 115);
-        down *= __uint_as_float(uint32_t(127 + 15 - e) << 23);
-        unit *= __uint_as_float(uint32_t(127 + 24 - 15 + e) << 23);  // and the codes' 2^24
-        inverse = 0x1p-24f;
-      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // the row's largest element to 2^15 .. 2^16 (float32, whose codes have no 2^-24: 2^-9 .. 2^-8),
+      // whatever its exponent: S^T holds for keys up to the end of the range
+      const int e = int(__float_as_uint(top) >> 23) - 127, down = (KF == Form::kHalf ? 15 : -9) - e;
+      unit = c2_exponent + 24 - 15 + e;
       uint32_t part[NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x_q[g][e] *= down;
+          x_q[g][e] = __builtin_ldexpf(x_q[g][e] * sign, down);
           sum += x_q[g][e];
         }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
-        sum *= inverse;
+        if constexpr (KF == Form::kHalf) sum *= 0x1p-24f;
         const uint32_t hi = __float_as_uint(sum) & 0xffff0000u;
         const float rest = sum - __uint_as_float(hi);
         const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
@@ -513,7 +512,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
           float sum = s[u][r];
 #pragma unroll
           for (int g = 0; g < NG; ++g) sum = fmaf(__uint_as_float(sw[g] << 16), acc[g][r], sum);
-          s[u][r] = sum * unit;
+          s[u][r] = __builtin_ldexpf(sum * c2, unit);
         }
       }
     };

@@ -89,3 +89,17 @@ def test_an_outlier_within_a_group_of_the_query(dtype):
         k[..., 5] = -32.0
         v = g.standard_normal((n, heads, d))
         _decode(dtype, torch.from_numpy(q).to(dtype), k, v, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("big", [1.6e35, 1e36, 1e38, 1e-36])
+def test_queries_near_the_ends_of_the_range(big, dtype):
+    g = np.random.default_rng(4)
+    for d, hq, heads, n in ((128, 8, 2, 300), (64, 4, 4, 90), (128, 32, 2, 33)):
+        q = g.uniform(0.5, 2, (1, hq, d)) * big
+        k = g.standard_normal((n, heads, d)) / big
+        v = g.standard_normal((n, heads, d))
+        # a row's unit is at most 2^24 * 2^(127 - 14) * scale * log2 e: 12 products that may lie
+        # below 2^-126 round by 2^-150 each
+        _decode(dtype, torch.from_numpy(q).to(dtype), k, v, d ** -0.5,
+                tiny=12 * 2.0 ** -150 * 2.0 ** 137 * d ** -0.5 if big > 1 else 0.0)
