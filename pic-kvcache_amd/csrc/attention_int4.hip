@@ -81,7 +81,10 @@ constexpr int kStages = 3;  // tiles in a wave's LDS
 constexpr int max_waves(int32_t dtype) { return dtype == CBK_DTYPE_F32 ? 4 : 8; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kRescale = 8.f;  // log2 headroom before the reference maximum is raised
+// Logits are held in units of 4 times log 2: float32's largest logit times log2 e
+// is past its range, a quarter of that is not.
+constexpr float kUnit = 4.f;
+constexpr float kRescale = 8.f / kUnit;  // headroom before the reference maximum is raised: weights to 2^8
 
 struct Int4AttnArgs {
   const void* q;
@@ -437,7 +440,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
       // the row's largest element to 2^15 .. 2^16 (float32, whose codes have no 2^-24: 2^-9 .. 2^-8),
       // whatever its exponent: S^T holds for keys up to the end of the range
       const int e = int(__float_as_uint(top) >> 23) - 127, down = (KF == Form::kHalf ? 15 : -9) - e;
-      unit = c2_exponent + 24 - 15 + e;
+      unit = c2_exponent - 2 + 24 - 15 + e;  // of kUnit
       uint32_t part[NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -476,7 +479,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
       o[2 * g] = o[2 * g + 1] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    f32x4 x[U];  // logits (log2 units), then weights, of key 8 j + 4 (u VT + v) + r and column c's row
+    f32x4 x[U];  // logits, then weights, of key 8 j + 4 (u VT + v) + r and column c's row
     uint32_t seen = 0xffu;  // which of the lane's keys its row sees: bit 4 t + r
     bool masked = false;    // uniform: not all keys of the tile, for all rows
 
@@ -539,7 +542,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
         float bm = fmaxf(lm, __shfl_xor(lm, 16));
         bm = fmaxf(bm, __shfl_xor(bm, 32));
         const float mn = fmaxf(m, bm);
-        const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float alpha = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - mn) * kUnit);
         m = mn;
         l *= alpha;
         float ao[4];
@@ -564,7 +567,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - ms);
+          x[u][r] = __builtin_amdgcn_exp2f((x[u][r] - ms) * kUnit);
           l += x[u][r];
         }
       // p step in bf16 parts, operand word r key r of the first half in its low
@@ -699,7 +702,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
         for (int t = 0; t < VT; ++t) {
           const float* res = reinterpret_cast<const float*>(&lds[w][0]);
           const uint32_t col = t * COLS + row;
-          const float f = __builtin_amdgcn_exp2f(res[16 * D + 2 * col] - ts);
+          const float f = __builtin_amdgcn_exp2f((res[16 * D + 2 * col] - ts) * kUnit);
           sum = fmaf(f, res[16 * D + 2 * col + 1], sum);
           acc = fmaf(f, res[col * D + dim], acc);
         }
@@ -755,7 +758,7 @@ __global__ __launch_bounds__(32 * SUBS) void int4_attn_merge_kernel(const Int4At
       const float2 ml = a.ml[id];
       const VecN part = *reinterpret_cast<const VecN*>(a.o + id * D + N * dim);
       const float mn = fmaxf(top, ml.x), ms = mn == kNegInf ? 0.f : mn;
-      const float f = __builtin_amdgcn_exp2f(top - ms), w = __builtin_amdgcn_exp2f(ml.x - ms);
+      const float f = __builtin_amdgcn_exp2f((top - ms) * kUnit), w = __builtin_amdgcn_exp2f((ml.x - ms) * kUnit);
       sum = f * sum + w * ml.y;
       acc = f * acc + w * part;
       top = mn;
@@ -775,7 +778,7 @@ __global__ __launch_bounds__(32 * SUBS) void int4_attn_merge_kernel(const Int4At
   const float ms = all == kNegInf ? 0.f : all;
 #pragma unroll
   for (int i = 0; i < SUBS; ++i) {
-    const float w = __builtin_amdgcn_exp2f(s_m[i] - ms);
+    const float w = __builtin_amdgcn_exp2f((s_m[i] - ms) * kUnit);
     l = fmaf(w, s_l[i], l);
     o = fmaf(w, s_o[i][threadIdx.x], o);
   }

@@ -103,3 +103,38 @@ def test_queries_near_the_ends_of_the_range(big, dtype):
         # below 2^-126 round by 2^-150 each
         _decode(dtype, torch.from_numpy(q).to(dtype), k, v, d ** -0.5,
                 tiny=12 * 2.0 ** -150 * 2.0 ** 137 * d ** -0.5 if big > 1 else 0.0)
+
+
+def _one_dim(n, heads, d, at):
+    """Keys [n, heads, d]: `at` in dim 0, nothing elsewhere."""
+    k = np.zeros((n, heads, d))
+    k[..., 0] = np.asarray(at)[:, None]
+    return k
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_logits_past_the_range_in_log2_units_over_pages(dtype):
+    # 2.4e38 .. 3.3e38: finite, but not times log2 e. One key leads by 1e37 and
+    # more, a thousand times a logit's rounding: its value alone is left
+    g = np.random.default_rng(7)
+    for d, heads, n in ((128, 2, 300), (64, 1, 90), (128, 1, 5000)):
+        for sign, rest in ((1, 2.4e18), (-1, 3.2e18), (1, -3.0e18)):
+            lead = int(g.integers(n))
+            at = np.full(n, rest)
+            at[lead] = 3.2e18 if sign > 0 else 2.5e18
+            q = torch.zeros(1, 4 * heads, d, dtype=dtype)
+            q[..., 0] = sign * 1e20
+            v = g.standard_normal((n, heads, d))
+            size = 16
+            blocks = (n + size - 1) // size
+            held = np.zeros((2, blocks * size, heads, KL.int4_row_bytes(d)), dtype=np.uint8)
+            held[:, :n] = R.int4_encode(np.stack([_one_dim(n, heads, d, at), v]))
+            pages = torch.from_numpy(held).reshape(2, blocks, size, heads, -1).to(DEV)
+            got = paged_attention_int4(q.to(DEV), pages, torch.arange(blocks, device=DEV)[None],
+                                       torch.tensor([n], device=DEV), size, 1.0)
+            want = R.int4_decode(held[1, lead]).repeat(4, axis=0)
+            _, offset = _held(held[1, lead], d)
+            step, _ = _held(held[1, lead], d)
+            room = (144 * step + offset).repeat(4, axis=0).repeat(32, axis=-1)
+            tol = (2.0 ** -14 if dtype == BF16 else 2.0 ** -21) * room + torch.finfo(dtype).eps / 2 * np.abs(want)
+            assert np.all(np.abs(got[0].double().cpu().numpy() - want) <= tol), (d, n, sign, rest)
