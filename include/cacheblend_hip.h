@@ -469,7 +469,10 @@ int cbk_prompt_attention(const void* q_dev, int64_t q_token_stride, int64_t q_he
  *   out[b, r, h] = sum_k softmax_k( scale q[b, r, h] . key[k, h/G] ) value[k, h/G]
  * with the logits, the softmax and the sums in float32 (16-bit queries enter the
  * first product exactly, or to 2^-36 of their row's largest element; the
- * softmax's terms the second to 2^-16 of themselves, float32 2^-23). lens [batch] int32
+ * softmax's terms the second to 2^-16 of themselves, float32 2^-23). Queries, keys
+ * and logits may lie anywhere in float32's range, and so may the values of up to
+ * 256 keys; of more keys, values up to 256 / keys of its end. Values below 1e-28
+ * lose bits. lens [batch] int32
  * (clamped to 0 .. table_width * block_size); tables [batch, table_width] int32,
  * row stride in entries: key k of a sequence is in page tables[k / block_size].
  * A page out of range holds no keys; a row that sees none is zero. head_dim 64

@@ -84,7 +84,14 @@ constexpr float kNegInf = -__builtin_inff();
 // Logits are held in units of 4 times log 2: float32's largest logit times log2 e
 // is past its range, a quarter of that is not.
 constexpr float kUnit = 4.f;
-constexpr float kRescale = 8.f / kUnit;  // headroom before the reference maximum is raised: weights to 2^8
+constexpr float kRescale = 8.f / kUnit;  // headroom before the reference maximum is raised
+// The weights before they are divided by their sum are 2^-18 at the reference maximum, so
+// 2^-10 at most: a tile's products with 128 + n (32 keys' 143 steps, of a 15th of
+// float32's whole range each: 2e38) stay within the range, and so do, beside them, the
+// sums of 256 keys of the largest values, of more keys if the values are smaller in
+// proportion. At the other end products are rounded to bf16's smallest number, 2^-133,
+// which over 2^-18 and for 15 steps is an absolute 2e-34.
+constexpr float kWeights = -18.f;
 
 struct Int4AttnArgs {
   const void* q;
@@ -567,7 +574,7 @@ __global__ __launch_bounds__(64 * max_waves(DT), 1) void int4_attn_kernel(const 
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          x[u][r] = __builtin_amdgcn_exp2f((x[u][r] - ms) * kUnit);
+          x[u][r] = __builtin_amdgcn_exp2f(fmaf(x[u][r] - ms, kUnit, kWeights));
           l += x[u][r];
         }
       // p step in bf16 parts, operand word r key r of the first half in its low

@@ -105,6 +105,28 @@ def test_queries_near_the_ends_of_the_range(big, dtype):
                 tiny=12 * 2.0 ** -150 * 2.0 ** 137 * d ** -0.5 if big > 1 else 0.0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("big", [1e33, 1e34, 1e36, 2e37])
+def test_values_near_the_end_of_the_range(big, dtype):
+    g = np.random.default_rng(5)
+    for d, hq, heads, n in ((128, 8, 2, 300), (64, 4, 4, 90), (128, 32, 2, 33), (64, 8, 1, 1000)):
+        q = g.standard_normal((1, hq, d))
+        k = g.standard_normal((n, heads, d))
+        v = g.standard_normal((n, heads, d)) * big
+        got = _decode(dtype, torch.from_numpy(q).to(dtype), k, v, d ** -0.5)
+        assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_small_values(dtype):
+    g = np.random.default_rng(6)
+    for d, hq, heads, n in ((128, 8, 2, 300), (64, 4, 4, 90)):
+        q = g.standard_normal((1, hq, d))
+        k = g.standard_normal((n, heads, d))
+        v = g.standard_normal((n, heads, d)) * 1e-25
+        _decode(dtype, torch.from_numpy(q).to(dtype), k, v, d ** -0.5)
+
+
 def _one_dim(n, heads, d, at):
     """Keys [n, heads, d]: `at` in dim 0, nothing elsewhere."""
     k = np.zeros((n, heads, d))
