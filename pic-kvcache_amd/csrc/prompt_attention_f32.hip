@@ -63,6 +63,7 @@ __device__ __forceinline__ f32x4 mma6(const s16x8 (&a)[3], const s16x8 (&b)[3], 
 template <int D>
 __device__ void attend_row(const float* q, const float* k, const float* v, int64_t k_token, int64_t v_token, float scale,
                            int32_t lo, int32_t hi, uint32_t lane, float& m, float& l, float& o0, float& o1) {
+#pragma clang fp contract(off)  // x - ms of two rounded logits: 0 for equal ones, however large
   const float q0 = q[lane], q1 = D > 64 ? q[lane + 64] : 0.f;
   m = kNegInf;
   l = o0 = o1 = 0.f;

@@ -1,4 +1,4 @@
-"""GPU: decode attention where magnitudes lie far apart or near
+"""GPU: the prompt and decode attentions where magnitudes lie far apart or near
 the ends of float32's range, against 64 bits.
 
 Tolerance over 4-bit pages. A logit sums, per 32 dims, a query element times a
@@ -17,7 +17,7 @@ import pytest
 import torch
 
 from cacheblend_vllm import kv_layout as KL
-from cacheblend_vllm.attention import paged_attention_int4
+from cacheblend_vllm.attention import paged_attention_int4, prompt_attention
 from oracle import operators as R
 
 pytestmark = pytest.mark.gpu
@@ -160,3 +160,39 @@ def test_logits_past_the_range_in_log2_units_over_pages(dtype):
             room = (144 * step + offset).repeat(4, axis=0).repeat(32, axis=-1)
             tol = (2.0 ** -14 if dtype == BF16 else 2.0 ** -21) * room + torch.finfo(dtype).eps / 2 * np.abs(want)
             assert np.all(np.abs(got[0].double().cpu().numpy() - want) <= tol), (d, n, sign, rest)
+
+
+@pytest.mark.parametrize("dtype", [F32])
+@pytest.mark.parametrize("largest", [3.2e38, 2.3e38, 1e30, 1e12, 3e9, 1e8])
+def test_large_logits_of_prompts(largest, dtype):
+    # past float32's range in log2 units, and past what a multiply-add's exponent holds:
+    # rows whose keys hold one leading logit, or many equal ones
+    top = 3.2e4
+    scale = largest / top
+    g = torch.Generator().manual_seed(8)
+    for d, lens, keys in ((128, [70, 3], [300, 3]), (64, [200], [200]), (128, [20], [3000])):
+        q = torch.zeros(sum(lens), 4, d)
+        q[..., 0] = 1.0
+        k = torch.zeros(sum(keys), 2, d)
+        k[..., 0] = -top * 0.75
+        v = torch.randn(sum(keys), 2, d, generator=g)
+        ends_q, ends_k = np.concatenate([[0], np.cumsum(lens)]), np.concatenate([[0], np.cumsum(keys)])
+        for c in ends_k[:-1]:
+            k[c, :, 0] = top       # every row's leading key
+        q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+
+        def run():
+            got = prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(ends_q, device=DEV), scale,
+                                   torch.tensor(ends_k, device=DEV))
+            return got.double().cpu()
+
+        got = run()
+        for a, b, c in zip(ends_q[:-1], ends_q[1:], ends_k[:-1]):
+            want = v[c].double().repeat_interleave(2, dim=0)[None].expand(int(b - a), -1, -1)
+            assert torch.equal(got[a:b], want), (d, lens, keys)
+        # all keys alike: the mean of what a row sees
+        k[..., 0] = float(k[0, 0, 0])
+        got = run()
+        want, mass = R.prompt_attention(*(t.double().numpy() * f for t, f in ((q, 0.0), (k, 0.0), (v, 1.0))), ends_q, ends_k, 1.0)
+        tol = (2.0 ** -23 * sum(keys) + torch.finfo(dtype).eps) * mass + 2.0 ** -24
+        assert np.all(np.abs(got.numpy() - want) <= tol), (d, lens, keys)
