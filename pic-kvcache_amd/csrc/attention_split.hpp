@@ -53,7 +53,8 @@ size_t attn_parts_bytes(uint32_t splits, uint64_t rows, int64_t d);
 AttnParts attn_parts(uint32_t splits, uint64_t rows, void* workspace);
 
 // Packed sequences: only queries ends[0] .. ends[batch] have partial results;
-// the others' rows become zero, or stay as they are.
+// the others' rows become zero, or stay as they are. Their references are in
+// units of 2 log 2, whatever the type.
 struct AttnSpan {
   const int32_t* ends;  // NULL: every query has
   uint32_t batch;

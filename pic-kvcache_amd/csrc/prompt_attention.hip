@@ -42,13 +42,19 @@ constexpr int kRows = kWaves * 16 * kRowTiles;
 constexpr int kKeyBlock = kAttnKeyBlock;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kRescale = 8.f;  // log2 headroom of the lazy softmax rescaling
+// The lazy rescaling's logits are in units of 2 log 2: float32's largest logit
+// times log2 e is past its range, half of that is not. Its headroom: 2^8.
+constexpr float kUnit = 2.f;
+constexpr float kRescale = 8.f / kUnit;
+constexpr float kLargest = 0x1p26f;  // to there a reference is rounded by 4 at most: a common factor of 2^4 in the weights
 
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// p = 2^(S c2 - m) (MASK: 0 past each row's position), rounded to the dtype:
-// the A operand of P . V; nms = -m (0 while m is -inf).
-template <bool F16, int RT, bool MASK>
+// p = 2^(S c2 - m) (MASK: 0 past each row's position), rounded to the dtype: the A
+// operand of P . V; nms = -m (0 while m is -inf). In one multiply-add, which leaves
+// m's rounding error in the exponent, harmless up to kLargest; LAZY, for any m: in
+// units of kUnit, the product rounded as m was.
+template <bool F16, int RT, bool MASK, bool LAZY>
 __device__ __forceinline__ void probs_block(const f32x4 (&s)[RT][2], int32_t k0, float c2, const int32_t (&rpos)[RT],
                                             const float (&nms)[RT], uint32_t grp, typename Ops<F16>::A8 (&pa)[RT]) {
   using O = Ops<F16>;
@@ -60,7 +66,14 @@ __device__ __forceinline__ void probs_block(const f32x4 (&s)[RT][2], int32_t k0,
       float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float y = fmaf(s[t][h][i], c2, nms[t]);
+        float y;
+        if constexpr (LAZY) {
+#pragma clang fp contract(off)
+          const float x = s[t][h][i] * c2;
+          y = (x + nms[t]) * kUnit;
+        } else {
+          y = fmaf(s[t][h][i], c2, nms[t]);
+        }
         if constexpr (MASK) y = k0 + 16 * h + int32_t(4 * grp) + i > rpos[t] ? kNegInf : y;
         p[i] = __builtin_amdgcn_exp2f(y);
       }
@@ -70,7 +83,7 @@ __device__ __forceinline__ void probs_block(const f32x4 (&s)[RT][2], int32_t k0,
   }
 }
 
-// This lane's largest logit of each row tile (log2 units; -inf: none visible).
+// This lane's largest logit of each row tile (in c2's units; -inf: none visible).
 template <int RT>
 __device__ __forceinline__ void logits_max(const f32x4 (&s)[RT][2], int32_t k0, float c2, const int32_t (&rpos)[RT],
                                            uint32_t grp, float (&lm)[RT]) {
@@ -119,7 +132,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   const uint32_t r_wave = tl.tile * kRows + wave * 16 * RT;
   const int32_t shift = int32_t(tl.nk) - int32_t(tl.nq);  // a query's position minus its index
   const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale goes into the queries
-  const float c2 = fabsf(a.scale) * kLog2e;
+  const float c2 = fabsf(a.scale) * kLog2e, c2_lazy = fabsf(a.scale) * (kLog2e / kUnit);
 
   // this lane's rows (one per row tile): (query, head) and their Q fragments
   typename O::A8 qf[RT][D / 32];
@@ -162,8 +175,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   wmax -= key0;
   wmin -= key0;
 
-  // per row tile: the reference m (log2 units) and -m for the exponents (0
-  // while m is -inf)
+  // per row tile: the reference m (log2 units, or kUnit of them where it is lazy) and
+  // -m for the exponents (0 while m is -inf)
   float m[RT], nms[RT];
   f32x4 o[RT][D / 16], ol[RT];
   auto clear = [&]() __attribute__((always_inline)) {
@@ -325,7 +338,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         qk_block<F16, D, RT>(ks, off, qf, sn);
         if constexpr (!FIX) {
           float lm[RT];
-          logits_max<RT>(sc, b * kKeyBlock, c2, rpos, grp, lm);
+          logits_max<RT>(sc, b * kKeyBlock, c2_lazy, rpos, grp, lm);
           uint64_t over = 0;
 #pragma unroll
           for (int t = 0; t < RT; ++t) over |= __ballot(lm[t] > m[t] + kRescale);
@@ -338,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
               if (__any(lm[t] > m[t] + kRescale)) {
                 const float bm = fmaxf(lm[t], __shfl_xor(lm[t], 16));
                 const float mn = fmaxf(m[t], fmaxf(bm, __shfl_xor(bm, 32)));
-                alpha[t] = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[t] - mn);
+                alpha[t] = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m[t] - mn) * kUnit);
                 m[t] = mn;
                 nms[t] = mn == kNegInf ? 0.f : -mn;  // a row that sees no key of the range yet
                 pending = true;
@@ -346,7 +359,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
             }
           }
         }
-        probs_block<F16, RT, KIND == 1>(sc, b * kKeyBlock, c2, rpos, nms, grp, pc);
+        probs_block<F16, RT, KIND == 1, !FIX>(sc, b * kKeyBlock, FIX ? c2 : c2_lazy, rpos, nms, grp, pc);
         if constexpr (!FIRST) pv();
         // P of block b is computed here, beside P . V of block b - 1 (the
         // compiler would otherwise sink it to its use in the next step)
@@ -432,8 +445,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     if (b_w > 0) {
       qk_block<F16, D, RT>(lds_at(lds_address(kbuf[0])), off, qf, sa);
       // the masked form, whatever the block: one copy of the step fewer
-      if (first_ref) single(masked(), yes(), fix, b);
-      else single(masked(), yes(), no(), b);
+      if (first_ref) {
+        single(masked(), yes(), fix, b);
+      } else {
+        single(masked(), yes(), no(), b);
+        if constexpr (decltype(fix)::value) {  // the references in log2 units
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            m[t] *= kUnit;
+            nms[t] *= kUnit;
+          }
+        }
+      }
     }
     run(visible(), fix, b, b_m);
     run(masked(), fix, b, b_w);
@@ -448,16 +471,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   // where a row that sees anything sees key 0 (a logit of the row, so no term
   // exceeds 2^(max - m)): no per-logit maximum. The key ranges share it. A row
   // whose terms outgrew it (its sum past 2^100, or a term past float16), that
-  // has no reference although it sees keys, or whose output is not finite is
-  // recomputed, workgroup-wide, with the lazy rescaling and with the masked
-  // blocks' P . V key by key.
+  // has no reference although it sees keys, or one past kLargest, or whose output
+  // is not finite is recomputed, workgroup-wide, with the lazy rescaling and with
+  // the masked blocks' P . V key by key.
   __shared__ uint32_t s_redo;
+  float to_unit = 1.f / kUnit;  // of m
   if (nblocks > 0) {
     pass(yes());
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      bad |= m[t] == kNegInf && rpos[t] >= 0;
+      bad |= !(fabsf(m[t]) < kLargest) && rpos[t] >= 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         bad |= !finite_bits(ol[t][i]) || ol[t][i] >= 0x1p100f;
@@ -475,6 +499,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
       kg = kg0;
       vg = vg0;
       pass(no());
+      to_unit = 1.f;
     }
   }
   __syncthreads();  // every wave is done with the K buffers the output staging reuses
@@ -490,7 +515,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         if (rr >= nrows) continue;
         const uint32_t qi = a.group_div.div(rr);
         const uint64_t id = split * rows_all + uint64_t(tl.q0 + qi) * a.hq + kvh * a.group + rr - qi * a.group;
-        if (row == 0) a.parts.ml[id] = make_float2(rm, ol[t][i]);
+        // (a row that sees no key of the range may have the sequence's first reference, infinite perhaps)
+        if (row == 0) a.parts.ml[id] = make_float2(ol[t][i] == 0.f ? kNegInf : rm * to_unit, ol[t][i]);
         float* po = a.parts.o + id * D + row;
         if (nblocks > 0)
 #pragma unroll

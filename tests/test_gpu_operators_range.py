@@ -162,7 +162,7 @@ def test_logits_past_the_range_in_log2_units_over_pages(dtype):
             assert np.all(np.abs(got[0].double().cpu().numpy() - want) <= tol), (d, n, sign, rest)
 
 
-@pytest.mark.parametrize("dtype", [F32])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("largest", [3.2e38, 2.3e38, 1e30, 1e12, 3e9, 1e8])
 def test_large_logits_of_prompts(largest, dtype):
     # past float32's range in log2 units, and past what a multiply-add's exponent holds:
