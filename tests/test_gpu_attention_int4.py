@@ -333,3 +333,12 @@ def test_int4_attention_refuses():
     # pages past the context's are not looked at
     paged_attention_int4(q, pages, torch.tensor([[3, 99, -1]]), torch.tensor([16]), 16, 1.0)
     assert not paged_attention_int4(q, pages, tables[:, :0], torch.tensor([0]), 16, 1.0).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("hkv", [3, 5, 6, 7, 10, 12, 16])
+def test_counts_of_kv_heads(hkv, dtype):
+    # workgroups of 3 to 8 waves, several of them a range (more than 8 heads), several
+    # waves a head; a long sequence that ranges share beside short ones
+    _check(dtype, 2 * hkv, hkv, 128, [1, 1900, 0, 63, 33], seed=hkv)
+    _check(dtype, 3 * hkv, hkv, 64, [300, 2, 700], rows=2, seed=hkv + 1)
