@@ -245,7 +245,8 @@ def int4_row_bytes(head_size: int) -> int:
     ``2i`` in the low half of byte ``i``), then a bf16 step and a bf16 offset
     for every 32 dims; a dim's value is ``offset + step * code``. A 4-bit layer
     is an ordinary paged layer of ``uint8`` with rows ``[kv_heads,
-    int4_row_bytes(head_size)]``, so everything here that moves rows moves it."""
+    int4_row_bytes(head_size)]``, so what moves rows here moves it; what rotates
+    or compares them does not take it."""
     if head_size <= 0 or head_size % INT4_GROUP:
         raise ValueError(f"4-bit rows need a head size that is a multiple of {INT4_GROUP}, not {head_size}")
     return head_size // INT4_GROUP * (INT4_GROUP // 2 + 4)

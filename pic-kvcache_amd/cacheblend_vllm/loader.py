@@ -171,6 +171,11 @@ class PagedBlendLoader:
                 f"{plan.allocation_end} tokens"
             )
         src, old, relocate = build_source_map(plan)
+        if self.dtype not in _native.DTYPE_CODES and (relocate or self._row_bytes % 2):
+            raise ValueError(
+                f"{self.dtype} rows of {self._row_bytes} bytes cannot be relocated: only rows whose chunks stay at "
+                "their positions are loaded as they are" if relocate else
+                f"{self.dtype} rows of {self._row_bytes} bytes are not whole 16-bit words")
         self._relocate = relocate
         num_slots = key.shape[0] * block_size
         slots = self.slot_mapping
@@ -337,7 +342,7 @@ class PagedBlendLoader:
             if self._zero_copy == "auto":
                 commands = _native.memcpy_commands(dst_off, src, nbytes)
                 host_read = int(nbytes.sum()) / max(1, commands) < self._dma_min_run_bytes
-            if host_read:
+            if host_read and self._row_bytes % 16 == 0:  # the kernel reads 16-byte pieces
                 # publish the layer's chunk addresses; the assembly kernel
                 # reads the hit rows over the host link
                 if self._ptr_host is None:
@@ -379,6 +384,9 @@ class PagedBlendLoader:
         hit = self._hit_ring[self._hit_slot(layer_id)] if self._hit_ring is not None else None
         heads = int(np.prod(self.row_shape[:-1])) if len(self.row_shape) > 1 else 1
         head_dim = self.row_shape[-1]
+        code = _native.DTYPE_CODES.get(self.dtype)
+        if code is None:  # rows that are only moved (4-bit pages): 16-bit words
+            heads, head_dim, code = 1, self._row_bytes // 2, _native.DTYPE_CODES[torch.bfloat16]
         table = None
         neox = 0
         if self._relocate:
@@ -411,7 +419,7 @@ class PagedBlendLoader:
                 head_dim,
                 int(self._relocate),
                 neox,
-                _native.DTYPE_CODES[self.dtype],
+                code,
                 buffer[0].data_ptr(),
                 buffer[1].data_ptr(),
                 buffer.stride(1) * es,
@@ -439,7 +447,7 @@ class PagedBlendLoader:
             head_dim,
             int(self._relocate),
             neox,
-            _native.DTYPE_CODES[self.dtype],
+            code,
             buffer[0].data_ptr(),
             buffer[1].data_ptr(),
             buffer.stride(1) * es,

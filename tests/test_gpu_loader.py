@@ -389,3 +389,44 @@ def test_loader_blend_load_full_span_both_paths():
             np.testing.assert_array_equal(_bits(layers[l]), pages[l], err_msg=f"{zero_copy} commit {l}")
         # "auto" takes DMA for these runs; True reads the chunks in place
         assert (len(loader._zc_layers) > 0) == (zero_copy is True)
+
+
+@pytest.mark.parametrize("zero_copy", [True, False, "auto"])
+@pytest.mark.parametrize("heads,dim", [(8, 128), (1, 64), (3, 96)])  # rows of 640, 40 and 180 bytes
+def test_loader_moves_4_bit_rows_as_they_are(heads, dim, zero_copy):
+    """Chunks of 4-bit pages that stay at their positions: buffer and pages hold
+    their bytes. At other positions they are refused, for their keys cannot be
+    rotated in 4 bits."""
+    from cacheblend_vllm import kv_layout as KL
+
+    bs, nb, apc, end, chunk = 16, 40, 20, 300, 32
+    row = KL.int4_row_bytes(dim)
+    gen = torch.Generator().manual_seed(heads)
+    pool = torch.randint(0, 256, (2, nb, bs, heads, row), generator=gen, dtype=torch.uint8)
+    pages = pool.to(DEV)
+    slots = synthetic.block_slots(torch.randperm(nb, generator=gen)[: (end + bs - 1) // bs], bs, end)
+    store = PinnedChunkStore(chunk, 1 << 30)
+    host = torch.randint(0, 256, (2, 96, heads, row), generator=gen, dtype=torch.uint8).pin_memory()
+    here, moved = [], []
+    for c0 in range(0, 96, chunk):
+        sid = store.begin_put("m", 100 + c0, list(range(c0, c0 + chunk)), 1)
+        store.put_layer_host(sid, 0, host[:, c0 : c0 + chunk])
+        here.append(BlendSegment(sid, 100 + c0))
+        moved.append(BlendSegment(sid, 101 + c0))
+    store.pin("req", here)
+    plan = BlendPlan(apc, end, 96, tuple(here))
+    loader = PagedBlendLoader([pages], store, "req", plan, slots, bs, _cfg(chunk_size=chunk), zero_copy=zero_copy)
+    loader.prefetch(0, Rope(dim, 512, True))
+    buf = loader.get(0)
+    want = torch.zeros(2, end, heads, row, dtype=torch.uint8)
+    flat = pool.flatten(1, 2)
+    want[:, :apc] = flat[:, slots[:apc]]
+    want[:, 100:196] = host
+    assert torch.equal(buf.cpu(), want)
+    loader.commit(0, buf)
+    torch.cuda.synchronize()
+    expect = flat.clone()
+    expect[:, slots[apc:]] = want[:, apc:]
+    assert torch.equal(pages.cpu().flatten(1, 2), expect)
+    with pytest.raises(ValueError, match="cannot be relocated"):
+        PagedBlendLoader([pages], store, "req", BlendPlan(apc, end, 96, tuple(moved)), slots, bs, _cfg(chunk_size=chunk))
