@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .kv_layout import KVLayer, int4_geometry, paged_layer
+from .kv_layout import KVLayer, int4_geometry, paged_layer, rows_apart
 
 
 def blend_attention(
@@ -93,11 +93,8 @@ def _check_out(out: torch.Tensor, query: torch.Tensor) -> None:
         raise ValueError(f"out must be {tuple(query.shape)} {query.dtype} on {query.device}")
     if out.stride(-1) != 1:
         raise ValueError("out rows must hold contiguous dims")
-    span = out.shape[-1]
-    for n, stride in sorted(zip(out.shape[:-1], out.stride()[:-1]), key=lambda d: d[1]):
-        if n > 1 and stride < span:
-            raise ValueError("out rows must not overlap")
-        span += (n - 1) * stride
+    if not rows_apart(out):
+        raise ValueError("out rows must not overlap")
 
 
 def _prompt_ends(ends: torch.Tensor, tokens: int, name: str, device: torch.device) -> torch.Tensor:

@@ -261,6 +261,21 @@ def int4_geometry(dtype: torch.dtype, row: tuple) -> tuple[int, int]:
     return row[0], row[1] // per_group * INT4_GROUP
 
 
+def rows_apart(t: torch.Tensor) -> bool:
+    """Whether the rows (the last dim) of a strided tensor lie apart, whatever the
+    order of its dims in memory."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) == 3 and shape[0] > 1 and shape[1] > 1 and strides[1] >= shape[2] \
+            and strides[0] >= (shape[1] - 1) * strides[1] + shape[2]:
+        return True  # tokens outside heads, as most are
+    span = shape[-1]
+    for stride, n in sorted(zip(strides[:-1], shape[:-1])):
+        if n > 1 and stride < span:
+            return False
+        span += (n - 1) * stride
+    return True
+
+
 def _check_rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, out: bool = False) -> None:
     """[tokens, heads, head_size] with contiguous dims, of ``like``'s type and device; rows apart if written."""
     if t.shape != shape:
@@ -269,8 +284,7 @@ def _check_rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, ou
         raise ValueError(f"{name} must match the keys' dtype and device")
     if t.stride(2) != 1 and shape[2] > 1:
         raise ValueError(f"{name} rows must hold contiguous dims")
-    if out and ((shape[1] > 1 and t.stride(1) < shape[2]) or
-                (shape[0] > 1 and t.stride(0) < (shape[1] - 1) * t.stride(1) + shape[2])):
+    if out and not rows_apart(t):
         raise ValueError(f"{name} rows must not overlap")
 
 

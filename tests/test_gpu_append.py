@@ -307,3 +307,23 @@ def test_append_and_gather_refuse():
     assert KL.append_paged_kv(k[:0], k[:0], pages, slots[:0], 16) is None
     empty = KL.append_paged_kv(k[:0], k[:0], p4, slots[:0], 16, query=k[:0])
     assert empty.shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("int4", [False, True])
+@pytest.mark.parametrize("d,rotary", [(128, 128), (40, 24)])  # 16-byte pieces, and row by row
+def test_outputs_whose_heads_lie_outside_the_tokens(d, rotary, int4):
+    g = torch.Generator().manual_seed(31)
+    d = 96 if int4 and d % 32 else d
+    row = (2, KL.int4_row_bytes(d)) if int4 else (2, d)
+    pages = [torch.zeros(2, 3, 16, *row, dtype=torch.uint8 if int4 else BF16, device=DEV) for _ in range(3)]
+    q, k, v = (_rows(g, 33, h, d, dtype=BF16) for h in (4, 2, 2))
+    slots, pos, rope = torch.randperm(48, generator=g)[:33], torch.arange(33), _rope(40, d, rotary, True)
+    key = torch.empty_like(k)
+    want = KL.append_paged_kv(k, v, pages[0], slots, 16, pos, rope, query=q, key_out=key)
+    q_out, k_out = (torch.empty(h, 33, d, dtype=BF16, device=DEV).transpose(0, 1) for h in (4, 2))
+    got = KL.append_paged_kv(k, v, pages[1], slots, 16, pos, rope, query=q, query_out=q_out, key_out=k_out)
+    assert got is q_out and torch.equal(got, want) and torch.equal(k_out, key) and torch.equal(pages[1], pages[0])
+    # in place, the inputs head by head
+    q2, k2 = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k))
+    KL.append_paged_kv(k2, v, pages[2], slots, 16, pos, rope, query=q2, query_out=q2, key_out=k2)
+    assert torch.equal(q2, want) and torch.equal(k2, key) and torch.equal(pages[2], pages[0])

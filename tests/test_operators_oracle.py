@@ -206,3 +206,15 @@ def test_prompt_entry_refuses(over, word):
     assert _prompt(lib, **over) == _native.CBK_ERR_INVALID
     assert word in lib.cbk_last_error(), lib.cbk_last_error()
     assert _prompt(lib, total_q=0) == _native.CBK_OK
+
+
+def test_rows_that_lie_apart():
+    from cacheblend_vllm.kv_layout import rows_apart
+
+    x = torch.zeros(6, 4, 10)
+    for t in (x, x.transpose(0, 1), x[:, ::2], x[..., 2:8], x[:1].expand(1, 4, 10), x.permute(1, 0, 2)[::2], x[:0],
+              x.as_strided((3, 4, 5), (5, 30, 1)), x.as_strided((1, 2, 3), (0, 3, 1))):
+        assert rows_apart(t), (t.shape, t.stride())
+    for t in (x[:1].expand(6, 4, 10), x[:, :1].expand(6, 4, 10), x.as_strided((3, 4, 5), (5, 12, 1)),
+              x.as_strided((3, 4, 5), (4, 40, 1))):
+        assert not rows_apart(t), (t.shape, t.stride())
