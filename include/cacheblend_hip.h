@@ -439,7 +439,8 @@ int cbk_blend_attention_ws(const void* q_dev, int64_t q_row_stride_elems, const 
  * Causal attention of packed prompts: sequence s has the queries ends_q[s] ..
  * ends_q[s + 1] of q [total_q, hq, head_dim] and the keys ends_k[s] ..
  * ends_k[s + 1] of k, v [total_k, hkv, head_dim] (ends: [batch + 1] int32 on
- * the device, rising; strides in elements). Its last query is its last key:
+ * the device, rising, taken as the tensors' end past it; ends that fall leave
+ * the output's rows undefined; strides in elements). Its last query is its last key:
  * query i sees keys k <= i + keys - queries of the sequence, and is zero where
  * that is none:
  *   out[i, h] = sum_k softmax_k( scale q[i, h] . key[k, h/G] ) value[k, h/G]

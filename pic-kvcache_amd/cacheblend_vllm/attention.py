@@ -137,7 +137,8 @@ def prompt_attention(
     copied first.
 
     ``cu_seqlens`` on the host is checked (``IndexError``); on the device it is not
-    read back: ends past the tensors are taken as their end.
+    read back: ends past the tensors are taken as their end, and ends that fall,
+    which no batch has, leave ``out``'s rows undefined (nothing else is touched).
     """
     for name, t in (("query", query), ("key", key), ("value", value)):
         _native.require_device(t, name)

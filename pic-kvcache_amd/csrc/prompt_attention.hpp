@@ -52,8 +52,10 @@ struct PromptSeq {
   uint32_t q0, nq, k0, nk;
 };
 
-// Sequence s; ends that do not rise, or past the tensors, are taken as if they
-// stopped there.
+// Sequence s; ends past the tensors are taken as their end, and a sequence whose
+// end lies before its start is empty. (After ends that fall sequences may overlap,
+// and tiles be more than workgroups: rows are then written twice, in either order, or
+// not at all, but always within the tensors.)
 __device__ __forceinline__ PromptSeq prompt_seq(const PromptArgs& a, uint32_t s) {
   auto at = [](int32_t x, uint32_t total) { return min(uint32_t(max(x, 0)), total); };
   PromptSeq r;

@@ -321,3 +321,28 @@ def test_prompt_attention_refuses():
     assert prompt_attention(q[:0], k[:0], k[:0], torch.tensor([0]), 0.1).shape == (0, 4, 64)
     assert not prompt_attention(q + 1, k, k, torch.tensor([0]), 0.1).any()  # no sequence at all
     assert not prompt_attention(q + 1, k[:0], k[:0], ends, 0.1, torch.tensor([0, 0])).any()  # no keys
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,hkv", [(16, 2), (4, 4)])
+def test_falling_ends_on_the_device_touch_the_output_only(hq, hkv, dtype):
+    # overlapping sequences, more tiles than workgroups, keys that end before they begin:
+    # rows of `out` are undefined, what lies around and between them is not
+    g = torch.Generator().manual_seed(31)
+    q, k, v = (t.to(DEV) for t in _make(g, 300, 900, hq, hkv, 64, dtype))
+    held = torch.full((5 + 300 + 5, hq, 96), 7.0, dtype=dtype, device=DEV)
+    keep = [t.clone() for t in (q, k, v)]
+    for ends_q, ends_k in (([0, 100, 50, 200], [0, 100, 50, 200]), ([200, 0, 300, 100], [0, 900, 0, 900]),
+                           ([0, 300] * 40, [0, 900] * 40), ([0, 300] * 100, [0, 300] * 100),
+                           ([300, 200, 100, 0], [900, 0, 900, 0]), ([-5, 300, -5, 1 << 30], [-5, 900, -5, 1 << 30])):
+        print(dtype, hq, ends_q[:4], len(ends_q), flush=True)
+        ends = [torch.tensor(e, dtype=torch.int32, device=DEV) for e in (ends_q, ends_k)]
+        prompt_attention(q, k, v, ends[0], 0.125, ends[1], out=held[5:305, :, 16:80])
+        got = prompt_attention(q, k, v, ends[0], 0.125, ends[1])
+        torch.cuda.synchronize()
+        assert got.shape == q.shape
+        assert bool((held[:5] == 7).all()) and bool((held[305:] == 7).all())
+        assert bool((held[..., :16] == 7).all()) and bool((held[..., 80:] == 7).all())
+        assert all(torch.equal(a, b) for a, b in zip((q, k, v), keep))
+    # and calls in order are what they were
+    _check(dtype, 4, 2, 64, [40, 90], seed=32)
