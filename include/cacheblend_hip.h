@@ -445,7 +445,8 @@ int cbk_blend_attention_ws(const void* q_dev, int64_t q_row_stride_elems, const 
  * that is none:
  *   out[i, h] = sum_k softmax_k( scale q[i, h] . key[k, h/G] ) value[k, h/G]
  * with logits, softmax and sums in float32 (the softmax's terms enter the
- * second product rounded to the inputs' type). Keys and values that a row does
+ * second product rounded to the inputs' type: float16's below 2^-14 of the
+ * first 32 keys' largest to 2^-25 of it). Keys and values that a row does
  * not see may hold anything. Rows of no sequence become zero (zero_outside) or
  * stay as they are. head_dim 64 or 128; 16-byte aligned pointers and strides,
  * K/V token strides below 2^24.

@@ -129,7 +129,10 @@ def prompt_attention(
     from ``cu_seqlens_k[s]`` to ``cu_seqlens_k[s + 1]``). A sequence's last query is its
     last key: with more keys than queries the first keys are context from before
     (a chunk of a longer prompt), with fewer the first queries see nothing and are
-    zero. Head sizes 64 and 128; logits, softmax and sums in float32.
+    zero. Head sizes 64 and 128; logits, softmax and sums in float32. For the product
+    with the values the softmax's terms are rounded to the inputs' type (float16: terms
+    below 2^-14 of the largest of the first 32 keys' to 2^-25 of that, none below);
+    float32 terms and products hold 24 bits.
 
     Tokens before the first sequence and behind the last (padding) are zero in a
     new output and left as they are in ``out``. What a query does not see may hold

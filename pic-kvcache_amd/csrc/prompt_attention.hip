@@ -20,7 +20,10 @@
 // inputs' type, positions and sequences follow from the lengths.
 // The weights, as the second product's operand, are rounded to the inputs' type
 // (half a step each, as the output itself); their sums are of the rounded ones,
-// in float32, so that equal values come out as they are.
+// in float32, so that equal values come out as they are. float16 weights of less
+// than 2^-14 of the reference's are rounded to 2^-25 of that: the reference, from the
+// first block, is at 1, for later weights may be up to 2^16 times it before the
+// tile is computed again.
 //
 // float32 inputs: prompt_attention_f32.hip.
 //
