@@ -43,6 +43,12 @@ constexpr float kNegInf = -__builtin_inff();
 
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
+// rounded (a * b - c in one step would leave the error of a rounded a * b that is c)
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // One row's keys [k_lo, k_hi] by the whole wave: every lane two dims. The sum
 // l and the maximum m (natural units) of the keys, o the lane's outputs.
 __device__ void attend_row(const AttnF32Args& a, uint32_t qi, uint32_t h, int32_t k_lo, int32_t k_hi, uint32_t lane,
@@ -59,7 +65,7 @@ __device__ void attend_row(const AttnF32Args& a, uint32_t qi, uint32_t h, int32_
     float dot = (lane < a.d ? q0 * kr[lane] : 0.f) + (lane + 64 < a.d ? q1 * kr[lane + 64] : 0.f);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off);
-    const float x = dot * a.scale;
+    const float x = product(dot, a.scale);
     const float mn = fmaxf(m, x);
     const float ms = mn == kNegInf ? 0.f : mn;
     const float alpha = expf(m - ms);

@@ -257,3 +257,30 @@ def test_blend_attention_random_shapes(seed):
     print(label, flush=True)
     got = blend_attention(q.to(DEV), k.to(DEV), v.to(DEV), pos, scale)
     _check(got, _oracle(q, k, v, pos, scale, "bf16" if dtype == torch.bfloat16 else "f16"), label)
+
+
+@pytest.mark.parametrize("dtype,largest", [(torch.float32, x) for x in (3.2e38, 2.4e38, 1e30, 1e12, 3e9, 1e8)])
+def test_large_logits(largest, dtype):
+    """Logits whose rounding, to the type or to float32, is far more than 1: a
+    leading logit takes the row, equal ones share it, in one key range and in
+    several. (A weight's power is the difference of two rounded logits.)"""
+    top = 1.3e4
+    g = torch.Generator().manual_seed(41)
+    for n, m in ((40, 300), (20, 3000)):
+        q = torch.zeros(n, 4, 128)
+        q[..., 0] = 1
+        k = torch.zeros(m, 2, 128)
+        k[..., 0] = -top * 0.75
+        k[0, :, 0] = top
+        v = torch.randn(m, 2, 128, generator=g).to(dtype)
+        pos = torch.arange(m - n, m)
+        got = blend_attention(q.to(DEV, dtype), k.to(DEV, dtype), v.to(DEV), pos, largest / top).cpu()
+        assert torch.equal(got, v[0].repeat_interleave(2, dim=0)[None].expand(n, -1, -1)), (n, m)
+        k[..., 0] = top
+        got = blend_attention(q.to(DEV, dtype), k.to(DEV, dtype), v.to(DEV), pos, largest / top).cpu()
+        mean = v.double().cumsum(0)[pos] / (pos[:, None, None] + 1)
+        mass = v.double().abs().cumsum(0)[pos] / (pos[:, None, None] + 1)
+        # equal weights: a sum of m values, each product and sum rounded once in float32, and the type's half step
+        tol = (2.0 ** -24 * (m + 64)) * mass + torch.finfo(dtype).eps / 2 * mean.abs() + 2.0 ** -25
+        err = (got.double() - mean.repeat_interleave(2, dim=1)).abs()
+        assert bool((err <= tol.repeat_interleave(2, dim=1)).all()), (n, m)
