@@ -53,9 +53,13 @@ constexpr int kWaves = 4;
 constexpr int kRowTiles = 2;  // 16-row tiles per wave
 constexpr int kKeyBlock = kAttnKeyBlock;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHalfLog2e = 0.5f * kLog2e;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kRescale = 8.f;  // log2 headroom of the lazy softmax rescaling
+// The largest fixed reference (log2 units): a logit's second rounding, half a step of
+// the type, then moves its term by 2^64 at most (float16, whose range is 2^-14 .. 2^16: 2^4).
+template <bool F16> constexpr float kLargest = F16 ? 0x1p13f : 0x1p15f;
 
 struct AttnArgs {
   const uint16_t* q;      // [nq, hq, d], row stride q_stride elements
@@ -87,8 +91,9 @@ __device__ __forceinline__ void round2(float& x, float& y) {
 // dtype's einsum and multiply produce them (MASK: -inf past each row's
 // position); lm[t] = this lane's maximum over its logits of row tile t, taken
 // before the second rounding (rounding is monotonic, and the reference
-// maximum only needs to bound the logits within the rescale headroom).
-template <bool F16, int RT, bool MASK, bool WITH_MAX = true>
+// maximum only needs to bound the logits within the rescale headroom), or
+// after it (ROUNDED: a large logit's rounding is more than that headroom).
+template <bool F16, int RT, bool MASK, bool WITH_MAX = true, bool ROUNDED = false>
 __device__ __forceinline__ void logits_block(f32x4 (&s)[RT][2], int32_t k0, float scale, const int32_t (&rpos)[RT],
                                              float (&lm)[RT], uint32_t grp) {
 #pragma unroll
@@ -106,7 +111,7 @@ __device__ __forceinline__ void logits_block(f32x4 (&s)[RT][2], int32_t k0, floa
           if (k0 + 16 * h + int32_t(4 * grp) + i > rpos[t]) y[h][i] = kNegInf;
       }
     }
-    if constexpr (WITH_MAX)
+    if constexpr (WITH_MAX && !ROUNDED)
       lm[t] = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])),
                     fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
 #pragma unroll
@@ -115,12 +120,23 @@ __device__ __forceinline__ void logits_block(f32x4 (&s)[RT][2], int32_t k0, floa
       round2<F16>(y[h][2], y[h][3]);
       s[t][h] = f32x4{y[h][0], y[h][1], y[h][2], y[h][3]};
     }
+    if constexpr (WITH_MAX && ROUNDED)
+      lm[t] = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])),
+                    fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
   }
+}
+
+__device__ __forceinline__ float difference(float x, float f, float nms) {
+#pragma clang fp contract(off)
+  const float y = x * f;
+  return y + nms;
 }
 
 // p = 2^(x log2 e - m), rounded to the dtype: the A operand of P . V (the
 // two 16-key halves' registers, concatenated); nms = -m (0 while m is -inf).
-template <bool F16, int RT>
+// AGAIN: m in units of 2 log 2, the product rounded as m was (the multiply-add
+// leaves m's rounding error in the exponent).
+template <bool F16, int RT, bool AGAIN>
 __device__ __forceinline__ void probs_block(const f32x4 (&x)[RT][2], const float (&nms)[RT],
                                             typename Ops<F16>::A8 (&pa)[RT]) {
   using O = Ops<F16>;
@@ -131,7 +147,10 @@ __device__ __forceinline__ void probs_block(const f32x4 (&x)[RT][2], const float
     for (int h = 0; h < 2; ++h) {
       float p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(x[t][h][i], kLog2e, nms[t]));
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (AGAIN) p[i] = __builtin_amdgcn_exp2f(difference(x[t][h][i], kHalfLog2e, nms[t]) * 2.f);
+        else p[i] = __builtin_amdgcn_exp2f(fmaf(x[t][h][i], kLog2e, nms[t]));
+      }
       const u32x2 pk = u32x2{O::pack(p[0], p[1]), O::pack(p[2], p[3])};
       ph[h] = __builtin_bit_cast(typename O::A4, pk);
     }
@@ -345,6 +364,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     }
     if (inner) g += stride_bytes;
   };
+  using yes = std::true_type;
+  using no = std::false_type;
+  struct again : std::false_type {};  // FIX of the second pass
   // KIND: 0 visible, 1 masked, 2 P . V of the wave's last block only, 3 no
   // work; FIRST: no block before; PHASE: b % kPhases when known at compile time
   // (then every LDS address is a lane's offset plus a constant the DS
@@ -358,7 +380,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     constexpr int KIND = decltype(kind)::value;
     constexpr bool FIRST = decltype(first)::value;
     constexpr int PHASE = decltype(phase)::value;
-    constexpr bool FIX = decltype(fix)::value;
+    constexpr bool FIX = decltype(fix)::value, AGAIN = std::is_same<decltype(fix), again>::value;
     // K(b + 1) and V(b - 1) have landed: all but the requests of the last kBuffers - 2 steps
     CBK_WAIT_VM_LGKM0(2 * (kBuffers - 2) * kInsts);
     asm volatile("s_barrier" ::: "memory");
@@ -385,14 +407,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         qk_block<F16, D, RT>(ks, off, qf, sn);
         float lm[RT];
         logits_block<F16, RT, KIND == 1, false>(sc, b * kKeyBlock, a.scale, rpos, lm, grp);
-        probs_block<F16, RT>(sc, nms, pc);
+        probs_block<F16, RT, false>(sc, nms, pc);
         if constexpr (!FIRST) pv_block<F16, D, RT>(vs, off, pp, o, ol);
 #pragma unroll
         for (int t = 0; t < RT; ++t) asm volatile("" : "+v"(pc[t]));
       } else if constexpr (KIND < 2) {
         qk_block<F16, D, RT>(ks, off, qf, sn);
         float lm[RT];
-        logits_block<F16, RT, KIND == 1>(sc, b * kKeyBlock, a.scale, rpos, lm, grp);
+        logits_block<F16, RT, KIND == 1, true, AGAIN>(sc, b * kKeyBlock, a.scale, rpos, lm, grp);
+        if constexpr (AGAIN)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {  // in m's units (a large m is its own threshold)
+            lm[t] *= kHalfLog2e;
+            thr[t] = m[t] + 0.5f * kRescale;
+          }
         uint64_t over = 0;
 #pragma unroll
         for (int t = 0; t < RT; ++t) over |= __ballot(lm[t] > thr[t]);
@@ -406,16 +434,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
               float bm = lm[t];
               bm = fmaxf(bm, __shfl_xor(bm, 16));
               bm = fmaxf(bm, __shfl_xor(bm, 32));
-              const float mn = fmaxf(m[t], bm * kLog2e + 1.f);  // +1: covers the second rounding
-              alpha[t] = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[t] - mn);
+              const float mn = fmaxf(m[t], AGAIN ? bm : bm * kLog2e + 1.f);  // +1: covers the second rounding
+              alpha[t] = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f((AGAIN ? 2.f : 1.f) * (m[t] - mn));
               m[t] = mn;
               nms[t] = mn == kNegInf ? 0.f : -mn;  // a row that sees no key of the range yet
-              thr[t] = (mn + kRescale) * kLn2;
+              if constexpr (!AGAIN) thr[t] = (mn + kRescale) * kLn2;
               pending = true;
             }
           }
         }
-        probs_block<F16, RT>(sc, nms, pc);
+        probs_block<F16, RT, AGAIN>(sc, nms, pc);
         if constexpr (!FIRST) pv_block<F16, D, RT>(vs, off, pp, o, ol);
         // P of block b is computed here, beside P . V of block b - 1 (the
         // compiler would otherwise sink it to its use in the next step)
@@ -434,8 +462,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   using masked = std::integral_constant<int, 1>;
   using last = std::integral_constant<int, 2>;
   using none = std::integral_constant<int, 3>;
-  using yes = std::true_type;
-  using no = std::false_type;
   f32x4 sa[RT][2], sb[RT][2];
   typename O::A8 pa[RT], pb[RT];
   using any = std::integral_constant<int, -1>;
@@ -509,7 +535,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     }
     int32_t b = 0;
     if (b_w > 0) {  // the masked form, whatever the block: one copy of the step fewer
-      step(masked(), yes(), any(), no(), b++, sa, sb, pa, pb);
+      step(masked(), yes(), any(), std::conditional_t<decltype(fix)::value, no, decltype(fix)>(), b++, sa, sb, pa, pb);
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         sa[t][0] = sb[t][0];
@@ -538,15 +564,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   // 2^100: a logit more than ~69 above the first block's maximum), whose
   // output is not finite, or that was left without a reference although it
   // sees keys (every logit of its first block -inf, which an f16 dot product
-  // below -65504 rounds to) is recomputed, workgroup-wide, with the lazy
-  // rescaling.
+  // below -65504 rounds to) or with one past kLargest is recomputed,
+  // workgroup-wide, with the lazy rescaling, by references that are rounded
+  // logits, in units of 2 log 2 (which hold any logit of the type).
   __shared__ uint32_t s_redo;
+  float to_unit = 0.5f;  // of m, to units of 2 log 2
   if (nblocks > 0) {
     pass(yes());
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      bad |= m[t] == kNegInf && rpos[t] >= 0;
+      bad |= !(fabsf(m[t]) < kLargest<F16>) && rpos[t] >= 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         bad |= !(ol[t][i] < 0x1p100f);
@@ -572,7 +600,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
       }
       kg = kg0;
       vg = vg0;
-      pass(no());
+      pass(again());
+      to_unit = 1.f;
     }
   }
   __syncthreads();  // every wave is done with the K buffers the output staging reuses
@@ -587,7 +616,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         const uint32_t rr = r_wave + 16 * t + 4 * grp + i;
         if (rr >= nrows) continue;
         const uint64_t id = split * rows_all + uint64_t(rr / a.group) * a.hq + kvh * a.group + rr % a.group;
-        if (row == 0) a.parts.ml[id] = make_float2(rm, ol[t][i]);
+        // (a row that sees no key of the range may have the context's first reference, infinite perhaps)
+        if (row == 0) a.parts.ml[id] = make_float2(ol[t][i] == 0.f ? kNegInf : rm * to_unit, ol[t][i]);
         float* po = a.parts.o + id * D + row;
         if (nblocks > 0)
 #pragma unroll

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kMergeThreads) void attn_merge_kernel(const AttnPar
   for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 32));
   // a range without visible keys for the row: its sum is 0, its output may be
   // unwritten (never in float32)
-  const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f((F32 || span.ends != nullptr ? 2.f : 1.f) * (ml.x - m));
+  const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(2.f * (ml.x - m));
   // every other output counts, also with a weight of 0 (an infinity in it is
   // NaN then, as in one range)
   const uint64_t any = __ballot(F32 || ml.y != 0.f);

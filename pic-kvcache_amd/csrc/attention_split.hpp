@@ -11,9 +11,9 @@ namespace cbk {
 constexpr int kAttnKeyBlock = 32;  // keys per block of the attention kernels
 
 // Partial results of `splits` key ranges: for range s and row r = query *
-// hq + head, ml[s * rows + r] = (reference m in log2 units, sum of 2^(x - m))
-// and o[(s * rows + r) * d ..] the sum of 2^(x - m) * value, float32. From
-// float32 inputs m is halved: it holds every logit of the type that way.
+// hq + head, ml[s * rows + r] = (half the reference m, in log2 units, the sum of
+// 2^(x - m)) and o[(s * rows + r) * d ..] the sum of 2^(x - m) * value, float32.
+// Half of m holds every logit of any type.
 struct AttnParts {
   uint32_t splits;  // 1: no partials, the workgroups write the output
   float2* ml;
@@ -53,8 +53,7 @@ size_t attn_parts_bytes(uint32_t splits, uint64_t rows, int64_t d);
 AttnParts attn_parts(uint32_t splits, uint64_t rows, void* workspace);
 
 // Packed sequences: only queries ends[0] .. ends[batch] have partial results;
-// the others' rows become zero, or stay as they are. Their references are in
-// units of 2 log 2, whatever the type.
+// the others' rows become zero, or stay as they are.
 struct AttnSpan {
   const int32_t* ends;  // NULL: every query has
   uint32_t batch;

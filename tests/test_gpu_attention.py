@@ -259,7 +259,9 @@ def test_blend_attention_random_shapes(seed):
     _check(got, _oracle(q, k, v, pos, scale, "bf16" if dtype == torch.bfloat16 else "f16"), label)
 
 
-@pytest.mark.parametrize("dtype,largest", [(torch.float32, x) for x in (3.2e38, 2.4e38, 1e30, 1e12, 3e9, 1e8)])
+@pytest.mark.parametrize("dtype,largest", [(torch.bfloat16, x) for x in (3.2e38, 2.3e38, 1e30, 1e12, 3e9, 1e8, 1.23e6, 5e4, 1.7e4)]
+                         + [(torch.float16, x) for x in (6.3e4, 4.1e4, 2.3e4, 9e3)]
+                         + [(torch.float32, x) for x in (3.2e38, 2.4e38, 1e30, 1e12, 3e9, 1e8)])
 def test_large_logits(largest, dtype):
     """Logits whose rounding, to the type or to float32, is far more than 1: a
     leading logit takes the row, equal ones share it, in one key range and in
