@@ -478,7 +478,8 @@ int cbk_prompt_attention(const void* q_dev, int64_t q_token_stride, int64_t q_he
  * (clamped to 0 .. table_width * block_size); tables [batch, table_width] int32,
  * row stride in entries: key k of a sequence is in page tables[k / block_size].
  * A page out of range holds no keys; a row that sees none is zero. head_dim 64
- * or 128, pages 4-byte aligned (16: the faster transfers at head_dim 128).
+ * or 128, pages 4-byte aligned (16: transfers that take a head_dim of 128 in 0.6
+ * of the time).
  * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
  * function gives on the current device, max_len = table_width * block_size.
  */

@@ -54,9 +54,9 @@
 // heads' rows share cache lines, and side by side the waves ask for them at the
 // same time. (With a workgroup a head, on one XCD, the heads drifted apart, L2
 // fetched 1.6 GB for 0.83 of pages, and 64 sequences of up to 16K keys took 255
-// us whatever the work per key; now 208, 3.9 TB/s. Without the work 157 to 190,
-// without the transfers 154 to 173: what is left is their dependences, at the
-// two waves a SIMD that the registers allow.) With fewer heads several waves of a head take
+// us whatever the work per key; now 209 to 215, 3.9 TB/s. Without the work 187,
+// without the transfers 171: what is left is their dependences, at the two waves
+// a SIMD that the registers allow.) With fewer heads several waves of a head take
 // its tiles in turn. A sequence that one range holds whole is written at once,
 // the others' partial results are merged by a second launch.
 #include <algorithm>
@@ -848,7 +848,9 @@ int launch_pieces(const Int4AttnArgs& a, hipStream_t s) {
 
 template <int DT, int NG>
 int launch(const Int4AttnArgs& a, bool pieces16, hipStream_t s) {
-  // 16-byte pieces of a row: whole ones, where the pages are aligned to them
+  // 16-byte pieces of a row: whole ones, where the pages are aligned to them. In
+  // 4-byte pieces a tile of 128 dims takes four times the requests, and the addresses
+  // spill 40 to 50 registers: 64 sequences of up to 16K keys 369 us, 217 in 16 bytes.
   constexpr int P = kInt4GroupBytes * NG % 16 == 0 ? 16 : 4;
   if (int rc = pieces16 ? launch_pieces<DT, NG, P>(a, s) : launch_pieces<DT, NG, 4>(a, s)) return rc;
   // a sequence of many ranges: more lanes for each of its rows (a call in us with
