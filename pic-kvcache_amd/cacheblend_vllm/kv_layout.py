@@ -416,7 +416,8 @@ def gather_paged_kv_int4(
 ) -> torch.Tensor:
     """:func:`gather_paged_kv` of a 4-bit layer (:func:`int4_row_bytes`) as values
     ``[2, tokens, kv_heads, head_size]`` of ``dtype`` (or ``out``'s): one launch
-    (cbk_paged_gather_int4). Slots as there."""
+    (cbk_paged_gather_int4). Slots as there. What a row holds may lie past what went
+    in by a step: beside a type's largest value that is an infinity of the type."""
     desc, row, plane = paged_layer(kv_layer, block_size)
     heads, head_size = int4_geometry(plane.dtype, row)
     device = plane.device
