@@ -492,6 +492,33 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
                              int64_t out_batch_stride, int64_t out_row_stride, int64_t out_head_stride,
                              void* workspace_dev, size_t workspace_bytes, cbk_stream_t stream);
 
+/*
+ * Attention of each sequence's latest tokens over its context in pages of the
+ * queries' dtype, as cbk_paged_attention_int4 over 4-bit pages: q and out [batch,
+ * rows, hq, head_dim], strides in ELEMENTS; row r of a sequence sees keys up to
+ * lens_dev[b] - rows + r (lengths are clamped to the tables), a page out of range
+ * holds no keys, a row that sees none is zero; head_dim 64 or 128. Logits, softmax
+ * and sums in float32; 16-bit softmax weights enter the product with the values in
+ * two parts of the type. Pages aligned to their elements.
+ * key_weights_dev (NULL: none) [batch, weight_sets, max_len] float32, strides in
+ * elements, contiguous keys: to key k of sequence b, k < lens_dev[b], the softmax
+ * weights that the rows give it are added, of a KV head's query heads (weight_sets
+ * = hkv) or of all (1); in the rows' order, no atomics.
+ * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
+ * function gives on the current device, max_len = table_width * block_size; with
+ * key weights it holds the logits, 4 bytes for each of rows * hq and key of the
+ * tables.
+ */
+size_t cbk_paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
+                                           int64_t max_len, int32_t dtype, int32_t key_weights);
+int cbk_paged_attention(const void* q_dev, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+                        int64_t batch, int64_t rows, int64_t hq, const cbk_kv_desc* kv, int64_t hkv, int64_t head_dim,
+                        const int32_t* tables_dev, int64_t table_stride, int64_t table_width, const int32_t* lens_dev,
+                        float scale, int32_t dtype, void* out_dev, int64_t out_batch_stride, int64_t out_row_stride,
+                        int64_t out_head_stride, float* key_weights_dev, int64_t weights_batch_stride,
+                        int64_t weights_set_stride, int64_t weight_sets, void* workspace_dev, size_t workspace_bytes,
+                        cbk_stream_t stream);
+
 /* Workspace bytes cbk_sparse_q_scores needs. Per (query, head), queries padded
  * to a multiple of 64: 264 bytes (row statistics, a dense copy of the query row
  * sized for head_dim 128) and 8 per key range (8 ranges; up to 64 while they

@@ -120,3 +120,47 @@ def paged_attention_int4(q, k_pages, v_pages, tables, lens, scale):
         last = np.searchsorted(at[held], np.arange(q.shape[1]) + lens[b] - q.shape[1], side="right") - 1
         out[b], mass[b] = attend(q[b], k, v, last, scale)
     return out, mass
+
+
+def paged_attention(q, k_pages, v_pages, tables, lens, scale):
+    """q [B, R, Hq, D], a sequence's rows its context's last tokens; pages [blocks,
+    block size, H, D]. Pages out of range hold no keys. Returns the outputs, sum p |v|,
+    and [B, H, keys of the tables]: each key's weights, summed over rows and the KV head's
+    query heads."""
+    out, mass = np.zeros(q.shape), np.zeros(q.shape)
+    blocks, size, heads = k_pages.shape[:3]
+    rows, group = q.shape[1], q.shape[2] // heads
+    added = np.zeros((q.shape[0], heads, np.asarray(tables).shape[1] * size))
+    for b in range(q.shape[0]):
+        at = np.arange(lens[b])
+        page = np.asarray(tables[b])[at // size]
+        held = (page >= 0) & (page < blocks)
+        at = at[held]
+        k, v = (p[page[held], at % size].astype(np.float64) for p in (k_pages, v_pages))
+        for r in range(rows):
+            seen = at <= lens[b] - rows + r
+            if not seen.any():
+                continue
+            for h in range(q.shape[2]):
+                with np.errstate(invalid="ignore", over="ignore"):
+                    x = k[seen, h // group] @ q[b, r, h].astype(np.float64) * scale
+                    p = np.exp(x - x.max())
+                    p /= p.sum()
+                    out[b, r, h] = p @ v[seen, h // group]
+                    mass[b, r, h] = p @ np.abs(v[seen, h // group])
+                added[b, h // group, at[seen]] += p
+    return out, mass, added
+
+
+def evict(weights: np.ndarray, length: int, keep: int, first: int, recent: int) -> np.ndarray:
+    """The keys, in order, that stay of ``length`` keys with these weights: the
+    ``first`` first, the ``recent`` last, and of the others the heaviest (NaN above
+    all, -0 as 0, ties to the lower index) up to ``keep`` keys together."""
+    keep = max(keep, first + recent)
+    if length <= keep:
+        return np.arange(length)
+    middle = np.arange(first, length - recent)
+    w = np.asarray(weights, dtype=np.float64)[middle] + 0.0
+    order = np.lexsort((middle, np.where(np.isnan(w), -np.inf, -w), ~np.isnan(w)))
+    return np.concatenate([np.arange(first), np.sort(middle[order[:keep - first - recent]]),
+                           np.arange(length - recent, length)])

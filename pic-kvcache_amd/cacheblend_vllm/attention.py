@@ -1,5 +1,5 @@
 """Attention on MI355X: of the selected queries, of packed prompts, and of single
-tokens over 4-bit pages.
+tokens over pages of their own type or of 4 bits.
 
 ``blend_attention`` keeps the signature of ``Qwen3BlendExecutor._attention``
 (cacheblend_vllm/ascend.py:798-846): queries ``[Nq, Hq, D]`` at absolute
@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .kv_layout import KVLayer, int4_geometry, paged_layer, rows_apart
+from .kv_layout import KVLayer, check_key_weights, int4_geometry, paged_layer, rows_apart, whole_int32
 
 
 def blend_attention(
@@ -77,16 +77,6 @@ def blend_attention(
     return out
 
 
-def _whole_int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    """Whole numbers as int32 on ``device``; what int32 does not hold stays out of range."""
-    if t.dtype != torch.int32:
-        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
-            raise ValueError(f"whole numbers expected, got {t.dtype}")
-        if t.dtype in (torch.int64, torch.uint32, torch.uint64):
-            t = t.to(torch.int64).clamp(-1, (1 << 31) - 1)
-    return t if t.dtype == torch.int32 and t.device == device else t.to(device=device, dtype=torch.int32)
-
-
 def _check_out(out: torch.Tensor, query: torch.Tensor) -> None:
     """An output of ``query``'s shape and type whose rows lie apart."""
     if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
@@ -103,7 +93,7 @@ def _prompt_ends(ends: torch.Tensor, tokens: int, name: str, device: torch.devic
     if ends.device.type == "cpu":
         if int(ends[0]) < 0 or int(ends[-1]) > tokens or bool((ends[1:] < ends[:-1]).any()):
             raise IndexError(f"{name} must rise within the {tokens} tokens")
-    return _whole_int32(ends, device).contiguous()
+    return whole_int32(ends, device).contiguous()
 
 
 def _pieces(t: torch.Tensor, es: int, strided: bool = False) -> bool:
@@ -205,39 +195,17 @@ def prompt_attention(
     return out
 
 
-def paged_attention_int4(
-    query: torch.Tensor,
-    kv_layer: KVLayer,
-    block_tables: torch.Tensor,
-    context_lens: torch.Tensor,
-    block_size: int,
-    scale: float,
-    out: torch.Tensor | None = None,
-) -> torch.Tensor:
-    """Attention of each sequence's latest tokens over its context in 4-bit pages
-    (``kv_layout.append_paged_kv`` to a ``uint8`` layer): a decode step.
-
-    ``query`` is ``[batch, q_heads, head_size]``, one token a sequence, or ``[batch,
-    rows, q_heads, head_size]``: the last ``rows`` tokens, each of which sees the
-    keys up to its own. Key ``k`` of sequence ``b`` is in page ``block_tables[b, k //
-    block_size]``; ``context_lens[b]`` counts the keys, those of ``query``'s tokens
-    among them (append before attending). Head sizes 64 and 128; logits, softmax
-    and sums in float32, whatever the queries' type: 16-bit queries enter the first
-    product exactly, or to 2^-36 of their row's largest element, the softmax's terms
-    the second to 2^-16 of themselves (float32: 2^-23).
-
-    Lengths on the host are checked, and the tables where both are there
-    (``IndexError``). On the device they are not read back: lengths are clamped
-    to what a table holds, a page outside the cache holds no keys, and a row that
-    sees no key is zero.
-    """
+def _check_tokens(query: torch.Tensor) -> None:
     _native.require_device(query, "query")
     if query.dim() not in (3, 4):
         raise ValueError("query must be [batch, q_heads, head_size] or [batch, rows, q_heads, head_size]")
     if query.dtype not in _native.DTYPE_CODES:
         raise ValueError(f"dtype {query.dtype} is not supported")
-    desc, row, plane = paged_layer(kv_layer, block_size)
-    hkv, d = int4_geometry(plane.dtype, row)
+
+
+def _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, block_size, out):
+    """The checks that attention over pages of any type makes of a step's tensors:
+    (query of four dims, out, tables and lengths as the kernels take them)."""
     device = query.device
     if plane.device != device:
         raise ValueError(f"query is on {device}, the cache on {plane.device}")
@@ -268,13 +236,51 @@ def paged_attention_int4(
     else:
         _check_out(out, query)
     if batch * rows * hq == 0:
-        return out
-    tables = _whole_int32(block_tables, device)
+        return q, out, None, None
+    tables = whole_int32(block_tables, device)
     if width and tables.stride(1) != 1:
         tables = tables.contiguous()
-    lens = _whole_int32(context_lens, device)
+    lens = whole_int32(context_lens, device)
     if not lens.is_contiguous():
         lens = lens.contiguous()
+    return q, out, tables, lens
+
+
+def paged_attention_int4(
+    query: torch.Tensor,
+    kv_layer: KVLayer,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    scale: float,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each sequence's latest tokens over its context in 4-bit pages
+    (``kv_layout.append_paged_kv`` to a ``uint8`` layer): a decode step.
+
+    ``query`` is ``[batch, q_heads, head_size]``, one token a sequence, or ``[batch,
+    rows, q_heads, head_size]``: the last ``rows`` tokens, each of which sees the
+    keys up to its own. Key ``k`` of sequence ``b`` is in page ``block_tables[b, k //
+    block_size]``; ``context_lens[b]`` counts the keys, those of ``query``'s tokens
+    among them (append before attending). Head sizes 64 and 128; logits, softmax
+    and sums in float32, whatever the queries' type: 16-bit queries enter the first
+    product exactly, or to 2^-36 of their row's largest element, the softmax's terms
+    the second to 2^-16 of themselves (float32: 2^-23).
+
+    Lengths on the host are checked, and the tables where both are there
+    (``IndexError``). On the device they are not read back: lengths are clamped
+    to what a table holds, a page outside the cache holds no keys, and a row that
+    sees no key is zero.
+    """
+    _check_tokens(query)
+    desc, row, plane = paged_layer(kv_layer, block_size)
+    hkv, d = int4_geometry(plane.dtype, row)
+    q, out, tables, lens = _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, block_size, out)
+    device = query.device
+    batch, rows, hq = q.shape[:3]
+    width = block_tables.shape[1]
+    if batch * rows * hq == 0:
+        return out
     o = out if out.dim() == 4 else out.unsqueeze(1)
     lib = _native.load()
     nbytes = _native.on_device(device, lib.cbk_paged_attention_int4_workspace_bytes, batch, rows, hq, hkv, d,
@@ -288,4 +294,70 @@ def paged_attention_int4(
         _native.stream_handle(device),
     )
     _native.check(rc, "paged_attention_int4")
+    return out
+
+
+def paged_attention(
+    query: torch.Tensor,
+    kv_layer: KVLayer,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    scale: float,
+    out: torch.Tensor | None = None,
+    key_weights: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each sequence's latest tokens over its context in pages of the
+    queries' type: a decode step. (Over 4-bit pages: :func:`paged_attention_int4`.)
+
+    ``query`` is ``[batch, q_heads, head_size]``, one token a sequence, or ``[batch,
+    rows, q_heads, head_size]``: the last ``rows`` tokens, each of which sees the
+    keys up to its own. Key ``k`` of sequence ``b`` is in page ``block_tables[b, k //
+    block_size]``; ``context_lens[b]`` counts the keys, those of ``query``'s tokens
+    among them (append before attending). Head sizes 64 and 128; logits, softmax and
+    sums in float32. For the product with the values the softmax's terms are held to
+    2^-16 (bf16) or 2^-22 (float16, those below 2^-8 of the largest to 2^-30 of that).
+
+    ``key_weights`` ``[batch, kv_heads, keys]``, float32, at least as many keys as the
+    tables hold: to every key of the context is added, in place, what the softmax
+    weights of the rows and of the KV head's query heads give it together;
+    ``[batch, 1, keys]``: of all heads. Summed over the steps they say which keys
+    matter (``kv_layout.evict_paged_kv``). The call then takes scratch for the logits,
+    4 bytes for each row, query head and key of the tables.
+
+    Lengths on the host are checked, and the tables where both are there
+    (``IndexError``). On the device they are not read back: lengths are clamped
+    to what a table holds, a page outside the cache holds no keys, and a row that
+    sees no key is zero. What a row does not see may hold anything, infinities and
+    NaN among it.
+    """
+    _check_tokens(query)
+    desc, row, plane = paged_layer(kv_layer, block_size)
+    if plane.dtype != query.dtype or len(row) != 2:
+        raise ValueError(f"the pages hold {plane.dtype} rows {tuple(row)}, the queries are {query.dtype}")
+    hkv, d = row
+    q, out, tables, lens = _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, block_size, out)
+    device = query.device
+    batch, rows, hq = q.shape[:3]
+    width = block_tables.shape[1]
+    sets, w = 0, (None, 0, 0)
+    if key_weights is not None:
+        sets = check_key_weights(key_weights, batch, hkv, width * block_size, device)
+        w = (key_weights.data_ptr(), key_weights.stride(0), key_weights.stride(1))
+    if batch * rows * hq == 0:
+        return out
+    o = out if out.dim() == 4 else out.unsqueeze(1)
+    lib = _native.load()
+    code = _native.DTYPE_CODES[query.dtype]
+    nbytes = _native.on_device(device, lib.cbk_paged_attention_workspace_bytes, batch, rows, hq, hkv, d,
+                               width * block_size, code, int(sets != 0))
+    # from torch's allocator on every call: a captured graph then owns its own
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    rc = _native.on_device(
+        device, lib.cbk_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), batch, rows, hq, desc,
+        hkv, d, tables.data_ptr() if width else None, tables.stride(0), width, lens.data_ptr(), float(scale), code,
+        o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), *w, sets, ws.data_ptr(), ws.numel(),
+        _native.stream_handle(device),
+    )
+    _native.check(rc, "paged_attention")
     return out

@@ -407,6 +407,29 @@ def append_paged_kv(
     return query_out
 
 
+def whole_int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Whole numbers as int32 on ``device``; what int32 does not hold stays out of range."""
+    if t.dtype != torch.int32:
+        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+            raise ValueError(f"whole numbers expected, got {t.dtype}")
+        if t.dtype in (torch.int64, torch.uint32, torch.uint64):
+            t = t.to(torch.int64).clamp(-1, (1 << 31) - 1)
+    return t if t.dtype == torch.int32 and t.device == device else t.to(device=device, dtype=torch.int32)
+
+
+def check_key_weights(weights: torch.Tensor, batch: int, heads: int, keys: int, device: torch.device) -> int:
+    """The sets of heads (1, or one a KV head) of ``[batch, sets, keys]`` float32 weights that lie apart."""
+    if weights.dim() != 3 or weights.shape[0] != batch or weights.shape[1] not in (1, heads) or weights.shape[2] < keys:
+        raise ValueError(f"key weights are {tuple(weights.shape)}, expected [{batch}, 1 or {heads}, at least {keys}]")
+    if weights.dtype != torch.float32 or weights.device != device:
+        raise ValueError(f"key weights must be float32 on {device}")
+    if weights.stride(2) != 1 and weights.shape[2] > 1:
+        raise ValueError("key weights must hold contiguous keys")
+    if not rows_apart(weights):
+        raise ValueError("key weights must not overlap")
+    return weights.shape[1]
+
+
 def gather_paged_kv_int4(
     kv_layer: KVLayer,
     slot_mapping: torch.Tensor,

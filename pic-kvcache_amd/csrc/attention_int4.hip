@@ -64,6 +64,7 @@
 #include <type_traits>
 
 #include "int4_rows.hpp"
+#include "paged_ranges.hpp"
 
 namespace cbk {
 namespace {
@@ -118,26 +119,11 @@ struct Int4AttnArgs {
   float* o;
 };
 
-// The tiles [first, end) of range r of `total` tiles.
-struct Ranges {
-  uint32_t each, more;  // tiles of a range; ranges that have one more
-  __device__ __forceinline__ Ranges(uint32_t total, uint32_t ranges) : each(total / ranges), more(total % ranges) {}
-  __device__ __forceinline__ uint32_t first(uint32_t r) const { return r * each + min(r, more); }
-  __device__ __forceinline__ uint32_t of(uint32_t tile) const {
-    const uint32_t big = more * (each + 1);
-    return tile < big ? tile / (each + 1) : more + (tile - big) / each;
-  }
-};
-
 __device__ __forceinline__ uint32_t context_of(const Int4AttnArgs& a, uint32_t b) {
   return uint32_t(min(max(a.lens[b], 0), int32_t(a.max_len)));
 }
 
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + kTile - 1) / kTile; }
-
-__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
-  return uint32_t(__builtin_amdgcn_readlane(int(wave_inclusive_scan(v)), 63));
-}
 
 // LDS DMA from a 64-bit address per lane (the rows of pages anywhere): lane
 // l's 16 or 4 bytes land at lds + l * size, N requests' one after another. M0
