@@ -128,6 +128,29 @@ int cbk_paged_gather_int4(const cbk_kv_desc* kv, const int64_t* slots_dev, int64
                           cbk_stream_t stream);
 
 /*
+ * Eviction: of each sequence's lens_dev[b] keys (clamped to the tables) the `first`
+ * first, the `recent` last and the heaviest others, `keep` together, stay; in their
+ * order their rows, K and V, move to the front of the sequence's pages, and their
+ * weights to the front of theirs; the weights behind them, up to the old length,
+ * become 0, rows behind them are left as they are. new_lens_dev[b] =
+ * min(length, keep). Ties go to the lower index, NaN is heavier than any number.
+ * weights_dev [batch, sets, table_width * block_size] float32, strides in elements:
+ * a set is a KV head's rows (sets = the row's heads), each of which chooses its own keys,
+ * or the whole row (1). keep < 0: keeps_dev[b] (at least first + recent).
+ * Rows of a page out of range stay as they are, their weights move. Pages of
+ * different sequences, and of one table, must differ (else the rows in them are undefined).
+ * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
+ * function gives.
+ */
+size_t cbk_paged_evict_workspace_bytes(const cbk_kv_desc* kv, int64_t table_width, int64_t batch, int64_t sets,
+                                       int64_t keep);
+int cbk_paged_evict(const cbk_kv_desc* kv, const int32_t* tables_dev, int64_t table_stride, int64_t table_width,
+                    const int32_t* lens_dev, int64_t batch, float* weights_dev, int64_t weights_batch_stride,
+                    int64_t weights_set_stride, int64_t sets, int64_t keep, const int32_t* keeps_dev, int64_t first,
+                    int64_t recent, int32_t* new_lens_dev, void* workspace_dev, size_t workspace_bytes,
+                    cbk_stream_t stream);
+
+/*
  * Multi-layer gather in one launch per 64 layers: for layer l,
  * out + l*out_layer_stride + c*out_plane_stride + t*out_token_stride
  * receives plane c of kv[l] at slot t. All layers share the geometry of

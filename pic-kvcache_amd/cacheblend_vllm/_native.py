@@ -71,6 +71,12 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.POINTER(KVDesc), c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp],
     ),
+    "cbk_paged_evict_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(KVDesc), c_i64, c_i64, c_i64, c_i64]),
+    "cbk_paged_evict": (
+        ctypes.c_int,
+        [ctypes.POINTER(KVDesc), c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64,
+         c_vp, c_vp, ctypes.c_size_t, c_vp],
+    ),
     "cbk_paged_gather_layers": (
         ctypes.c_int,
         [ctypes.POINTER(KVDesc), c_i32, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp],

@@ -16,7 +16,8 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .kv_layout import KVLayer, check_key_weights, int4_geometry, paged_layer, rows_apart, whole_int32
+from .kv_layout import (KVLayer, check_key_weights, check_tables, device_tables, int4_geometry, paged_layer, rows_apart,
+                        whole_int32)
 
 
 def blend_attention(
@@ -219,31 +220,14 @@ def _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, bloc
         raise ValueError(f"query heads ({hq}) must be divisible by KV heads ({hkv})")
     if q.stride(3) != 1:
         raise ValueError("query rows must hold contiguous dims")
-    if block_tables.dim() != 2 or block_tables.shape[0] != batch or context_lens.numel() != batch:
-        raise ValueError(f"{tuple(block_tables.shape)} block tables and {context_lens.numel()} lengths for {batch} sequences")
-    width = block_tables.shape[1]
-    if context_lens.device.type == "cpu" and batch:
-        lo, hi = int(context_lens.min()), int(context_lens.max())
-        if lo < 0 or hi > width * block_size:
-            raise IndexError(f"context lengths in [{lo}, {hi}] outside the {width} blocks of {block_size}")
-        if block_tables.device.type == "cpu":
-            used = torch.arange(width) * block_size < context_lens.reshape(-1, 1)
-            pages = block_tables[used]
-            if pages.numel() and (int(pages.min()) < 0 or int(pages.max()) >= desc.num_blocks):
-                raise IndexError(f"block tables hold pages outside [0, {desc.num_blocks})")
+    check_tables(block_tables, context_lens, batch, block_size, desc.num_blocks)
     if out is None:
         out = torch.empty(query.shape, dtype=query.dtype, device=device)
     else:
         _check_out(out, query)
     if batch * rows * hq == 0:
         return q, out, None, None
-    tables = whole_int32(block_tables, device)
-    if width and tables.stride(1) != 1:
-        tables = tables.contiguous()
-    lens = whole_int32(context_lens, device)
-    if not lens.is_contiguous():
-        lens = lens.contiguous()
-    return q, out, tables, lens
+    return q, out, *device_tables(block_tables, context_lens, device)
 
 
 def paged_attention_int4(

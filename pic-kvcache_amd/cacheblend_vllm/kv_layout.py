@@ -417,6 +417,33 @@ def whole_int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     return t if t.dtype == torch.int32 and t.device == device else t.to(device=device, dtype=torch.int32)
 
 
+def check_tables(block_tables: torch.Tensor, context_lens: torch.Tensor, batch: int, block_size: int,
+                 num_blocks: int) -> None:
+    """Block tables ``[batch, blocks]`` and lengths of a batch; ranges checked of what is on the host."""
+    if block_tables.dim() != 2 or block_tables.shape[0] != batch or context_lens.numel() != batch:
+        raise ValueError(f"{tuple(block_tables.shape)} block tables and {context_lens.numel()} lengths for {batch} sequences")
+    width = block_tables.shape[1]
+    if context_lens.device.type == "cpu" and batch:
+        lo, hi = int(context_lens.min()), int(context_lens.max())
+        if lo < 0 or hi > width * block_size:
+            raise IndexError(f"context lengths in [{lo}, {hi}] outside the {width} blocks of {block_size}")
+        if block_tables.device.type == "cpu":
+            used = torch.arange(width) * block_size < context_lens.reshape(-1, 1)
+            pages = block_tables[used]
+            if pages.numel() and (int(pages.min()) < 0 or int(pages.max()) >= num_blocks):
+                raise IndexError(f"block tables hold pages outside [0, {num_blocks})")
+
+
+def device_tables(block_tables: torch.Tensor, context_lens: torch.Tensor,
+                  device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tables and lengths as the kernels take them."""
+    tables = whole_int32(block_tables, device)
+    if tables.shape[1] and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    lens = whole_int32(context_lens, device)
+    return tables, lens if lens.is_contiguous() else lens.contiguous()
+
+
 def check_key_weights(weights: torch.Tensor, batch: int, heads: int, keys: int, device: torch.device) -> int:
     """The sets of heads (1, or one a KV head) of ``[batch, sets, keys]`` float32 weights that lie apart."""
     if weights.dim() != 3 or weights.shape[0] != batch or weights.shape[1] not in (1, heads) or weights.shape[2] < keys:
@@ -428,6 +455,74 @@ def check_key_weights(weights: torch.Tensor, batch: int, heads: int, keys: int, 
     if not rows_apart(weights):
         raise ValueError("key weights must not overlap")
     return weights.shape[1]
+
+
+def evict_paged_kv(
+    kv_layer: KVLayer,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    key_weights: torch.Tensor,
+    keep: int | torch.Tensor,
+    first: int = 0,
+    recent: int = 0,
+) -> torch.Tensor:
+    """Cut each sequence down to ``keep`` keys, in place: its ``first`` first keys, its
+    ``recent`` last ones and the heaviest of the others by ``key_weights``
+    (``attention.paged_attention`` sums them up) stay, in their order, in the first
+    places of its pages. Returns the new lengths, ``min(context_lens, keep)``, int32 on
+    the cache's device; pages past them are free.
+
+    ``key_weights`` ``[batch, kv_heads, keys]`` float32, at least as many keys as the
+    tables hold: every KV head keeps keys of its own (rows of one place then come from
+    different tokens; attention does not mind, the order of each head's keys is kept);
+    ``[batch, 1, keys]``: all heads keep the same. The weights of the keys that stay move
+    with them, those behind, up to the old lengths, become 0, so that keys appended
+    there start from nothing. Ties go to the lower index, a NaN is heavier than any number.
+    ``keep`` may be a tensor with a number for each sequence.
+
+    Any paged layer, rows ``[kv_heads, ...]`` of any type, 4-bit ones among them.
+    The pages must be the sequences' own (a page that two tables, or one table twice,
+    name holds undefined rows afterwards). Lengths, tables and ``keep`` are checked where they
+    are on the host (``IndexError``, ``ValueError``); on the device they are not read
+    back: lengths are clamped to what a table holds, a keep is at least ``first +
+    recent``, and rows of a page outside the cache do not move.
+    """
+    desc, row, plane = paged_layer(kv_layer, block_size)
+    device = plane.device
+    batch = block_tables.shape[0]
+    check_tables(block_tables, context_lens, batch, block_size, desc.num_blocks)
+    width = block_tables.shape[1]
+    sets = check_key_weights(key_weights, batch, row[0], width * block_size, device)
+    first, recent = int(first), int(recent)
+    if first < 0 or recent < 0:
+        raise ValueError(f"first {first} and recent {recent} must not be negative")
+    keeps = None
+    if isinstance(keep, torch.Tensor) and keep.dim():
+        if keep.numel() != batch:
+            raise ValueError(f"{keep.numel()} numbers to keep for {batch} sequences")
+        if keep.device.type == "cpu" and batch and int(keep.min()) < first + recent:
+            raise ValueError(f"keep {int(keep.min())} is less than first {first} and recent {recent} together")
+        keeps, keep = whole_int32(keep.reshape(-1), device).contiguous(), -1
+    else:
+        keep = int(keep)
+        if keep < first + recent:
+            raise ValueError(f"keep {keep} is less than first {first} and recent {recent} together")
+    new_lens = torch.empty(batch, dtype=torch.int32, device=device)
+    if batch == 0:
+        return new_lens
+    tables, lens = device_tables(block_tables, context_lens, device)
+    lib = _native.load()
+    # from torch's allocator on every call: a captured graph then owns its own
+    nbytes = lib.cbk_paged_evict_workspace_bytes(desc, width, batch, sets, keep)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    rc = _native.on_device(
+        device, lib.cbk_paged_evict, desc, tables.data_ptr() if width else None, tables.stride(0), width, lens.data_ptr(),
+        batch, key_weights.data_ptr(), key_weights.stride(0), key_weights.stride(1), sets, keep, _native.ptr(keeps), first,
+        recent, new_lens.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(device),
+    )
+    _native.check(rc, "evict_paged_kv")
+    return new_lens
 
 
 def gather_paged_kv_int4(
