@@ -3,9 +3,9 @@
 // others stay, `keep` together, moved to the front of its pages in their order.
 //
 // Two launches. A workgroup per (sequence, set of heads) chooses: the weight of
-// the last key that stays is found digit by digit (12, 12 and 8 bits of the
-// weights as ordered whole numbers, histograms in LDS, the weights read again for
-// each: they are in L2), then one pass over the keys in order writes the list of
+// the last key that stays is found digit by digit (11, 11 and 10 bits of the
+// weights as ordered whole numbers, histograms in LDS; up to 8192 weights stay in
+// LDS meanwhile, more are read again from L2), then one pass over the keys in order writes the list of
 // those that stay and moves their weights. Then tiles of rows move.
 //
 // The rows move within their own pages, so a row must not be written before
@@ -13,14 +13,15 @@
 // it, so what lies in a tile's rows is read by the tile itself or by
 // tiles before it, of which the choice leaves the bounds: a tile reads all of its
 // rows into registers, says so in a flag, waits for the flags of the one or
-// two tiles that read from its rows, and writes. Tiles are handed out by a
-// counter, a unit's in order: a tile only waits for tiles that were handed out
+// two tiles that read from its rows, and writes. Tiles are handed out by
+// counters, a unit's in order: a tile only waits for tiles that were handed out
 // before, to workgroups that run, and these read, and raise their flag, before they
 // wait for anything; so every wait ends, whatever else the GPU does. (Only reads have to
 // be done, nothing is passed on: the flags need no fences, only loads that
 // have come back.)
 // Bound by HBM: the rows behind the first one that leaves are read and written once.
 #include <algorithm>
+#include <type_traits>
 
 #include "cbk_common.hpp"
 
@@ -28,9 +29,13 @@ namespace cbk {
 namespace {
 
 constexpr int kThreads = 1024;   // of the choice
+constexpr int kPass = 8192;      // keys in LDS
 constexpr int kMove = 256;       // of a move
 constexpr int kPieces = 8;       // a thread's pieces of a tile
 constexpr uint32_t kMaxRows = 512;
+constexpr uint32_t kNoSlot = 0xffffffffu;  // a page out of range
+constexpr uint32_t kGroups = 128;  // workgroups of a move for each CU, at most
+constexpr uint32_t kTickets = 16, kTicketPitch = 32;  // counters, a cache line each
 
 struct EvictArgs {
   char* k_base;
@@ -51,14 +56,15 @@ struct EvictArgs {
   // rows [k rows, (k + 1) rows) of the list), split into `chunks` of columns
   uint32_t rows, tiles, chunks, chunk_pieces, pieces_row;
   int64_t set_bytes;
-  FastDiv chunk_div;
-  // scratch: for each (sequence, set) the rows that move [begin, end), the list [most],
+  bool once;  // a workgroup a tile
+  FastDiv chunk_div, rows_div;
+  // scratch: for each (sequence, set) the rows that move [begin, end), the list of slots [most],
   // the keys below k rows that stay [tiles + 1], and the flags [2 planes][chunks][tiles]
   uint2* moved;
-  int32_t* list;
+  uint32_t* list;
   int32_t* below;
   uint32_t* flags;
-  uint32_t* ticket;
+  uint32_t* tickets;
 };
 
 __device__ __forceinline__ uint32_t ordered(float w) {
@@ -77,109 +83,159 @@ __device__ __forceinline__ void count_bin(uint32_t* bins, uint32_t bin) {
 }
 
 // The bin, from the highest down, in which the count reaches `want` (>= 1), and
-// what is still wanted of it.
-__device__ __forceinline__ uint32_t find_bin(const uint32_t* bins, uint32_t count, uint32_t* want, uint32_t* scratch,
-                                             uint32_t* found) {
-  const uint32_t per = count / kThreads > 0 ? count / kThreads : 1;
-  const bool mine = threadIdx.x * per < count;
-  const uint32_t top = count - threadIdx.x * per;  // bins [top - per, top)
+// what is still wanted of it; by each wave for itself, so that nobody waits.
+template <int BINS>
+__device__ __forceinline__ uint32_t find_bin(const uint32_t* bins, uint32_t& want) {
+  constexpr int PER = BINS / 64;  // lane l: bins [BINS - PER (l + 1), BINS - PER l)
+  const uint32_t lane = threadIdx.x & 63;
   uint32_t sum = 0;
-  if (mine)
-    for (uint32_t i = 1; i <= per; ++i) sum += bins[top - i];
-  uint32_t total;
-  uint32_t before = block_exclusive_scan<kThreads>(sum, scratch, &total);
-  if (mine && before < *want && before + sum >= *want) {
-    for (uint32_t i = 1; i <= per; ++i) {
-      const uint32_t n = bins[top - i];
-      if (before + n >= *want) {
-        found[0] = top - i;
-        found[1] = *want - before;
-        break;
-      }
-      before += n;
-    }
+#pragma unroll
+  for (int i = 0; i < PER; i += 4) {  // (from another place in each lane: neighbours' bins lie in the same banks)
+    const Vec<16>::T n = *reinterpret_cast<const Vec<16>::T*>(&bins[BINS - PER * (lane + 1) + ((i + 4 * lane) & (PER - 1))]);
+    sum += (n[0] + n[1]) + (n[2] + n[3]);
   }
-  __syncthreads();
-  const uint32_t bin = found[0];
-  *want = found[1];
-  __syncthreads();
-  return bin;
+  const uint32_t upto = wave_inclusive_scan(sum);
+  const int at = __builtin_ctzll(__ballot(upto >= want));
+  want -= uint32_t(__builtin_amdgcn_readlane(int(upto - sum), at));
+  // its bins, a lane each
+  static_assert(PER <= 64, "a lane a bin");
+  const uint32_t top = BINS - PER * uint32_t(at) - 1;
+  const uint32_t n = lane < PER ? bins[top - lane] : 0u;
+  const uint32_t past = wave_inclusive_scan(n);
+  const int bin = __builtin_ctzll(__ballot(past >= want));
+  want -= uint32_t(__builtin_amdgcn_readlane(int(past - n), bin));
+  return top - uint32_t(bin);
 }
 
 __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs a) {
-  __shared__ uint32_t bins[4096];
-  __shared__ uint32_t scratch[kThreads / 64], found[2], s_gone;
+  __shared__ __attribute__((aligned(16))) uint32_t bins[3][2048];
+  __shared__ float held[kPass];       // the weights of a pass's keys
+  __shared__ uint32_t places[kPass];  // where they go
+  __shared__ uint32_t scratch[kThreads / 64], s_gone;
   const uint32_t unit = blockIdx.x, b = unit / a.sets, set = unit - b * a.sets, tid = threadIdx.x;
   const uint32_t n = uint32_t(min(max(a.lens[b], 0), int32_t(a.max_len)));
   uint32_t keep = a.keeps ? uint32_t(max(a.keeps[b], 0)) : a.keep;
   keep = max(keep, a.first + a.recent);
-  if (unit == 0 && tid == 0) *a.ticket = 0;
+  if (unit == 0 && tid < kTickets) a.tickets[tid * kTicketPitch] = 0;
   if (set == 0 && tid == 0) a.new_lens[b] = int32_t(min(n, keep));
-  uint32_t* const flags = a.flags + int64_t(unit) * 2 * a.chunks * a.tiles;
   if (n <= keep) {
     if (tid == 0) a.moved[unit] = make_uint2(0, 0);
     return;
   }
+  float* const w = a.weights + int64_t(b) * a.w_batch + int64_t(set) * a.w_set;
+  auto fetch = [&](uint32_t i0) {
+    float x[kPass / kThreads];
+#pragma unroll
+    for (uint32_t k = 0; k < kPass / kThreads; ++k) x[k] = w[min(i0 + tid + k * kThreads, n - 1)];
+#pragma unroll
+    for (uint32_t k = 0; k < kPass / kThreads; ++k) held[tid + k * kThreads] = x[k];
+  };
+  fetch(0);
+  uint32_t* const flags = a.flags + int64_t(unit) * 2 * a.chunks * a.tiles;
   for (uint32_t i = tid; i < 2 * a.chunks * a.tiles; i += kThreads) flags[i] = 0;
   int32_t* const below = a.below + int64_t(unit) * (a.tiles + 1);
   for (uint32_t i = tid; i <= a.tiles; i += kThreads) below[i] = int32_t(keep);
-  float* const w = a.weights + int64_t(b) * a.w_batch + int64_t(set) * a.w_set;
   const uint32_t lo = a.first, hi = n - a.recent;  // the keys to choose from
   uint32_t want = keep - a.first - a.recent;        // of them; fewer than there are
 
   // the lowest ordered weight that stays, and how many of those that have it
   uint32_t limit = 0xffffffffu, equal = 0;
   const bool some = want != 0;
-  if (some) {
-    limit = 0;
-    int shift = 20, bits = 12;
-    for (int digit = 0; digit < 3; ++digit) {
-      const uint32_t count = 1u << bits;
-      for (uint32_t i = tid; i < count; i += kThreads) bins[i] = 0;
-      __syncthreads();
-      const uint64_t above = uint64_t(1) << (shift + bits);  // of the digits before
-      for (uint32_t i = lo + tid; i < hi; i += kThreads) {
-        const uint32_t key = ordered(w[i]);
-        if (((uint64_t(key) ^ uint64_t(limit)) & ~(above - 1)) == 0) count_bin(bins, (key >> shift) & (count - 1));
-      }
-      __syncthreads();
-      limit |= find_bin(bins, count, &want, scratch, found) << shift;
-      bits = digit == 0 ? 12 : 8;
-      shift -= bits;
-    }
-    equal = want;
-  }
+  for (uint32_t i = tid; i < 3 * 2048; i += kThreads) bins[0][i] = 0;
   if (tid == 0) s_gone = n;
   __syncthreads();
+  if (some) {
+    limit = 0;
+    auto digit = [&](auto top, auto width, uint32_t* counts) {  // bits [top - width, top) of those alike above
+      constexpr int T = decltype(top)::value, W = decltype(width)::value;
+      for (uint32_t i0 = 0; i0 < n; i0 += kPass) {
+        if (n > kPass) {
+          __syncthreads();
+          fetch(i0);
+          __syncthreads();
+        }
+        const uint32_t past = min(hi, i0 + uint32_t(kPass));
+        for (uint32_t j = tid; i0 + j < past; j += 4 * kThreads) {
+          float x[4];
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u) x[u] = held[(j + u * kThreads) % kPass];
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u) {
+            const uint32_t i = i0 + j + u * kThreads, key = ordered(x[u]);
+            const bool alike = T == 32 || ((key ^ limit) >> (T & 31)) == 0;
+            if (i < past && i >= lo && alike) count_bin(counts, (key >> (T - W)) & ((1u << W) - 1));
+          }
+        }
+      }
+      __syncthreads();
+      limit |= find_bin<(1 << W)>(counts, want) << (T - W);
+    };
+    digit(std::integral_constant<int, 32>(), std::integral_constant<int, 11>(), bins[0]);
+    digit(std::integral_constant<int, 21>(), std::integral_constant<int, 11>(), bins[1]);
+    digit(std::integral_constant<int, 10>(), std::integral_constant<int, 10>(), bins[2]);
+    equal = want;
+  }
 
-  // the keys in order: the list, their weights moved down, the counts at tiles' starts
-  int32_t* const list = a.list + int64_t(unit) * a.most;
+  // the keys in order: the list of their slots, their weights moved down, the counts at tiles' starts
+  uint32_t* const list = a.list + int64_t(unit) * a.most;
+  const int32_t* const table = a.tables + int64_t(b) * a.table_stride;
   uint32_t base = 0;
-  for (uint32_t i0 = 0; i0 < n; i0 += kThreads) {
-    const uint32_t i = i0 + tid;
-    const float x = i < n ? w[i] : 0.f;
-    const uint32_t key = ordered(x);
-    const bool always = i < n && (i < lo || i >= hi), may = i < n && !always && some;
-    const bool sure = always || (may && key > limit), tie = may && key == limit;
-    // (at most 1024 of each: two sums in one scan)
-    uint32_t total;
-    const uint32_t before = block_exclusive_scan<kThreads>(uint32_t(sure) | (uint32_t(tie) << 16), scratch, &total);
-    const uint32_t ties = before >> 16;
-    const bool stays = sure || (tie && ties < equal);
-    const uint32_t at = base + (before & 0xffffu) + min(ties, equal);
-    if (stays) {
-      list[at] = int32_t(i);
-      w[at] = x;  // places up to i, which have been read
-    } else if (i < n) {
-      atomicMin(&s_gone, i);
+  for (uint32_t i0 = 0; i0 < n; i0 += kPass) {
+    if (n > kPass) {
+      __syncthreads();
+      fetch(i0);
+      __syncthreads();
     }
-    if (i < n && i % a.rows == 0 && i / a.rows <= a.tiles) below[i / a.rows] = int32_t(at);
+    const uint32_t count = min(n - i0, uint32_t(kPass));
+    // a thread's neighbours (an odd number: they lie in different banks)
+    const uint32_t per = ((count + kThreads - 1) / kThreads) | 1u, from = tid * per, past = min(from + per, count);
+    uint32_t kinds = 0, both = 0;  // two bits a key (1: stays, 2: has the lowest weight); counts of the two
+    static_assert(kPass / kThreads <= 8, "two bits each");
+#pragma unroll
+    for (uint32_t k = 0; k < 9; ++k) {
+      const uint32_t i = i0 + from + k, key = ordered(held[(from + k) % kPass]);
+      uint32_t is = !some || key < limit ? 0u : key > limit ? 1u : 2u;
+      if (i < lo || i >= hi) is = 1u;
+      if (k >= per || from + k >= count) is = 0u;
+      kinds |= is << (2 * k);
+      both += (is & 1u) | (is >> 1 << 16);
+    }
+    uint32_t total;
+    const uint32_t before = block_exclusive_scan<kThreads>(both, scratch, &total);
+    uint32_t ties = before >> 16, at = base + (before & 0xffffu) + min(ties, equal), gone = n;
+    for (uint32_t k = from; k < past; ++k, kinds >>= 2) {
+      const uint32_t i = i0 + k, t = a.rows_div.div(i), is = kinds & 3u;
+      if (t * a.rows == i && t <= a.tiles) below[t] = int32_t(at);
+      const bool stays = is == 1u || (is == 2u && ties < equal);
+      places[k] = stays ? at : kNoSlot;
+      if (!stays) gone = min(gone, i);
+      at += stays;
+      ties += is >> 1;
+    }
+    // the first lane that has one that leaves has the wave's first
+    const uint64_t leave = __ballot(gone < n);
+    if (leave && int(tid & 63) == __builtin_ctzll(leave)) atomicMin(&s_gone, gone);
+    __syncthreads();
+    for (uint32_t k = tid; k < count; k += 4 * kThreads) {
+      uint32_t page[4];  // (four at a time before their stores)
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) page[u] = uint32_t(table[a.block_div.div(min(i0 + k + u * kThreads, n - 1))]);
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t j = k + u * kThreads, i = i0 + j;
+        if (j >= count) break;
+        const uint32_t to = places[j], blk = a.block_div.div(i);
+        if (to != kNoSlot) {
+          list[to] = page[u] < a.num_blocks ? page[u] * a.block_div.d + (i - blk * a.block_div.d) : kNoSlot;
+          w[to] = held[j];  // places up to i: they are in LDS by now
+        }
+        if (i >= keep) w[i] = 0.f;
+      }
+    }
     const uint32_t used = min(total >> 16, equal);
     base += (total & 0xffffu) + used;
     equal -= used;
   }
-  __syncthreads();
-  for (uint32_t i = keep + tid; i < n; i += kThreads) w[i] = 0.f;
   if (tid == 0) a.moved[unit] = make_uint2(min(s_gone, keep), keep);
 }
 
@@ -187,51 +243,81 @@ template <int VB>
 __global__ __launch_bounds__(kMove) void evict_move_kernel(const EvictArgs a) {
   typedef typename Vec<VB>::T V;
   typedef typename Vec<(VB < 4 ? 4 : VB)>::T Held;  // of it in registers
-  __shared__ int64_t s_from[kMaxRows], s_to[kMaxRows];  // byte offsets; -1: a page out of range
-  __shared__ uint32_t s_tile;
+  __shared__ int64_t s_from[kMaxRows], s_to[kMaxRows];  // byte offsets; -1: does not move
+  __shared__ uint32_t s_tile, s_unit;
   const uint32_t tid = threadIdx.x;
   const uint32_t lanes = 2 * a.chunks;               // (plane, chunk) of a unit
   const uint32_t units = a.batch * a.sets * lanes;
+  // Counter c hands out the tiles of units c, c + counters, ..: one counter for all
+  // took 12 ns a tile, whatever the tiles. A workgroup stays with one while it lasts.
+  const uint32_t counters = min(units, kTickets);
+  uint32_t c = blockIdx.x % counters;
+  auto units_of = [&](uint32_t i) { return (units - i + counters - 1) / counters; };
   for (;;) {
-    if (tid == 0) s_tile = atomicAdd(a.ticket, 1u);
+    if (tid < 64) {
+      uint32_t t;
+      for (;;) {
+        t = 0;
+        if (tid == 0) t = atomicAdd(&a.tickets[c * kTicketPitch], 1u);
+        t = uint32_t(__builtin_amdgcn_readfirstlane(int(t)));
+        if (t < units_of(c) * a.tiles) break;
+        // the next counter that is not at its end, from this one on
+        const uint32_t i = tid < counters ? (c + tid) % counters : 0;
+        const uint32_t at = __hip_atomic_load(&a.tickets[i * kTicketPitch], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint64_t left = __ballot(tid < counters && at < units_of(i) * a.tiles);
+        if (left == 0) {
+          t = 0xffffffffu;
+          break;
+        }
+        c = (c + uint32_t(__builtin_ctzll(left))) % counters;
+      }
+      if (tid == 0) {
+        const uint32_t n = units_of(c), tile = t / n;
+        s_tile = t == 0xffffffffu ? t : tile;
+        s_unit = c + counters * (t - tile * n);
+      }
+    }
     __syncthreads();
-    const uint32_t t = uint32_t(__builtin_amdgcn_readfirstlane(int(s_tile)));
-    const uint32_t tile = t / units;
-    if (tile >= a.tiles) return;
-    const uint32_t rest = t - tile * units, unit = rest / lanes, lane = rest - unit * lanes;
+    const uint32_t tile = uint32_t(__builtin_amdgcn_readfirstlane(int(s_tile)));
+    if (tile == 0xffffffffu) return;
+    const uint32_t rest = uint32_t(__builtin_amdgcn_readfirstlane(int(s_unit))), unit = rest / lanes, lane = rest - unit * lanes;
     const uint32_t plane = lane & 1, chunk = lane >> 1;
+    const uint32_t b = unit / a.sets, set = unit - b * a.sets, row0 = tile * a.rows;
+    // (loads that do not wait for each other)
     const uint2 moved = a.moved[unit];
-    const uint32_t begin = max(moved.x, tile * a.rows), end = min(moved.y, (tile + 1) * a.rows);
-    if (begin >= end) {
-      __syncthreads();
+    const int32_t* below = a.below + int64_t(unit) * (a.tiles + 1) + tile;
+    const int32_t first_below = below[0], past_below = below[1];  // of the list: what lies in this tile's rows
+    const uint32_t* list = a.list + int64_t(unit) * a.most;
+    const int32_t* table = a.tables + int64_t(b) * a.table_stride;
+    for (uint32_t r = tid; r < a.rows; r += kMove) {
+      const uint32_t key = min(row0 + r, a.most - 1), blk = a.block_div.div(key);
+      const uint32_t slot = list[key], page = uint32_t(table[blk]);
+      const bool moves = row0 + r >= moved.x && row0 + r < moved.y && slot != kNoSlot && page < a.num_blocks;
+      const uint32_t from = a.block_div.div(slot);
+      s_from[r] = moves ? int64_t(from) * a.block_stride + int64_t(slot - from * a.block_div.d) * a.token_stride : -1;
+      s_to[r] = int64_t(page) * a.block_stride + int64_t(key - blk * a.block_div.d) * a.token_stride;
+    }
+    __syncthreads();
+    if (max(moved.x, row0) >= min(moved.y, row0 + a.rows)) {
+      if (a.once) return;
       continue;
     }
-    const uint32_t b = unit / a.sets, set = unit - b * a.sets, rows = end - begin;
-    const int32_t* list = a.list + int64_t(unit) * a.most;
-    const int32_t* table = a.tables + int64_t(b) * a.table_stride;
-    auto offset = [&](uint32_t key) {
-      const uint32_t blk = a.block_div.div(key), page = uint32_t(table[blk]);
-      if (page >= a.num_blocks) return int64_t(-1);
-      return int64_t(page) * a.block_stride + int64_t(key - blk * a.block_div.d) * a.token_stride;
-    };
-    for (uint32_t r = tid; r < rows; r += kMove) {
-      s_from[r] = offset(uint32_t(list[begin + r]));
-      s_to[r] = offset(begin + r);
-    }
-    __syncthreads();
     const uint32_t first_piece = chunk * a.chunk_pieces, width = min(a.chunk_pieces, a.pieces_row - first_piece);
     char* const base = (plane ? a.v_base : a.k_base) + int64_t(set) * a.set_bytes + int64_t(first_piece) * VB;
     Held v[kPieces];
-    int64_t to[kPieces];
+    // piece u of this thread, of row r; whether it moves
+    auto place = [&](int u, uint32_t& r, uint32_t& piece) __attribute__((always_inline)) {
+      const uint32_t f = tid + kMove * u;
+      r = a.chunk_div.div(f);
+      piece = f - r * a.chunk_pieces;
+      return r < a.rows && piece < width && s_from[r] >= 0;
+    };
 #pragma unroll
     for (int u = 0; u < kPieces; ++u) {
-      const uint32_t f = tid + kMove * u, r = a.chunk_div.div(f), piece = f - r * a.chunk_pieces;
-      to[u] = -1;
+      uint32_t r, piece;
       v[u] = Held{};
-      if (r < rows && piece < width && s_from[r] >= 0 && s_to[r] >= 0) {
+      if (place(u, r, piece))
         v[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(base + s_from[r] + int64_t(piece) * VB));
-        to[u] = s_to[r] + int64_t(piece) * VB;
-      }
     }
     // the loads have come back (their values are used here), then the flag
 #pragma unroll
@@ -240,25 +326,26 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(const EvictArgs a) {
     uint32_t* const flags = a.flags + (int64_t(unit) * lanes + lane) * a.tiles;
     if (tid == 0) {
       __hip_atomic_store(&flags[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int32_t* below = a.below + int64_t(unit) * (a.tiles + 1) + tile;
-      const int32_t from = below[0], past = below[1];  // of the list: what lies in this tile's rows
-      if (past > from) {
-        const uint32_t last = min(uint32_t(past - 1) / a.rows + 1, tile);
-        for (uint32_t u = uint32_t(from) / a.rows; u < last; ++u)
+      if (past_below > first_below) {
+        const uint32_t last = min(a.rows_div.div(uint32_t(past_below - 1)) + 1, tile);
+        for (uint32_t u = a.rows_div.div(uint32_t(first_below)); u < last; ++u)
           while (__hip_atomic_load(&flags[u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(2);
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
-      if (to[u] >= 0) __builtin_nontemporal_store(V(v[u]), reinterpret_cast<V*>(base + to[u]));
+    for (int u = 0; u < kPieces; ++u) {
+      uint32_t r, piece;
+      if (place(u, r, piece)) __builtin_nontemporal_store(V(v[u]), reinterpret_cast<V*>(base + s_to[r] + int64_t(piece) * VB));
+    }
+    if (a.once) return;
   }
 }
 
 struct Plan {
   uint32_t most, rows, tiles, chunks, chunk_pieces;
   size_t moved, list, below, flags;
-  size_t bytes() const { return moved + list + below + flags + 256; }
+  size_t bytes() const { return moved + list + below + flags + kTickets * kTicketPitch * sizeof(uint32_t); }
 };
 
 size_t padded(size_t n) { return (n + 255) & ~size_t(255); }
@@ -277,7 +364,7 @@ int plan_of(int64_t batch, int64_t sets, int64_t set_bytes, int64_t vec, int64_t
   const size_t units = size_t(batch) * size_t(sets);
   CBK_REQUIRE(units * 2 * p->chunks * (size_t(p->tiles) + 1) < (size_t(1) << 31), "eviction: too many tiles for one launch");
   p->moved = padded(units * sizeof(uint2));
-  p->list = padded(units * p->most * sizeof(int32_t));
+  p->list = padded(units * p->most * sizeof(uint32_t));
   p->below = padded(units * (size_t(p->tiles) + 1) * sizeof(int32_t));
   p->flags = padded(units * 2 * p->chunks * p->tiles * sizeof(uint32_t));
   return CBK_OK;
@@ -363,10 +450,11 @@ int cbk_paged_evict(const cbk_kv_desc* kv, const int32_t* tables_dev, int64_t ta
   a.pieces_row = uint32_t(set_bytes / vec);
   a.set_bytes = set_bytes;
   a.chunk_div = FastDiv::make(p.chunk_pieces);
+  a.rows_div = FastDiv::make(p.rows);
   char* at = static_cast<char*>(workspace_dev);
-  a.ticket = reinterpret_cast<uint32_t*>(at);
-  a.moved = reinterpret_cast<uint2*>(at += 256);
-  a.list = reinterpret_cast<int32_t*>(at += p.moved);
+  a.tickets = reinterpret_cast<uint32_t*>(at);
+  a.moved = reinterpret_cast<uint2*>(at += kTickets * kTicketPitch * sizeof(uint32_t));
+  a.list = reinterpret_cast<uint32_t*>(at += p.moved);
   a.below = reinterpret_cast<int32_t*>(at += p.list);
   a.flags = reinterpret_cast<uint32_t*>(at + p.below);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -374,7 +462,9 @@ int cbk_paged_evict(const cbk_kv_desc* kv, const int32_t* tables_dev, int64_t ta
   hipLaunchKernelGGL(evict_choose_kernel, dim3(uint32_t(units)), dim3(kThreads), 0, s, a);
   if (int rc = launch_status("eviction's choice")) return rc;
   if (p.tiles == 0) return CBK_OK;
-  const dim3 grid(uint32_t(std::min<uint64_t>(units * 2 * p.chunks * p.tiles, uint64_t(cus) * 8)));
+  const uint64_t all = units * 2 * p.chunks * p.tiles;
+  const dim3 grid(uint32_t(std::min(all, uint64_t(cus) * kGroups)));
+  a.once = all == grid.x;
   switch (vec) {
     case 16: hipLaunchKernelGGL((evict_move_kernel<16>), grid, dim3(kMove), 0, s, a); break;
     case 8: hipLaunchKernelGGL((evict_move_kernel<8>), grid, dim3(kMove), 0, s, a); break;
