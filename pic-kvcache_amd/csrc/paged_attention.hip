@@ -89,8 +89,8 @@ struct PagedAttnArgs {
   // entry ((2 r + which) hkv + kv head) * rows * group + row * group + head
   float2* ml;
   float* o;
-  // for the keys' weights: the rows' maximum and sum, (b hkv + kv head) * rows
-  // * group + ..; the logits [b][tile][kv head][row, head][key of the tile]
+  // for the keys' weights: the rows' statistics, (b hkv + kv head) * rows * group
+  // + ..; the logits [b][tile][kv head][row, head][key of the tile]
   float2* stats;
   float* logits;
 };
@@ -140,6 +140,11 @@ __device__ __forceinline__ uint32_t context_of(const PagedAttnArgs& a, uint32_t 
 template <int KEYS> __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + KEYS - 1) / KEYS; }
 
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// What turns a row's logits into weights: the reference maximum (0 without one), 1 / sum.
+__device__ __forceinline__ float2 statistics(float m, float l) {
+  return make_float2(m == kNegInf ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
+}
 
 // N values of a row, rounded to the type
 template <int DT, int N>
@@ -553,9 +558,9 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
             }
           }
         }
-        if (j == 0 && live[t] && (!whole || LOGITS)) {
-          float2* to = whole ? a.stats : a.ml;
-          to[first_id + row0 + c] = make_float2(m[t], lt);
+        if (j == 0 && live[t]) {
+          if (!whole) a.ml[first_id + row0 + c] = make_float2(m[t], lt);
+          else if (LOGITS) a.stats[first_id + row0 + c] = statistics(m[t], lt);
         }
       } else {
         float* mine = lds[wave];
@@ -594,7 +599,7 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
             const float inverse = sum == 0.f ? 0.f : 1.f / sum;
             const float y[4] = {acc[0] * inverse, acc[1] * inverse, acc[2] * inverse, acc[3] * inverse};
             store_row<DT, 4>(to, y);
-            if (LOGITS && dim == 0) a.stats[(int64_t(seq) * a.hkv + h) * head_rows + n] = make_float2(top, sum);
+            if (LOGITS && dim == 0) a.stats[(int64_t(seq) * a.hkv + h) * head_rows + n] = statistics(top, sum);
           } else {
             const int64_t id = (int64_t(2 * range + (first_seq ? 0 : 1)) * a.hkv + h) * head_rows + n;
             *reinterpret_cast<f32x4*>(a.o + id * D + dim) = acc;
@@ -673,30 +678,50 @@ __global__ __launch_bounds__(32 * SUBS) void paged_attn_merge_kernel(const Paged
   const float y = l == 0.f ? 0.f : o / l;
   if constexpr (DT == CBK_DTYPE_F32) reinterpret_cast<float*>(to)[threadIdx.x] = y;
   else reinterpret_cast<uint16_t*>(to)[threadIdx.x] = uint16_t(Type<DT>::pack(y, 0.f));
-  if (a.stats && threadIdx.x == 0) a.stats[(int64_t(seq) * a.hkv + kvh) * head_rows + n] = make_float2(all, l);
+  if (a.stats && threadIdx.x == 0) a.stats[(int64_t(seq) * a.hkv + kvh) * head_rows + n] = statistics(all, l);
 }
 
-// weights[b, set, k] += the sum of key k's softmax weights over the set's rows,
-// in their order; a thread a key.
-template <int DT>
+// weights[b, set, k] += the sum of key k's softmax weights over the set's rows. A
+// thread takes 4 keys and every SUBS-th row; the SUBS sums are added in their order.
+template <int DT, int SUBS>
 __global__ __launch_bounds__(256) void key_weights_kernel(const PagedAttnArgs a, float* weights, int64_t batch_stride,
                                                           int64_t set_stride, uint32_t sets) {
-  constexpr int KEYS = Type<DT>::KEYS;
+  constexpr int KEYS = Type<DT>::KEYS, KT = 256 / SUBS;  // threads beside each other
   constexpr float kWeights = Type<DT>::kWeights;
-  const uint32_t seq = blockIdx.z, set = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
+  typedef Piece<4>::V16 V;
+  __shared__ f32x4 s_sum[SUBS == 1 ? 1 : 256];
+  const uint32_t seq = blockIdx.z, set = blockIdx.y, sub = threadIdx.x / KT;
+  const uint32_t key = 4 * (blockIdx.x * KT + threadIdx.x % KT);
   const uint32_t len = context_of(a, seq);
-  if (key >= len) return;
-  const uint32_t heads = a.hkv / sets, head_rows = a.rows * a.group;
-  const float* x = a.logits + ((int64_t(seq) * a.max_tiles + key / KEYS) * a.hkv + set * heads) * int64_t(head_rows * KEYS) + key % KEYS;
-  const float2* stats = a.stats + (int64_t(seq) * a.hkv + set * heads) * head_rows;
-  float sum = 0.f;
-  for (uint32_t n = 0; n < heads * head_rows; ++n) {
-    const float2 ml = stats[n];
-    const float ms = ml.x == kNegInf ? 0.f : ml.x, inverse = ml.y == 0.f ? 0.f : 1.f / ml.y;
-    sum = fmaf(__builtin_amdgcn_exp2f(fmaf(x[int64_t(n) * KEYS] - ms, kUnit, kWeights)), inverse, sum);
+  if (4 * blockIdx.x * KT >= len) return;
+  const uint32_t heads = a.hkv / sets, rows = heads * a.rows * a.group;
+  const float* x = a.logits + ((int64_t(seq) * a.max_tiles + key / KEYS) * a.hkv + set * heads) * int64_t(a.rows * a.group * KEYS) + key % KEYS;
+  const float2* stats = a.stats + (int64_t(seq) * a.hkv + set * heads) * (a.rows * a.group);
+  float* const to = weights + int64_t(seq) * batch_stride + int64_t(set) * set_stride + key;
+  f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (key < len) {
+#pragma unroll 4
+    for (uint32_t n = sub; n < rows; n += SUBS) {
+      const float2 st = stats[n];
+      const f32x4 y = *reinterpret_cast<const f32x4*>(x + int64_t(n) * KEYS);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(y[e] - st.x, kUnit, kWeights)), st.y, sum[e]);
+    }
   }
-  float* to = weights + int64_t(seq) * batch_stride + int64_t(set) * set_stride + key;
-  *to += sum;
+  if constexpr (SUBS > 1) {
+    s_sum[threadIdx.x] = sum;
+    __syncthreads();
+    if (sub != 0) return;
+    for (int i = 1; i < SUBS; ++i) sum += s_sum[i * KT + threadIdx.x];
+  }
+  if (key + 4 <= len) {
+    const f32x4 old = __builtin_bit_cast(f32x4, *reinterpret_cast<const V*>(to));
+    *reinterpret_cast<V*>(to) = __builtin_bit_cast(u32x4, old + sum);
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e)
+      if (key + e < len) to[e] += sum[e];
+  }
 }
 
 struct Plan {
@@ -759,8 +784,14 @@ int launch(const PagedAttnArgs& a, const Plan& p, float* weights, int64_t batch_
   else hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 8>), grid, dim3(256), 0, s, a);
   if (int rc = launch_status("paged attention merge")) return rc;
   if (weights == nullptr || a.max_len == 0) return CBK_OK;
-  hipLaunchKernelGGL((key_weights_kernel<DT>), dim3((a.max_len + 255) / 256, sets, a.batch), dim3(256), 0, s, a, weights,
-                     batch_stride, set_stride, sets);
+  const uint32_t set_rows = a.rows * a.hq / sets;
+  auto run = [&](auto kernel, uint32_t keys) {
+    hipLaunchKernelGGL(kernel, dim3((a.max_len + keys - 1) / keys, sets, a.batch), dim3(256), 0, s, a, weights, batch_stride,
+                       set_stride, sets);
+  };
+  if (set_rows <= 8) run(key_weights_kernel<DT, 1>, 1024);
+  else if (set_rows <= 64) run(key_weights_kernel<DT, 4>, 256);
+  else run(key_weights_kernel<DT, 32>, 32);
   return launch_status("key weights");
 }
 
