@@ -82,6 +82,7 @@ struct PagedAttnArgs {
   uint32_t num_blocks, max_len, max_tiles;
   uint32_t row_tiles;                    // of (row, head of the group) pairs
   uint32_t ranges;
+  bool whole;                            // range r is sequence r, and no partial results
   uint32_t heads, turns;                 // of a workgroup: KV heads, and waves that share one's tiles
   float c;                               // scale log2 e / kUnit
   FastDiv block_div;
@@ -202,30 +203,38 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
   const uint32_t kvh = head0 + (wave - turn * a.heads);
   const uint32_t head_rows = a.rows * a.group;
 
-  // the tiles of 64 sequences, a lane each (the first 64 are read once), and of all
-  const uint32_t tiles0 = lane < a.batch ? tiles_of<KEYS>(context_of(a, lane)) : 0u;
-  uint32_t all = tiles0;
-  for (uint32_t b = lane + 64; b < a.batch; b += 64) all += tiles_of<KEYS>(context_of(a, b));
-  const Ranges cut(wave_total(all), a.ranges);
-  uint32_t at = cut.first(range);
-  const uint32_t end = cut.first(range + 1);
-  if (at == end) return;
-  // the sequence that holds tile `at`, and the tiles before it
-  uint32_t seq = 0, before = 0;
-  for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-    uint32_t n = tiles0;
-    if (b0 > 0) n = b0 + lane < a.batch ? tiles_of<KEYS>(context_of(a, b0 + lane)) : 0u;
-    const uint32_t upto = before + wave_inclusive_scan(n);
-    const uint64_t past = __ballot(upto > at);
-    if (past) {
-      const int first = __builtin_ctzll(past);
-      seq = b0 + uint32_t(first);
-      before = uint32_t(__builtin_amdgcn_readlane(int(upto - n), first));
-      break;
+  // the lengths of the first 64 sequences, a lane each
+  const uint32_t len0 = a.whole ? context_of(a, range) : lane < a.batch ? context_of(a, lane) : 0u;
+  auto length = [&](uint32_t s) __attribute__((always_inline)) {
+    return s < 64 ? uint32_t(__builtin_amdgcn_readlane(int(len0), int(s))) : context_of(a, s);
+  };
+  uint32_t at = 0, end, seq = 0, before = 0;  // the range, the sequence that holds tile `at`, the tiles before it
+  if (a.whole) {
+    seq = range;
+    end = tiles_of<KEYS>(uint32_t(__builtin_amdgcn_readfirstlane(int(len0))));
+  } else {
+    const uint32_t tiles0 = tiles_of<KEYS>(len0);
+    uint32_t all = tiles0;
+    for (uint32_t b = lane + 64; b < a.batch; b += 64) all += tiles_of<KEYS>(context_of(a, b));
+    const Ranges cut(wave_total(all), a.ranges);
+    at = cut.first(range);
+    end = cut.first(range + 1);
+    if (at == end) return;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+      uint32_t n = tiles0;
+      if (b0 > 0) n = b0 + lane < a.batch ? tiles_of<KEYS>(context_of(a, b0 + lane)) : 0u;
+      const uint32_t upto = before + wave_inclusive_scan(n);
+      const uint64_t past = __ballot(upto > at);
+      if (past) {
+        const int first = __builtin_ctzll(past);
+        seq = b0 + uint32_t(first);
+        before = uint32_t(__builtin_amdgcn_readlane(int(upto - n), first));
+        break;
+      }
+      before = uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
     }
-    before = uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
+    seq = __builtin_amdgcn_readfirstlane(seq);
   }
-  seq = __builtin_amdgcn_readfirstlane(seq);
 
   // row tile t's row of this lane's column c of S^T
   uint32_t q_r[RT], q_h[RT];
@@ -238,18 +247,18 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
     q_h[t] = kvh * a.group + (live[t] ? n - q_r[t] * a.group : 0);
   }
 
-  for (bool first_seq = true; at < end; first_seq = false) {
-    uint32_t len = context_of(a, seq);
-    while (before + tiles_of<KEYS>(len) <= at) {  // empty sequences, and on to the next
+  for (bool first_seq = true;; first_seq = false) {
+    uint32_t len = a.whole ? uint32_t(__builtin_amdgcn_readfirstlane(int(len0))) : length(seq);
+    while (!a.whole && before + tiles_of<KEYS>(len) <= at) {  // empty sequences, and on to the next
       before += tiles_of<KEYS>(len);
-      len = context_of(a, ++seq);
+      len = length(++seq);
     }
     seq = __builtin_amdgcn_readfirstlane(seq);
     len = __builtin_amdgcn_readfirstlane(len);
     before = __builtin_amdgcn_readfirstlane(before);
     const uint32_t seq_end = before + tiles_of<KEYS>(len);
     const uint32_t stop = min(end, seq_end);
-    const bool whole = at == before && stop == seq_end;
+    const bool whole = at == before && stop == seq_end;  // (a.whole: an empty one, too)
     const uint32_t tile0 = at - before + turn;  // the wave's first tile of the sequence
     const int32_t count = stop - at > turn ? int32_t((stop - at - turn + turns - 1) / turns) : 0;
     const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
@@ -272,23 +281,27 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
     // The block table's entry of this lane's key of step i (a tile's keys, one
     // a lane; behind the last step, the last key's), and, from it, the tile's rows.
     // Keys past the context or in a page out of range are read from the
-    // first page and masked: their bits of the result are clear. A step behind
-    // the last reads that page's first row alone, so that every step has the
-    // same loads after it and none waits for more than its own.
+    // wave's first row and masked: their bits of the result are clear. A step behind
+    // the last reads that row alone, so that every step has the same loads after
+    // it and none waits for more than its own. (The first row of the cache
+    // instead, for all waves at the same time: 4 us at the end of a call.)
     auto entry = [&](int32_t i) __attribute__((always_inline)) {
       const uint32_t key = min((tile0 + turns * uint32_t(i)) * KEYS + (lane & (KEYS - 1)), len - 1);
       return uint32_t(table[a.block_div.div(key)]);
     };
+    uint64_t spare = 0;
     const char* const k_base = a.k_base + int64_t(kvh) * (D * T::ES) + 16 * j;
     const char* const v_base = a.v_base + int64_t(kvh) * (D * T::ES);
     auto load = [&](int32_t i, uint32_t page, Tl& to) __attribute__((always_inline)) {
       const uint32_t key = (tile0 + turns * uint32_t(i)) * KEYS + (lane & (KEYS - 1));
       const bool held = i < count && key < len && page < a.num_blocks;
-      uint64_t row = 0;
+      uint64_t row = spare;
       if (held) {
         const uint32_t blk = a.block_div.div(key);
         row = uint64_t(page) * uint64_t(a.block_stride) + uint64_t(key - blk * a.block_div.d) * uint64_t(a.token_stride);
       }
+      if (i == 0) spare = (uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(row >> 32))))) << 32) |
+                          uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(row))));
       auto row_of = [&](uint32_t from) __attribute__((always_inline)) {
         return uint64_t(uint32_t(__shfl(int(uint32_t(row)), int(from)))) |
                (uint64_t(uint32_t(__shfl(int(uint32_t(row >> 32)), int(from)))) << 32);
@@ -610,6 +623,7 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
       }
     }
     at = stop;
+    if (at >= end) break;
   }
 }
 
@@ -724,8 +738,16 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const PagedAttnArgs a,
   }
 }
 
+// Sequences stay whole where that gives a wave few more tiles than equal ranges (a merge
+// is as long as two or three), and few altogether (they may differ in length, and the
+// longest counts). us a call, ranges / whole, bf16, 32 heads over 8 x 128: 1 sequence of
+// 600 12.6 / 12.0, of 1000 (weights summed, 4 tiles instead of 1) 15.6 / 21.0; 64 of 256 to 1024
+// 38.5 / 35.9; 256 of 128 to 512 88 / 77; 64 of 4 K to 16 K (512 tiles both) 451 / 534.
+constexpr int64_t kMergeTiles = 2, kWholeTiles = 16;
+
 struct Plan {
   uint32_t rt, row_tiles, ranges, heads, turns, max_tiles;
+  bool whole;
   size_t ml, o, stats, logits;  // bytes of the scratch's parts
   size_t bytes() const { return ml + o + stats + logits; }
 };
@@ -743,21 +765,37 @@ int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int
   p->row_tiles = uint32_t((n + 16 * p->rt - 1) / (16 * p->rt));
   const uint32_t waves = uint32_t(max_waves(int(p->rt)));
   for (p->heads = waves; hkv % p->heads != 0;) --p->heads;
-  p->turns = waves / p->heads;
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
-  // a workgroup of each CU (registers); fewer where its waves would have less
-  // than a tile each
   p->max_tiles = uint32_t((max_len + keys - 1) / keys);
   const int64_t most = batch * int64_t(p->max_tiles);
   CBK_REQUIRE(most < (int64_t(1) << 31), "context tiles out of range");
-  const int64_t units = hkv / p->heads * int64_t(p->row_tiles);
-  int64_t ranges = (int64_t(cus) + units - 1) / units;
-  ranges = std::min(ranges, (most + p->turns - 1) / p->turns);
-  p->ranges = uint32_t(ranges > 1 ? ranges : 1);
+  // Short sequences: a range each, no second launch, the waves of a workgroup
+  // taking a head's tiles in turns while that leaves no CU two workgroups.
+  uint32_t heads = p->heads;
+  for (uint32_t h = p->heads; h > 0; --h)
+    if (hkv % h == 0 && batch * (hkv / h) * int64_t(p->row_tiles) <= cus) heads = h;
+  const int64_t groups = batch * (hkv / heads) * int64_t(p->row_tiles), turns = waves / heads;
+  const int64_t alone = (p->max_tiles + turns - 1) / turns * ((groups + cus - 1) / cus);  // a wave's tiles
+  const int64_t cut = (most * hkv * p->row_tiles + int64_t(cus) * waves - 1) / (int64_t(cus) * waves);
+  p->whole = alone <= std::min(cut + kMergeTiles, kWholeTiles);
+  if (p->whole) {
+    p->heads = heads;
+    p->turns = uint32_t(turns);
+    p->ranges = uint32_t(std::max<int64_t>(batch, 1));
+  } else {
+    // a workgroup of each CU (registers); fewer where its waves would have less
+    // than a tile each
+    p->turns = waves / p->heads;
+    const int64_t units = hkv / p->heads * int64_t(p->row_tiles);
+    int64_t ranges = (int64_t(cus) + units - 1) / units;
+    ranges = std::min(ranges, (most + p->turns - 1) / p->turns);
+    p->ranges = uint32_t(ranges > 1 ? ranges : 1);
+  }
   const size_t all_rows = size_t(rows) * size_t(hq);
-  p->ml = padded(size_t(2) * p->ranges * all_rows * sizeof(float2));
-  p->o = padded(size_t(2) * p->ranges * all_rows * size_t(d) * sizeof(float));
+  const size_t parts = p->whole ? 0 : size_t(2) * p->ranges * all_rows;
+  p->ml = padded(parts * sizeof(float2));
+  p->o = padded(parts * size_t(d) * sizeof(float));
   p->stats = weights ? padded(size_t(batch) * all_rows * sizeof(float2)) : 0;
   p->logits = weights ? padded(size_t(most) * size_t(keys) * all_rows * sizeof(float)) : 0;
   return CBK_OK;
@@ -779,10 +817,12 @@ template <int DT, int D>
 int launch(const PagedAttnArgs& a, const Plan& p, float* weights, int64_t batch_stride, int64_t set_stride, uint32_t sets,
            hipStream_t s) {
   if (int rc = p.rt == 1 ? launch_attn<DT, D, 1>(a, s) : launch_attn<DT, D, 2>(a, s)) return rc;
-  const dim3 grid(a.rows * a.hq, a.batch);
-  if (a.ranges > 16 * a.batch) hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 32>), grid, dim3(1024), 0, s, a);
-  else hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 8>), grid, dim3(256), 0, s, a);
-  if (int rc = launch_status("paged attention merge")) return rc;
+  if (!a.whole) {
+    const dim3 grid(a.rows * a.hq, a.batch);
+    if (a.ranges > 16 * a.batch) hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 32>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 8>), grid, dim3(256), 0, s, a);
+    if (int rc = launch_status("paged attention merge")) return rc;
+  }
   if (weights == nullptr || a.max_len == 0) return CBK_OK;
   const uint32_t set_rows = a.rows * a.hq / sets;
   auto run = [&](auto kernel, uint32_t keys) {
@@ -867,6 +907,7 @@ int cbk_paged_attention(const void* q_dev, int64_t q_batch_stride, int64_t q_row
   a.max_tiles = p.max_tiles;
   a.row_tiles = p.row_tiles;
   a.ranges = p.ranges;
+  a.whole = p.whole;
   a.heads = p.heads;
   a.turns = p.turns;
   a.c = scale * (kLog2e / kUnit);
