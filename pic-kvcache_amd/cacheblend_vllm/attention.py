@@ -13,6 +13,8 @@ the logits as the reference's bf16/f16 einsum and ``* scale`` do.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native
@@ -222,7 +224,8 @@ def _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, bloc
         raise ValueError("query rows must hold contiguous dims")
     check_tables(block_tables, context_lens, batch, block_size, desc.num_blocks)
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+        # (of a contiguous query in half the time)
+        out = torch.empty_like(query) if query.is_contiguous() else torch.empty(query.shape, dtype=query.dtype, device=device)
     else:
         _check_out(out, query)
     if batch * rows * hq == 0:
@@ -281,6 +284,11 @@ def paged_attention_int4(
     return out
 
 
+@functools.lru_cache(maxsize=256)  # steps of one shape ask again and again (0.7 us a call)
+def _paged_workspace_bytes(device: torch.device, *sizes: int) -> int:
+    return max(_native.on_device(device, _native.load().cbk_paged_attention_workspace_bytes, *sizes), 256)
+
+
 def paged_attention(
     query: torch.Tensor,
     kv_layer: KVLayer,
@@ -333,10 +341,9 @@ def paged_attention(
     o = out if out.dim() == 4 else out.unsqueeze(1)
     lib = _native.load()
     code = _native.DTYPE_CODES[query.dtype]
-    nbytes = _native.on_device(device, lib.cbk_paged_attention_workspace_bytes, batch, rows, hq, hkv, d,
-                               width * block_size, code, int(sets != 0))
+    nbytes = _paged_workspace_bytes(device, batch, rows, hq, hkv, d, width * block_size, code, int(sets != 0))
     # from torch's allocator on every call: a captured graph then owns its own
-    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     rc = _native.on_device(
         device, lib.cbk_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), batch, rows, hq, desc,
         hkv, d, tables.data_ptr() if width else None, tables.stride(0), width, lens.data_ptr(), float(scale), code,

@@ -19,6 +19,14 @@ namespace {
 // 38.5 / 35.9; 256 of 128 to 512 88 / 77; 64 of 4 K to 16 K (512 tiles both) 451 / 534.
 constexpr int64_t kMergeTiles = 2, kWholeTiles = 16;
 
+// A sequence in more ranges than this: more waves for a head and fewer heads for a workgroup
+// (neighbouring heads' rows are then not read at the same time, but there is less to merge). us
+// a call with 8 / 4 / 2 / 1 heads, 32 heads over 8 x 128 and 256 ranges with 8 of them: 1
+// sequence of 3000 14.8 / 15.1 / 13.8 / 13.6, of 8 K 17.9 / 16.8 / 15.3 / 14.8, of 32 K 31.7 / 31.0 /
+// 29.8 / 29.9, of 128 K 102 / 101 / 101 / 106; 8 of 4 K 23.2 / 25.7 / 24.9 / 25.4; 64 of 16 K 394 /
+// 392 / 410 / 459.
+constexpr int64_t kMostRanges = 64;
+
 // Pages of more bytes than this (twice the last cache level) are read past the caches; of
 // what fits there a part may be found again. us a call, kept / past, bf16, 32 heads over
 // 8 x 128: up to 67 MB (1 x 32 K) 24.6 / 25.1, 168 (64 x 1 K) 35.6 / 43.9, 460 (24 x 8 K)
@@ -66,11 +74,14 @@ int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int
   } else {
     // a workgroup of each CU (registers); fewer where its waves would have less
     // than a tile each
-    p->turns = waves / p->heads;
-    const int64_t units = hkv / p->heads * int64_t(p->row_tiles);
-    int64_t ranges = (int64_t(cus) + units - 1) / units;
-    ranges = std::min(ranges, (most + p->turns - 1) / p->turns);
-    p->ranges = uint32_t(ranges > 1 ? ranges : 1);
+    for (;;) {
+      p->turns = waves / p->heads;
+      const int64_t units = hkv / p->heads * int64_t(p->row_tiles);
+      const int64_t ranges = std::min((int64_t(cus) + units - 1) / units, (most + p->turns - 1) / p->turns);
+      p->ranges = uint32_t(ranges > 1 ? ranges : 1);
+      if (p->heads == 1 || ranges <= kMostRanges * batch) break;
+      for (--p->heads; hkv % p->heads != 0;) --p->heads;
+    }
   }
   const size_t all_rows = size_t(rows) * size_t(hq);
   const size_t parts = p->whole ? 0 : size_t(2) * p->ranges * all_rows;

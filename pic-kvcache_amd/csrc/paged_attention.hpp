@@ -732,37 +732,45 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
   }
 }
 
-// The sequences that more than one range holds, and those without keys: a
-// workgroup per row, every 32 lanes each SUBS-th range of it, each lane D / 32
-// dims.
+// The ranges that hold a sequence (wave-uniform): r0 .. r1, one alone if it is written whole.
+struct Held {
+  uint32_t r0, r1;
+};
+template <int KEYS>
+__device__ __forceinline__ Held ranges_of(const PagedAttnArgs& a, uint32_t seq, uint32_t len) {
+  if (a.whole || len == 0) return Held{0, 0};
+  // places before the sequence, and of all
+  uint32_t before = 0, total = 0;
+  for (uint32_t b = threadIdx.x & 63; b < a.batch; b += 64) {
+    const uint32_t t = places_of<KEYS>(context_of(a, b));
+    total += t;
+    before += b < seq ? t : 0u;
+  }
+  total = wave_total(total);
+  before = wave_total(before);
+  const Ranges cut(total, a.ranges);
+  return Held{cut.of(before + kHead), cut.of(before + kHead + tiles_of<KEYS>(len) - 1)};
+}
+
+// A row of a sequence that more than one range holds, or that has no keys: every 32
+// lanes each SUBS-th range, each lane D / 32 dims.
 template <int DT, int D, int SUBS>
-__global__ __launch_bounds__(32 * SUBS) void paged_attn_merge_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void merge_row(const PagedAttnArgs& a, uint32_t seq, uint32_t row) {
   constexpr int N = D / 32, KEYS = Type<DT>::KEYS;
   typedef float VecN __attribute__((ext_vector_type(N)));
   __shared__ float s_o[SUBS][D], s_l[SUBS], s_m[SUBS];
-  const uint32_t seq = blockIdx.y;
-  const uint32_t lane = threadIdx.x & 63, dim = threadIdx.x & 31, sub = threadIdx.x >> 5;
-  const uint32_t tiles = tiles_of<KEYS>(context_of(a, seq));
+  const uint32_t dim = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const uint32_t len = context_of(a, seq);
   const uint32_t head_rows = a.rows * a.group;
-  const uint32_t kvh = blockIdx.x / head_rows, n = blockIdx.x - kvh * head_rows;
+  const uint32_t kvh = row / head_rows, n = row - kvh * head_rows;
   float top = kNegInf, sum = 0.f;
   VecN acc = VecN(0.f);
-  if (tiles != 0) {
-    // places before the sequence, and of all
-    uint32_t before = 0, total = 0;
-    for (uint32_t b = lane; b < a.batch; b += 64) {
-      const uint32_t t = places_of<KEYS>(context_of(a, b));
-      total += t;
-      before += b < seq ? t : 0u;
-    }
-    total = wave_total(total);
-    before = wave_total(before);
-    const Ranges cut(total, a.ranges);
-    const uint32_t r0 = cut.of(before + kHead), r1 = cut.of(before + kHead + tiles - 1);
-    if (r0 == r1) return;  // written by its range
+  if (len != 0) {
+    const Held held = ranges_of<KEYS>(a, seq, len);
+    if (held.r0 == held.r1) return;  // written by its range
 #pragma unroll 4
-    for (uint32_t r = r0 + sub; r <= r1; r += SUBS) {
-      const int64_t id = (int64_t(2 * r + (r == r0 ? 1u : 0u)) * a.hkv + kvh) * head_rows + n;
+    for (uint32_t r = held.r0 + sub; r <= held.r1; r += SUBS) {
+      const int64_t id = (int64_t(2 * r + (r == held.r0 ? 1u : 0u)) * a.hkv + kvh) * head_rows + n;
       const float2 ml = a.ml[id];
       const VecN part = *reinterpret_cast<const VecN*>(a.o + id * D + N * dim);
       const float mn = fmaxf(top, ml.x), ms = mn == kNegInf ? 0.f : mn;
@@ -798,21 +806,23 @@ __global__ __launch_bounds__(32 * SUBS) void paged_attn_merge_kernel(const Paged
   if (a.stats && threadIdx.x == 0) a.stats[(int64_t(seq) * a.hkv + kvh) * head_rows + n] = statistics(all, l);
 }
 
+template <int DT, int D, int SUBS>
+__global__ __launch_bounds__(32 * SUBS) void paged_attn_merge_kernel(const PagedAttnArgs a) {
+  merge_row<DT, D, SUBS>(a, blockIdx.y, blockIdx.x);
+}
+
 // weights[b, set, k] += the sum of key k's softmax weights over the set's rows. A
 // thread takes 4 keys and every SUBS-th row; the SUBS sums are added in their order.
 template <int DT, int SUBS>
-__global__ __launch_bounds__(256) void key_weights_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void key_weights(const PagedAttnArgs& a, uint32_t seq, uint32_t len, uint32_t set, uint32_t chunk,
+                                            const float2* stats) {
   constexpr int KEYS = Type<DT>::KEYS, KT = 256 / SUBS;  // threads beside each other
   constexpr float kWeights = Type<DT>::kWeights;
   typedef Piece<4>::V16 V;
   __shared__ f32x4 s_sum[SUBS == 1 ? 1 : 256];
-  const uint32_t seq = blockIdx.z, set = blockIdx.y, sub = threadIdx.x / KT;
-  const uint32_t key = 4 * (blockIdx.x * KT + threadIdx.x % KT);
-  const uint32_t len = context_of(a, seq);
-  if (4 * blockIdx.x * KT >= len) return;
+  const uint32_t sub = threadIdx.x / KT, key = 4 * (chunk * KT + threadIdx.x % KT);
   const uint32_t heads = a.hkv / a.w_sets, rows = heads * a.rows * a.group;
   const float* x = a.logits + ((int64_t(seq) * a.max_tiles + key / KEYS) * a.hkv + set * heads) * int64_t(a.rows * a.group * KEYS) + key % KEYS;
-  const float2* stats = a.stats + (int64_t(seq) * a.hkv + set * heads) * (a.rows * a.group);
   float* const to = a.weights + int64_t(seq) * a.w_batch + int64_t(set) * a.w_set + key;
   f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
   if (key < len) {
@@ -840,6 +850,55 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const PagedAttnArgs a)
   }
 }
 
+template <int DT, int SUBS>
+__global__ __launch_bounds__(256) void key_weights_kernel(const PagedAttnArgs a) {
+  const uint32_t seq = blockIdx.z, set = blockIdx.y, len = context_of(a, seq);
+  if (blockIdx.x * (1024 / SUBS) >= len) return;
+  key_weights<DT, SUBS>(a, seq, len, set, blockIdx.x,
+                        a.stats + (int64_t(seq) * a.hkv + set * (a.hkv / a.w_sets)) * (a.rows * a.group));
+}
+
+// Both, for sets of few rows: the first workgroups merge a row each, the others take
+// keys, and the statistics of their rows from the partial results once more. One
+// launch less: 3 to 5 us.
+constexpr uint32_t kJoinRows = 64;
+template <int DT, int D, int SUBS>
+__global__ __launch_bounds__(256) void join_kernel(const PagedAttnArgs a) {
+  constexpr int KEYS = Type<DT>::KEYS;
+  const uint32_t seq = blockIdx.y, all_rows = a.rows * a.hq;
+  if (blockIdx.x < all_rows) {
+    merge_row<DT, D, 8>(a, seq, blockIdx.x);
+    return;
+  }
+  const uint32_t chunk = (blockIdx.x - all_rows) / a.w_sets, set = blockIdx.x - all_rows - chunk * a.w_sets;
+  const uint32_t len = context_of(a, seq);
+  if (chunk * (1024 / SUBS) >= len) return;
+  const uint32_t head_rows = a.rows * a.group, head0 = set * (a.hkv / a.w_sets), rows = a.hkv / a.w_sets * head_rows;
+  const Held held = ranges_of<KEYS>(a, seq, len);
+  const float2* stats = a.stats + (int64_t(seq) * a.hkv + head0) * head_rows;
+  if (held.r0 != held.r1) {
+    // 16 lanes a row
+    __shared__ float2 s_stats[kJoinRows];
+    const uint32_t lane = threadIdx.x & 15;
+    for (uint32_t n = threadIdx.x >> 4; n < rows; n += 16) {
+      float top = kNegInf, sum = 0.f;
+#pragma unroll 4
+      for (uint32_t r = held.r0 + lane; r <= held.r1; r += 16) {
+        const float2 ml = a.ml[(int64_t(2 * r + (r == held.r0 ? 1u : 0u)) * a.hkv + head0) * head_rows + n];
+        const float mn = fmaxf(top, ml.x), ms = mn == kNegInf ? 0.f : mn;
+        sum = __builtin_amdgcn_exp2f((top - ms) * kUnit) * sum + __builtin_amdgcn_exp2f((ml.x - ms) * kUnit) * ml.y;
+        top = mn;
+      }
+      const float most = row16_reduce(top, [](float x, float y) { return fmaxf(x, y); }), ms = most == kNegInf ? 0.f : most;
+      sum = row16_reduce(__builtin_amdgcn_exp2f((top - ms) * kUnit) * sum, [](float x, float y) { return x + y; });
+      if (lane == 0) s_stats[n] = statistics(most, sum);
+    }
+    __syncthreads();
+    stats = s_stats;
+  }
+  key_weights<DT, SUBS>(a, seq, len, set, chunk, stats);
+}
+
 template <int DT, int D, int RT, int MODE>
 int launch_attn(const PagedAttnArgs& a, hipStream_t s) {
   const uint64_t groups = uint64_t(a.hkv / a.heads) * a.row_tiles * ((a.ranges + 7) / 8 * 8);
@@ -861,14 +920,22 @@ int launch_mode(const PagedAttnArgs& a, hipStream_t s) {
 template <int DT, int D>
 int launch(const PagedAttnArgs& a, hipStream_t s) {
   if (int rc = a.rt == 1 ? launch_mode<DT, D, 1>(a, s) : launch_mode<DT, D, 2>(a, s)) return rc;
+  const bool weigh = a.weights != nullptr && a.max_len != 0;
+  const uint32_t set_rows = weigh ? a.rows * a.hq / a.w_sets : 0;
+  if (weigh && !a.whole && set_rows <= kJoinRows) {
+    const uint32_t keys = set_rows <= 8 ? 1024 : 256;
+    const dim3 grid(a.rows * a.hq + (a.max_len + keys - 1) / keys * a.w_sets, a.batch);
+    if (set_rows <= 8) hipLaunchKernelGGL((join_kernel<DT, D, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((join_kernel<DT, D, 4>), grid, dim3(256), 0, s, a);
+    return launch_status("paged attention merge and key weights");
+  }
   if (!a.whole) {
     const dim3 grid(a.rows * a.hq, a.batch);
     if (a.ranges > 16 * a.batch) hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 32>), grid, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 8>), grid, dim3(256), 0, s, a);
     if (int rc = launch_status("paged attention merge")) return rc;
   }
-  if (a.weights == nullptr || a.max_len == 0) return CBK_OK;
-  const uint32_t set_rows = a.rows * a.hq / a.w_sets;
+  if (!weigh) return CBK_OK;
   auto run = [&](auto kernel, uint32_t keys) {
     hipLaunchKernelGGL(kernel, dim3((a.max_len + keys - 1) / keys, a.w_sets, a.batch), dim3(256), 0, s, a);
   };
