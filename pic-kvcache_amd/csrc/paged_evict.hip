@@ -110,7 +110,7 @@ __device__ __forceinline__ uint32_t find_bin(const uint32_t* bins, uint32_t& wan
 __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs a) {
   __shared__ __attribute__((aligned(16))) uint32_t bins[3][2048];
   __shared__ float held[kPass];       // the weights of a pass's keys
-  __shared__ uint32_t places[kPass];  // where they go
+  __shared__ uint32_t places[kPass];  // these as ordered numbers; then where the keys go
   __shared__ uint32_t scratch[kThreads / 64], s_gone;
   const uint32_t unit = blockIdx.x, b = unit / a.sets, set = unit - b * a.sets, tid = threadIdx.x;
   const uint32_t n = uint32_t(min(max(a.lens[b], 0), int32_t(a.max_len)));
@@ -123,12 +123,21 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
     return;
   }
   float* const w = a.weights + int64_t(b) * a.w_batch + int64_t(set) * a.w_set;
+  const int32_t* const table = a.tables + int64_t(b) * a.table_stride;
+  uint32_t page[kPass / kThreads];  // of the keys i0 + tid + k kThreads
   auto fetch = [&](uint32_t i0) {
     float x[kPass / kThreads];
 #pragma unroll
-    for (uint32_t k = 0; k < kPass / kThreads; ++k) x[k] = w[min(i0 + tid + k * kThreads, n - 1)];
+    for (uint32_t k = 0; k < kPass / kThreads; ++k) {
+      const uint32_t i = min(i0 + tid + k * kThreads, n - 1);
+      x[k] = w[i];
+      page[k] = uint32_t(table[a.block_div.div(i)]);
+    }
 #pragma unroll
-    for (uint32_t k = 0; k < kPass / kThreads; ++k) held[tid + k * kThreads] = x[k];
+    for (uint32_t k = 0; k < kPass / kThreads; ++k) {
+      held[tid + k * kThreads] = x[k];
+      places[tid + k * kThreads] = ordered(x[k]);
+    }
   };
   fetch(0);
   uint32_t* const flags = a.flags + int64_t(unit) * 2 * a.chunks * a.tiles;
@@ -156,14 +165,14 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
         }
         const uint32_t past = min(hi, i0 + uint32_t(kPass));
         for (uint32_t j = tid; i0 + j < past; j += 4 * kThreads) {
-          float x[4];
+          uint32_t key[4];
 #pragma unroll
-          for (uint32_t u = 0; u < 4; ++u) x[u] = held[(j + u * kThreads) % kPass];
+          for (uint32_t u = 0; u < 4; ++u) key[u] = places[(j + u * kThreads) % kPass];
 #pragma unroll
           for (uint32_t u = 0; u < 4; ++u) {
-            const uint32_t i = i0 + j + u * kThreads, key = ordered(x[u]);
-            const bool alike = T == 32 || ((key ^ limit) >> (T & 31)) == 0;
-            if (i < past && i >= lo && alike) count_bin(counts, (key >> (T - W)) & ((1u << W) - 1));
+            const uint32_t i = i0 + j + u * kThreads;
+            const bool alike = T == 32 || ((key[u] ^ limit) >> (T & 31)) == 0;
+            if (i - lo < past - lo && alike) count_bin(counts, (key[u] >> (T - W)) & ((1u << W) - 1));
           }
         }
       }
@@ -178,7 +187,6 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
 
   // the keys in order: the list of their slots, their weights moved down, the counts at tiles' starts
   uint32_t* const list = a.list + int64_t(unit) * a.most;
-  const int32_t* const table = a.tables + int64_t(b) * a.table_stride;
   uint32_t base = 0;
   for (uint32_t i0 = 0; i0 < n; i0 += kPass) {
     if (n > kPass) {
@@ -190,15 +198,17 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
     // a thread's neighbours (an odd number: they lie in different banks)
     const uint32_t per = ((count + kThreads - 1) / kThreads) | 1u, from = tid * per, past = min(from + per, count);
     uint32_t kinds = 0, both = 0;  // two bits a key (1: stays, 2: has the lowest weight); counts of the two
-    static_assert(kPass / kThreads <= 8, "two bits each");
+    static_assert(kPass / kThreads <= 8, "nine keys at most, two bits each");
+    for (uint32_t k = 0; k < per; k += 3) {
 #pragma unroll
-    for (uint32_t k = 0; k < 9; ++k) {
-      const uint32_t i = i0 + from + k, key = ordered(held[(from + k) % kPass]);
-      uint32_t is = !some || key < limit ? 0u : key > limit ? 1u : 2u;
-      if (i < lo || i >= hi) is = 1u;
-      if (k >= per || from + k >= count) is = 0u;
-      kinds |= is << (2 * k);
-      both += (is & 1u) | (is >> 1 << 16);
+      for (uint32_t u = 0; u < 3; ++u) {
+        const uint32_t j = from + k + u, i = i0 + j, key = places[j % kPass];
+        uint32_t is = !some || key < limit ? 0u : key > limit ? 1u : 2u;
+        if (i < lo || i >= hi) is = 1u;
+        if (k + u >= per || j >= count) is = 0u;
+        kinds |= is << (2 * (k + u));
+        both += (is & 1u) | (is >> 1 << 16);
+      }
     }
     uint32_t total;
     const uint32_t before = block_exclusive_scan<kThreads>(both, scratch, &total);
@@ -216,21 +226,16 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
     const uint64_t leave = __ballot(gone < n);
     if (leave && int(tid & 63) == __builtin_ctzll(leave)) atomicMin(&s_gone, gone);
     __syncthreads();
-    for (uint32_t k = tid; k < count; k += 4 * kThreads) {
-      uint32_t page[4];  // (four at a time before their stores)
 #pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) page[u] = uint32_t(table[a.block_div.div(min(i0 + k + u * kThreads, n - 1))]);
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) {
-        const uint32_t j = k + u * kThreads, i = i0 + j;
-        if (j >= count) break;
-        const uint32_t to = places[j], blk = a.block_div.div(i);
-        if (to != kNoSlot) {
-          list[to] = page[u] < a.num_blocks ? page[u] * a.block_div.d + (i - blk * a.block_div.d) : kNoSlot;
-          w[to] = held[j];  // places up to i: they are in LDS by now
-        }
-        if (i >= keep) w[i] = 0.f;
+    for (uint32_t k = 0; k < kPass / kThreads; ++k) {
+      const uint32_t j = tid + k * kThreads, i = i0 + j;
+      if (j >= count) break;
+      const uint32_t to = places[j], blk = a.block_div.div(i);
+      if (to != kNoSlot) {
+        list[to] = page[k] < a.num_blocks ? page[k] * a.block_div.d + (i - blk * a.block_div.d) : kNoSlot;
+        w[to] = held[j];  // places up to i: they are in LDS by now
       }
+      if (i >= keep) w[i] = 0.f;
     }
     const uint32_t used = min(total >> 16, equal);
     base += (total & 0xffffu) + used;
