@@ -208,29 +208,34 @@ def _check_tokens(query: torch.Tensor) -> None:
 
 def _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, block_size, out):
     """The checks that attention over pages of any type makes of a step's tensors:
-    (query of four dims, out, tables and lengths as the kernels take them)."""
+    (batch, rows, query heads, the query's strides, out, its strides, tables, lengths),
+    strides of sequences, rows and heads, tables and lengths as the kernels take them."""
     device = query.device
     if plane.device != device:
         raise ValueError(f"query is on {device}, the cache on {plane.device}")
-    q = query if query.dim() == 4 else query.unsqueeze(1)
-    batch, rows, hq = q.shape[:3]
-    if q.shape[3] != d:
-        raise ValueError(f"query head size {q.shape[3]} does not match the pages' {d}")
+    shape, strides = query.shape, query.stride()
+    one = len(shape) == 3  # one token a sequence
+    batch, rows, hq = (shape[0], 1, shape[1]) if one else shape[:3]
+    if shape[-1] != d:
+        raise ValueError(f"query head size {shape[-1]} does not match the pages' {d}")
     if d not in (64, 128):
         raise ValueError(f"head size {d}: 64 or 128 supported")
     if hkv == 0 or hq % hkv or (hq == 0 and batch * rows):
         raise ValueError(f"query heads ({hq}) must be divisible by KV heads ({hkv})")
-    if q.stride(3) != 1:
+    if strides[-1] != 1:
         raise ValueError("query rows must hold contiguous dims")
     check_tables(block_tables, context_lens, batch, block_size, desc.num_blocks)
     if out is None:
         # (of a contiguous query in half the time)
-        out = torch.empty_like(query) if query.is_contiguous() else torch.empty(query.shape, dtype=query.dtype, device=device)
+        out = torch.empty_like(query) if query.is_contiguous() else torch.empty(shape, dtype=query.dtype, device=device)
     else:
         _check_out(out, query)
+    o_strides = out.stride()
+    if one:
+        strides, o_strides = (strides[0], 0, strides[1]), (o_strides[0], 0, o_strides[1])
     if batch * rows * hq == 0:
-        return q, out, None, None
-    return q, out, *device_tables(block_tables, context_lens, device)
+        return batch, rows, hq, strides[:3], out, o_strides[:3], None, None
+    return batch, rows, hq, strides[:3], out, o_strides[:3], *device_tables(block_tables, context_lens, device)
 
 
 def paged_attention_int4(
@@ -262,22 +267,21 @@ def paged_attention_int4(
     _check_tokens(query)
     desc, row, plane = paged_layer(kv_layer, block_size)
     hkv, d = int4_geometry(plane.dtype, row)
-    q, out, tables, lens = _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, block_size, out)
+    batch, rows, hq, q_strides, out, o_strides, tables, lens = _decode_tensors(
+        query, plane, desc, hkv, d, block_tables, context_lens, block_size, out)
     device = query.device
-    batch, rows, hq = q.shape[:3]
     width = block_tables.shape[1]
     if batch * rows * hq == 0:
         return out
-    o = out if out.dim() == 4 else out.unsqueeze(1)
     lib = _native.load()
     nbytes = _native.on_device(device, lib.cbk_paged_attention_int4_workspace_bytes, batch, rows, hq, hkv, d,
                                width * block_size, _native.DTYPE_CODES[query.dtype])
     # from torch's allocator on every call: a captured graph then owns its own
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     rc = _native.on_device(
-        device, lib.cbk_paged_attention_int4, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), batch, rows, hq,
+        device, lib.cbk_paged_attention_int4, query.data_ptr(), *q_strides, batch, rows, hq,
         desc, hkv, d, tables.data_ptr() if width else None, tables.stride(0), width, lens.data_ptr(), float(scale),
-        _native.DTYPE_CODES[query.dtype], o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), ws.data_ptr(), ws.numel(),
+        _native.DTYPE_CODES[query.dtype], out.data_ptr(), *o_strides, ws.data_ptr(), ws.numel(),
         _native.stream_handle(device),
     )
     _native.check(rc, "paged_attention_int4")
@@ -328,26 +332,25 @@ def paged_attention(
     if plane.dtype != query.dtype or len(row) != 2:
         raise ValueError(f"the pages hold {plane.dtype} rows {tuple(row)}, the queries are {query.dtype}")
     hkv, d = row
-    q, out, tables, lens = _decode_tensors(query, plane, desc, hkv, d, block_tables, context_lens, block_size, out)
+    batch, rows, hq, q_strides, out, o_strides, tables, lens = _decode_tensors(
+        query, plane, desc, hkv, d, block_tables, context_lens, block_size, out)
     device = query.device
-    batch, rows, hq = q.shape[:3]
     width = block_tables.shape[1]
     sets, w = 0, (None, 0, 0)
     if key_weights is not None:
-        sets = check_key_weights(key_weights, batch, hkv, width * block_size, device)
-        w = (key_weights.data_ptr(), key_weights.stride(0), key_weights.stride(1))
+        sets, *strides = check_key_weights(key_weights, batch, hkv, width * block_size, device)
+        w = (key_weights.data_ptr(), *strides)
     if batch * rows * hq == 0:
         return out
-    o = out if out.dim() == 4 else out.unsqueeze(1)
     lib = _native.load()
     code = _native.DTYPE_CODES[query.dtype]
     nbytes = _paged_workspace_bytes(device, batch, rows, hq, hkv, d, width * block_size, code, int(sets != 0))
     # from torch's allocator on every call: a captured graph then owns its own
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     rc = _native.on_device(
-        device, lib.cbk_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), batch, rows, hq, desc,
+        device, lib.cbk_paged_attention, query.data_ptr(), *q_strides, batch, rows, hq, desc,
         hkv, d, tables.data_ptr() if width else None, tables.stride(0), width, lens.data_ptr(), float(scale), code,
-        o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), *w, sets, ws.data_ptr(), ws.numel(),
+        out.data_ptr(), *o_strides, *w, sets, ws.data_ptr(), nbytes,
         _native.stream_handle(device),
     )
     _native.check(rc, "paged_attention")

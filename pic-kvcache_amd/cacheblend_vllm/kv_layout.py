@@ -444,17 +444,20 @@ def device_tables(block_tables: torch.Tensor, context_lens: torch.Tensor,
     return tables, lens if lens.is_contiguous() else lens.contiguous()
 
 
-def check_key_weights(weights: torch.Tensor, batch: int, heads: int, keys: int, device: torch.device) -> int:
-    """The sets of heads (1, or one a KV head) of ``[batch, sets, keys]`` float32 weights that lie apart."""
-    if weights.dim() != 3 or weights.shape[0] != batch or weights.shape[1] not in (1, heads) or weights.shape[2] < keys:
-        raise ValueError(f"key weights are {tuple(weights.shape)}, expected [{batch}, 1 or {heads}, at least {keys}]")
+def check_key_weights(weights: torch.Tensor, batch: int, heads: int, keys: int, device: torch.device) -> tuple:
+    """(sets, strides of sequences and sets) of ``[batch, sets, keys]`` float32
+    weights that lie apart; sets of heads: 1, or one a KV head."""
+    shape = weights.shape
+    if len(shape) != 3 or shape[0] != batch or shape[1] not in (1, heads) or shape[2] < keys:
+        raise ValueError(f"key weights are {tuple(shape)}, expected [{batch}, 1 or {heads}, at least {keys}]")
     if weights.dtype != torch.float32 or weights.device != device:
         raise ValueError(f"key weights must be float32 on {device}")
-    if weights.stride(2) != 1 and weights.shape[2] > 1:
+    strides = weights.stride()
+    if strides[2] != 1 and shape[2] > 1:
         raise ValueError("key weights must hold contiguous keys")
     if not rows_apart(weights):
         raise ValueError("key weights must not overlap")
-    return weights.shape[1]
+    return shape[1], strides[0], strides[1]
 
 
 def evict_paged_kv(
@@ -493,7 +496,7 @@ def evict_paged_kv(
     batch = block_tables.shape[0]
     check_tables(block_tables, context_lens, batch, block_size, desc.num_blocks)
     width = block_tables.shape[1]
-    sets = check_key_weights(key_weights, batch, row[0], width * block_size, device)
+    sets, *w_strides = check_key_weights(key_weights, batch, row[0], width * block_size, device)
     first, recent = int(first), int(recent)
     if first < 0 or recent < 0:
         raise ValueError(f"first {first} and recent {recent} must not be negative")
@@ -518,8 +521,8 @@ def evict_paged_kv(
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     rc = _native.on_device(
         device, lib.cbk_paged_evict, desc, tables.data_ptr() if width else None, tables.stride(0), width, lens.data_ptr(),
-        batch, key_weights.data_ptr(), key_weights.stride(0), key_weights.stride(1), sets, keep, _native.ptr(keeps), first,
-        recent, new_lens.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(device),
+        batch, key_weights.data_ptr(), *w_strides, sets, keep, _native.ptr(keeps), first, recent,
+        new_lens.data_ptr(), ws.data_ptr(), ws.numel(), _native.stream_handle(device),
     )
     _native.check(rc, "evict_paged_kv")
     return new_lens
