@@ -520,13 +520,13 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
  * queries' dtype, as cbk_paged_attention_int4 over 4-bit pages: q and out [batch,
  * rows, hq, head_dim], strides in ELEMENTS; row r of a sequence sees keys up to
  * lens_dev[b] - rows + r (lengths are clamped to the tables), a page out of range
- * holds no keys, a row that sees none is zero; head_dim 64 or 128. Logits, softmax
- * and sums in float32; 16-bit softmax weights enter the product with the values in
- * two parts of the type. Pages aligned to their elements.
+ * holds no keys, a row that sees none, or only logits of -inf, is zero; head_dim 64
+ * or 128. Logits, softmax and sums in float32; 16-bit softmax weights enter the
+ * product with the values in two parts of the type. Pages aligned to their elements.
  * key_weights_dev (NULL: none) [batch, weight_sets, max_len] float32, strides in
  * elements, contiguous keys: to key k of sequence b, k < lens_dev[b], the softmax
  * weights that the rows give it are added, of a KV head's query heads (weight_sets
- * = hkv) or of all (1); in the rows' order, no atomics.
+ * = hkv) or of all (1); in a fixed order, no atomics.
  * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
  * function gives on the current device, max_len = table_width * block_size; with
  * key weights it holds the logits, 4 bytes for each of rows * hq and key of the

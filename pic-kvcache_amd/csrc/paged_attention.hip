@@ -49,6 +49,9 @@ int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int
   CBK_REQUIRE(rows > 0 && hq < (1 << 16) && rows < (1 << 16) && rows * hq < (int64_t(1) << 31), "rows or heads out of range");
   CBK_REQUIRE(max_len >= 0 && max_len < (int64_t(1) << 31) - 32, "context out of range");
   const int64_t n = rows * (hq / hkv), keys = dtype == CBK_DTYPE_F32 ? 16 : 32;
+  // (two row tiles a wave take the registers of two waves: half as many read at a time, but
+  // each tile once for both: 32 sequences of up to 8 K, 5 rows of 32 heads over 8, 112 us, one
+  // row tile a wave 142; 9 of 3 K, 4 rows of 40 over 8, 24.3 and 25.4; four spill)
   p->rt = n <= 16 ? 1 : 2;
   p->row_tiles = uint32_t((n + 16 * p->rt - 1) / (16 * p->rt));
   const uint32_t waves = uint32_t(max_waves(int(p->rt)));
@@ -84,6 +87,8 @@ int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int
     }
   }
   const size_t all_rows = size_t(rows) * size_t(hq);
+  CBK_REQUIRE(!weights || size_t(most) * size_t(keys) <= (size_t(1) << 44) / all_rows, "logits of %zu rows and %lld tiles are too many",
+              all_rows, (long long)most);
   const size_t parts = p->whole ? 0 : size_t(2) * p->ranges * all_rows;
   p->ml = padded(parts * sizeof(float2));
   p->o = padded(parts * size_t(d) * sizeof(float));

@@ -10,11 +10,12 @@
 //
 // Bound by HBM: each key and value row is read once for all rows of a group.
 // Beside that the matrix cores and the VALU have little to do (a 32-key tile of
-// a KV head, 16 KB, is 16 MFMAs and some 300 VALU instructions for up to 16
-// rows), so the kernel is laid out for loads in flight and nothing else: a wave
-// takes a tile of one KV head at a time straight into registers, K and V of
-// the next tile requested before this one's are waited for, no LDS and no
-// barrier on the way.
+// a KV head, 16 KB, is 24 MFMAs and some 250 VALU instructions for up to 16
+// rows, a tenth of the time its bytes take), so the kernel is laid out for loads
+// in flight and nothing else: a wave takes a tile of one KV head at a time straight
+// into registers, K and V of the next tile requested before this one's are waited for,
+// no LDS and no barrier on the way. 64 sequences of 4 K to 16 K keys, 32 heads over 8 x
+// 128, bf16, 2.6 GB: 396 us, 6.6 TB/s (what a 4 GiB copy moves: 4.9).
 //  - S^T = K . Q^T: lane (j = lane / 16, c) reads 16 bytes of key c's row, dims
 //    32 st + 8 j .., which is an operand of step st as it is.
 //  - O = P . V: S^T leaves lane (j, c) with keys 4 j .. 4 j + 3 of each 16-key
@@ -25,15 +26,21 @@
 //    lane's 8 keys x 8 dims. float32: 16-key tiles, four 16x16x4 products where
 //    16 bits have one 16x16x32, the same lanes' keys and no permutes.
 // 16-bit weights enter the second product in two parts, so they are held to 2^-16
-// (bf16) or 2^-22 (float16) of themselves (below that, float16: 2^-30 of the
-// largest); sums and statistics are float32.
+// (bf16) or 2^-22 (float16) of themselves (below 2^-8 of the largest, float16: 2^-30 of
+// that); sums and statistics are float32.
+// The waits for loads are the compiler's counts of what was requested later, which only
+// straight code keeps exact: so a step behind the last loads too (nothing, or a row that
+// is there), and pages in whole 16-key pieces (FAST) are addressed by scalars, for
+// vector registers that hold an address now and a tile's rows then are waited for
+// (64 x 16 K: 451 us; 397 with both, and the caches passed by).
 //
 // The batch's tiles are cut into equal ranges (paged_ranges.hpp); a workgroup
 // takes one, a wave a KV head, or several waves a head's tiles in turns. A
 // sequence that one range holds whole is written at once, the others' partial
 // results are merged by a second launch. For the keys' weights the waves leave
 // the logits in scratch (4 bytes a row and key, beside 4 D or 8 D bytes a key that
-// they read), and a third launch turns them into weights with the rows' statistics.
+// they read), and the second launch turns them into weights with the rows'
+// statistics, or, for sets of many rows, a third one does.
 #pragma once
 
 #include <type_traits>
@@ -83,7 +90,9 @@ int launch_paged_attention_f16(const PagedAttnArgs& a, int64_t head_dim, hipStre
 int launch_paged_attention_f32(const PagedAttnArgs& a, int64_t head_dim, hipStream_t s);
 
 // Ranges are cut in places: a sequence has one for each tile, and kHead before
-// them, for what a workgroup does at a sequence's start and end.
+// them, for what a workgroup does at a sequence's start and end. (us with 0 / 1 / 2 / 4, bf16,
+// 128: 9 sequences of up to 3 K, 4 rows of 40 heads over 8, 26.2 / 24.3 / 24.3 / 24.5; 8 of 4 K, 32
+// heads over 8, 25.5 / 23.5 / 23.7 / 23.6; 64 of 16 K 397 / 397 / 397 / 400.)
 constexpr uint32_t kHead = 1;
 
 // waves of a workgroup, at most: two a SIMD; one where two row tiles take its registers
@@ -117,7 +126,6 @@ template <> struct Piece<4> {
 
 typedef const __attribute__((address_space(4))) int32_t* Const32;  // read by scalar loads
 constexpr int kBufferWord = 0x00027000;  // of a buffer's descriptor: bytes, 32-bit data
-
 
 // What differs between the types. KEYS: of a tile; kWeights: log2 of a weight at the
 // reference maximum. 2^-18: a weight is 2^-10 at most, so that sums of 1000 of the
@@ -433,8 +441,9 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
     }
 
     // The logits of the wave's tiles wait in LDS and leave it together: written tile by
-    // tile they break up the reads of all memory channels (64 sequences of up to 16 K
-    // keys, 3% of the bytes: 555 us, 400 without them).
+    // tile they break up the reads of all memory channels (64 sequences of 4 K to 16 K
+    // keys, 3% of the bytes: 555 us, 400 without them; the
+    // whole call 586, 515 so).
     float* const stage = lds[wave];
     const uint32_t stage_floats = min(head_rows - row_tile * ROWS, uint32_t(ROWS)) * KEYS, stage_room = kLds / stage_floats;
     uint32_t staged = 0;

@@ -5,21 +5,30 @@
 // Two launches. A workgroup per (sequence, set of heads) chooses: the weight of
 // the last key that stays is found digit by digit (11, 11 and 10 bits of the
 // weights as ordered whole numbers, histograms in LDS; up to 8192 weights stay in
-// LDS meanwhile, more are read again from L2), then one pass over the keys in order writes the list of
-// those that stay and moves their weights. Then tiles of rows move.
+// LDS meanwhile, more are read again from L2), then one pass over the keys in order
+// writes the list of those that stay and moves their weights. Then tiles of rows move.
 //
 // The rows move within their own pages, so a row must not be written before
 // what lies there has been read. Row j of the list comes from a place not before
 // it, so what lies in a tile's rows is read by the tile itself or by
 // tiles before it, of which the choice leaves the bounds: a tile reads all of its
 // rows into registers, says so in a flag, waits for the flags of the one or
-// two tiles that read from its rows, and writes. Tiles are handed out by
-// counters, a unit's in order: a tile only waits for tiles that were handed out
+// two tiles that read from its rows, and writes. A counter for each set's plane
+// hands out its tiles in order: a tile only waits for tiles that were handed out
 // before, to workgroups that run, and these read, and raise their flag, before they
 // wait for anything; so every wait ends, whatever else the GPU does. (Only reads have to
 // be done, nothing is passed on: the flags need no fences, only loads that
-// have come back.)
-// Bound by HBM: the rows behind the first one that leaves are read and written once.
+// have come back.) As many workgroups take a tile as there are tiles that move;
+// the others that the tables and `keep` have room for end at once.
+// Bound by HBM: the rows behind the first one that leaves are read and written once. A
+// workgroup takes one tile and ends: one that went on to the next waited for its stores
+// before it had its next loads (32 sequences of 2 K to 8 K to 4 K, 8 x 128, bf16, 0.7 GB: the
+// move 217 us, 114 now, 6.2 TB/s). A set's tiles turn through the XCDs, which a column of
+// its own on one leaves unequal work (both kernels there 149 us, 131 turned), and take 68
+// registers, so that 7 fit a SIMD (350 us with 254, to which the compiler unrolls the pieces'
+// addresses). 32 KB a tile: 16 KB and 64 KB take 33.6 us for 4 sequences of 8 K to 2 K, not
+// 31.5, and 47.0 and 45.7 for 32 of 8 K to 7000 for each head by itself, not 42.9.
+// The choice is bound by its chain of loads and barriers: 9 us for 1 K keys, 14 for 8 K.
 #include <algorithm>
 #include <type_traits>
 
@@ -34,8 +43,8 @@ constexpr int kMove = 256;       // of a move
 constexpr int kPieces = 8;       // a thread's pieces of a tile
 constexpr uint32_t kMaxRows = 512;
 constexpr uint32_t kNoSlot = 0xffffffffu;  // a page out of range
-constexpr uint32_t kGroups = 128;  // workgroups of a move for each CU, at most
-constexpr uint32_t kTickets = 16, kTicketPitch = 32;  // counters, a cache line each
+constexpr uint32_t kTicketPitch = 32;    // a counter in each cache line
+constexpr uint32_t kGroups = 1u << 22;   // workgroups of a launch, at most (a grid's 2^32 threads are 2^24)
 
 struct EvictArgs {
   char* k_base;
@@ -56,10 +65,10 @@ struct EvictArgs {
   // rows [k rows, (k + 1) rows) of the list), split into `chunks` of columns
   uint32_t rows, tiles, chunks, chunk_pieces, pieces_row;
   int64_t set_bytes;
-  bool once;  // a workgroup a tile
+  uint32_t group0;  // of this launch
   FastDiv chunk_div, rows_div;
   // scratch: for each (sequence, set) the rows that move [begin, end), the list of slots [most],
-  // the keys below k rows that stay [tiles + 1], and the flags [2 planes][chunks][tiles]
+  // the keys below k rows that stay [tiles + 1], and by [2 planes][chunks] the flags [tiles] and a counter
   uint2* moved;
   uint32_t* list;
   int32_t* below;
@@ -116,7 +125,6 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
   const uint32_t n = uint32_t(min(max(a.lens[b], 0), int32_t(a.max_len)));
   uint32_t keep = a.keeps ? uint32_t(max(a.keeps[b], 0)) : a.keep;
   keep = max(keep, a.first + a.recent);
-  if (unit == 0 && tid < kTickets) a.tickets[tid * kTicketPitch] = 0;
   if (set == 0 && tid == 0) a.new_lens[b] = int32_t(min(n, keep));
   if (n <= keep) {
     if (tid == 0) a.moved[unit] = make_uint2(0, 0);
@@ -142,6 +150,7 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
   fetch(0);
   uint32_t* const flags = a.flags + int64_t(unit) * 2 * a.chunks * a.tiles;
   for (uint32_t i = tid; i < 2 * a.chunks * a.tiles; i += kThreads) flags[i] = 0;
+  for (uint32_t i = tid; i < 2 * a.chunks; i += kThreads) a.tickets[(int64_t(unit) * 2 * a.chunks + i) * kTicketPitch] = 0;
   int32_t* const below = a.below + int64_t(unit) * (a.tiles + 1);
   for (uint32_t i = tid; i <= a.tiles; i += kThreads) below[i] = int32_t(keep);
   const uint32_t lo = a.first, hi = n - a.recent;  // the keys to choose from
@@ -245,112 +254,82 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
 }
 
 template <int VB>
-__global__ __launch_bounds__(kMove) void evict_move_kernel(const EvictArgs a) {
+__global__ __launch_bounds__(kMove, 4) void evict_move_kernel(const EvictArgs a) {
   typedef typename Vec<VB>::T V;
   typedef typename Vec<(VB < 4 ? 4 : VB)>::T Held;  // of it in registers
   __shared__ int64_t s_from[kMaxRows], s_to[kMaxRows];  // byte offsets; -1: does not move
-  __shared__ uint32_t s_tile, s_unit;
+  __shared__ uint32_t s_ticket;
   const uint32_t tid = threadIdx.x;
-  const uint32_t lanes = 2 * a.chunks;               // (plane, chunk) of a unit
-  const uint32_t units = a.batch * a.sets * lanes;
-  // Counter c hands out the tiles of units c, c + counters, ..: one counter for all
-  // took 12 ns a tile, whatever the tiles. A workgroup stays with one while it lasts.
-  const uint32_t counters = min(units, kTickets);
-  uint32_t c = blockIdx.x % counters;
-  auto units_of = [&](uint32_t i) { return (units - i + counters - 1) / counters; };
-  for (;;) {
-    if (tid < 64) {
-      uint32_t t;
-      for (;;) {
-        t = 0;
-        if (tid == 0) t = atomicAdd(&a.tickets[c * kTicketPitch], 1u);
-        t = uint32_t(__builtin_amdgcn_readfirstlane(int(t)));
-        if (t < units_of(c) * a.tiles) break;
-        // the next counter that is not at its end, from this one on
-        const uint32_t i = tid < counters ? (c + tid) % counters : 0;
-        const uint32_t at = __hip_atomic_load(&a.tickets[i * kTicketPitch], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const uint64_t left = __ballot(tid < counters && at < units_of(i) * a.tiles);
-        if (left == 0) {
-          t = 0xffffffffu;
-          break;
-        }
-        c = (c + uint32_t(__builtin_ctzll(left))) % counters;
-      }
-      if (tid == 0) {
-        const uint32_t n = units_of(c), tile = t / n;
-        s_tile = t == 0xffffffffu ? t : tile;
-        s_unit = c + counters * (t - tile * n);
-      }
-    }
-    __syncthreads();
-    const uint32_t tile = uint32_t(__builtin_amdgcn_readfirstlane(int(s_tile)));
-    if (tile == 0xffffffffu) return;
-    const uint32_t rest = uint32_t(__builtin_amdgcn_readfirstlane(int(s_unit))), unit = rest / lanes, lane = rest - unit * lanes;
-    const uint32_t plane = lane & 1, chunk = lane >> 1;
-    const uint32_t b = unit / a.sets, set = unit - b * a.sets, row0 = tile * a.rows;
-    // (loads that do not wait for each other)
-    const uint2 moved = a.moved[unit];
-    const int32_t* below = a.below + int64_t(unit) * (a.tiles + 1) + tile;
-    const int32_t first_below = below[0], past_below = below[1];  // of the list: what lies in this tile's rows
-    const uint32_t* list = a.list + int64_t(unit) * a.most;
-    const int32_t* table = a.tables + int64_t(b) * a.table_stride;
-    for (uint32_t r = tid; r < a.rows; r += kMove) {
-      const uint32_t key = min(row0 + r, a.most - 1), blk = a.block_div.div(key);
-      const uint32_t slot = list[key], page = uint32_t(table[blk]);
-      const bool moves = row0 + r >= moved.x && row0 + r < moved.y && slot != kNoSlot && page < a.num_blocks;
-      const uint32_t from = a.block_div.div(slot);
-      s_from[r] = moves ? int64_t(from) * a.block_stride + int64_t(slot - from * a.block_div.d) * a.token_stride : -1;
-      s_to[r] = int64_t(page) * a.block_stride + int64_t(key - blk * a.block_div.d) * a.token_stride;
-    }
-    __syncthreads();
-    if (max(moved.x, row0) >= min(moved.y, row0 + a.rows)) {
-      if (a.once) return;
-      continue;
-    }
-    const uint32_t first_piece = chunk * a.chunk_pieces, width = min(a.chunk_pieces, a.pieces_row - first_piece);
-    char* const base = (plane ? a.v_base : a.k_base) + int64_t(set) * a.set_bytes + int64_t(first_piece) * VB;
-    Held v[kPieces];
-    // piece u of this thread, of row r; whether it moves
-    auto place = [&](int u, uint32_t& r, uint32_t& piece) __attribute__((always_inline)) {
-      const uint32_t f = tid + kMove * u;
-      r = a.chunk_div.div(f);
-      piece = f - r * a.chunk_pieces;
-      return r < a.rows && piece < width && s_from[r] >= 0;
-    };
+  // all units' first tiles, their second ones, ..
+  const uint32_t lanes = 2 * a.chunks;  // (plane, chunk) of a unit
+  const uint32_t group = a.group0 + blockIdx.x, columns = a.batch * a.sets * lanes;
+  const uint32_t turn = group / columns, column = (group + turn) % columns;  // (its tiles on all XCDs)
+  const uint32_t unit = column / lanes, lane = column - unit * lanes;
+  const uint2 moved = a.moved[unit];
+  if (moved.x >= moved.y) return;
+  const uint32_t first_tile = a.rows_div.div(moved.x);
+  if (turn > a.rows_div.div(moved.y - 1) - first_tile) return;  // the others are as many as the tiles
+  if (tid == 0) s_ticket = atomicAdd(&a.tickets[int64_t(column) * kTicketPitch], 1u);
+  __syncthreads();
+  const uint32_t tile = first_tile + uint32_t(__builtin_amdgcn_readfirstlane(int(s_ticket)));
+  const uint32_t plane = lane & 1, chunk = lane >> 1;
+  const uint32_t b = unit / a.sets, set = unit - b * a.sets, row0 = tile * a.rows;
+  // (loads that do not wait for each other)
+  const int32_t* below = a.below + int64_t(unit) * (a.tiles + 1) + tile;
+  const int32_t first_below = below[0], past_below = below[1];  // of the list: what lies in this tile's rows
+  const uint32_t* list = a.list + int64_t(unit) * a.most;
+  const int32_t* table = a.tables + int64_t(b) * a.table_stride;
+  for (uint32_t r = tid; r < a.rows; r += kMove) {
+    const uint32_t key = min(row0 + r, a.most - 1), blk = a.block_div.div(key);
+    const uint32_t slot = list[key], page = uint32_t(table[blk]);
+    const bool moves = row0 + r >= moved.x && row0 + r < moved.y && slot != kNoSlot && page < a.num_blocks;
+    const uint32_t from = a.block_div.div(slot);
+    s_from[r] = moves ? int64_t(from) * a.block_stride + int64_t(slot - from * a.block_div.d) * a.token_stride : -1;
+    s_to[r] = int64_t(page) * a.block_stride + int64_t(key - blk * a.block_div.d) * a.token_stride;
+  }
+  __syncthreads();
+  const uint32_t first_piece = chunk * a.chunk_pieces, width = min(a.chunk_pieces, a.pieces_row - first_piece);
+  char* const base = (plane ? a.v_base : a.k_base) + int64_t(set) * a.set_bytes + int64_t(first_piece) * VB;
+  Held v[kPieces];
+  // piece u of this thread, of row r; whether it moves
+  auto place = [&](int u, uint32_t& r, uint32_t& piece) __attribute__((always_inline)) {
+    const uint32_t f = tid + kMove * u;
+    r = a.chunk_div.div(f);
+    piece = f - r * a.chunk_pieces;
+    return r < a.rows && piece < width && s_from[r] >= 0;
+  };
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) {
-      uint32_t r, piece;
-      v[u] = Held{};
-      if (place(u, r, piece))
-        v[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(base + s_from[r] + int64_t(piece) * VB));
-    }
-    // the loads have come back (their values are used here), then the flag
+  for (int u = 0; u < kPieces; ++u) {
+    uint32_t r, piece;
+    v[u] = Held{};
+    if (place(u, r, piece))
+      v[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(base + s_from[r] + int64_t(piece) * VB));
+  }
+  // the loads have come back (their values are used here), then the flag
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) asm volatile("" : "+v"(v[u])::"memory");
-    __syncthreads();
-    uint32_t* const flags = a.flags + (int64_t(unit) * lanes + lane) * a.tiles;
-    if (tid == 0) {
-      __hip_atomic_store(&flags[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (past_below > first_below) {
-        const uint32_t last = min(a.rows_div.div(uint32_t(past_below - 1)) + 1, tile);
-        for (uint32_t u = a.rows_div.div(uint32_t(first_below)); u < last; ++u)
-          while (__hip_atomic_load(&flags[u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(2);
-      }
+  for (int u = 0; u < kPieces; ++u) asm volatile("" : "+v"(v[u])::"memory");
+  __syncthreads();
+  uint32_t* const flags = a.flags + (int64_t(unit) * lanes + lane) * a.tiles;
+  if (tid == 0) {
+    __hip_atomic_store(&flags[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (past_below > first_below) {
+      const uint32_t last = min(a.rows_div.div(uint32_t(past_below - 1)) + 1, tile);
+      for (uint32_t u = a.rows_div.div(uint32_t(first_below)); u < last; ++u)
+        while (__hip_atomic_load(&flags[u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(2);
     }
-    __syncthreads();
+  }
+  __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u) {
-      uint32_t r, piece;
-      if (place(u, r, piece)) __builtin_nontemporal_store(V(v[u]), reinterpret_cast<V*>(base + s_to[r] + int64_t(piece) * VB));
-    }
-    if (a.once) return;
+  for (int u = 0; u < kPieces; ++u) {
+    uint32_t r, piece;
+    if (place(u, r, piece)) __builtin_nontemporal_store(V(v[u]), reinterpret_cast<V*>(base + s_to[r] + int64_t(piece) * VB));
   }
 }
 
 struct Plan {
   uint32_t most, rows, tiles, chunks, chunk_pieces;
-  size_t moved, list, below, flags;
-  size_t bytes() const { return moved + list + below + flags + kTickets * kTicketPitch * sizeof(uint32_t); }
+  size_t moved, list, below, flags, tickets;
+  size_t bytes() const { return moved + list + below + flags + tickets; }
 };
 
 size_t padded(size_t n) { return (n + 255) & ~size_t(255); }
@@ -372,6 +351,7 @@ int plan_of(int64_t batch, int64_t sets, int64_t set_bytes, int64_t vec, int64_t
   p->list = padded(units * p->most * sizeof(uint32_t));
   p->below = padded(units * (size_t(p->tiles) + 1) * sizeof(int32_t));
   p->flags = padded(units * 2 * p->chunks * p->tiles * sizeof(uint32_t));
+  p->tickets = units * 2 * p->chunks * kTicketPitch * sizeof(uint32_t);
   return CBK_OK;
 }
 
@@ -424,8 +404,6 @@ int cbk_paged_evict(const cbk_kv_desc* kv, const int32_t* tables_dev, int64_t ta
   if (workspace_dev == nullptr || workspace_bytes < p.bytes())
     return set_error(CBK_ERR_WORKSPACE, "eviction workspace %zu < %zu bytes", workspace_bytes, p.bytes());
   CBK_REQUIRE((reinterpret_cast<uintptr_t>(workspace_dev) & 255) == 0, "workspace must be 256-byte aligned");
-  int cus = 0;
-  if (int rc = device_cus(&cus)) return rc;
   EvictArgs a;
   a.k_base = static_cast<char*>(kv->k_base);
   a.v_base = static_cast<char*>(kv->v_base);
@@ -458,7 +436,7 @@ int cbk_paged_evict(const cbk_kv_desc* kv, const int32_t* tables_dev, int64_t ta
   a.rows_div = FastDiv::make(p.rows);
   char* at = static_cast<char*>(workspace_dev);
   a.tickets = reinterpret_cast<uint32_t*>(at);
-  a.moved = reinterpret_cast<uint2*>(at += kTickets * kTicketPitch * sizeof(uint32_t));
+  a.moved = reinterpret_cast<uint2*>(at += p.tickets);
   a.list = reinterpret_cast<uint32_t*>(at += p.moved);
   a.below = reinterpret_cast<int32_t*>(at += p.list);
   a.flags = reinterpret_cast<uint32_t*>(at + p.below);
@@ -467,17 +445,19 @@ int cbk_paged_evict(const cbk_kv_desc* kv, const int32_t* tables_dev, int64_t ta
   hipLaunchKernelGGL(evict_choose_kernel, dim3(uint32_t(units)), dim3(kThreads), 0, s, a);
   if (int rc = launch_status("eviction's choice")) return rc;
   if (p.tiles == 0) return CBK_OK;
-  const uint64_t all = units * 2 * p.chunks * p.tiles;
-  const dim3 grid(uint32_t(std::min(all, uint64_t(cus) * kGroups)));
-  a.once = all == grid.x;
-  switch (vec) {
-    case 16: hipLaunchKernelGGL((evict_move_kernel<16>), grid, dim3(kMove), 0, s, a); break;
-    case 8: hipLaunchKernelGGL((evict_move_kernel<8>), grid, dim3(kMove), 0, s, a); break;
-    case 4: hipLaunchKernelGGL((evict_move_kernel<4>), grid, dim3(kMove), 0, s, a); break;
-    case 2: hipLaunchKernelGGL((evict_move_kernel<2>), grid, dim3(kMove), 0, s, a); break;
-    default: hipLaunchKernelGGL((evict_move_kernel<1>), grid, dim3(kMove), 0, s, a); break;
+  const uint32_t all = uint32_t(units * 2 * p.chunks * p.tiles);  // < 2^31
+  for (a.group0 = 0; a.group0 < all; a.group0 += kGroups) {
+    const dim3 grid(std::min(all - a.group0, kGroups));
+    switch (vec) {
+      case 16: hipLaunchKernelGGL((evict_move_kernel<16>), grid, dim3(kMove), 0, s, a); break;
+      case 8: hipLaunchKernelGGL((evict_move_kernel<8>), grid, dim3(kMove), 0, s, a); break;
+      case 4: hipLaunchKernelGGL((evict_move_kernel<4>), grid, dim3(kMove), 0, s, a); break;
+      case 2: hipLaunchKernelGGL((evict_move_kernel<2>), grid, dim3(kMove), 0, s, a); break;
+      default: hipLaunchKernelGGL((evict_move_kernel<1>), grid, dim3(kMove), 0, s, a); break;
+    }
+    if (int rc = launch_status("eviction's move")) return rc;
   }
-  return launch_status("eviction's move");
+  return CBK_OK;
 }
 
 }  // extern "C"

@@ -392,3 +392,13 @@ def test_a_decode_loop_with_a_bounded_cache(dtype, shared):
         n = n + 1
         attend(torch.randn(batch, 1, hq, d, generator=g).to(dtype), n)
     assert n.tolist() == [41, 41, 41]
+
+
+def test_more_tiles_than_a_launch_has_workgroups():
+    # 60000 sequences with room for 40 rows of 32 KB, a tile each, in two planes; two move any
+    _check((256, 128), U8, [48] + [0] * 59998 + [47], 40, 3, 2, shared=True, seed=7)
+
+
+def test_long_tables_of_short_sequences():
+    _check((4, 64), BF16, [333, 0, 64, 700, 5] * 20, 60, 4, 8, seed=8, more=900)
+    _check((4, 64), BF16, [333, 0, 64, 700, 5] * 20, [300, 7, 60, 20, 0] * 20, 0, 0, seed=9, more=900, shared=True)
