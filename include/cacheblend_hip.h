@@ -528,8 +528,8 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
  * weights that the rows give it are added, of a KV head's query heads (weight_sets
  * = hkv) or of all (1); in a fixed order, no atomics.
  * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
- * function gives on the current device, max_len = table_width * block_size; with
- * key weights it holds the logits, 4 bytes for each of rows * hq and key of the
+ * function gives on the current device, max_len = table_width * block_size (0 where no
+ * scratch is needed, or where the call refuses the sizes); with key weights it holds the logits, 4 bytes for each of rows * hq and key of the
  * tables.
  */
 size_t cbk_paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,

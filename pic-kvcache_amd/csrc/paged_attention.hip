@@ -140,7 +140,7 @@ int cbk_paged_attention(const void* q_dev, int64_t q_batch_stride, int64_t q_row
                             int64_t(reinterpret_cast<uintptr_t>(kv->v_base)), kv->block_stride, kv->token_stride,
                             int64_t(reinterpret_cast<uintptr_t>(q_dev)), int64_t(reinterpret_cast<uintptr_t>(out_dev))};
   CBK_REQUIRE(common_vec_bytes(words, 6) >= es, "tensors must be aligned to their elements");
-  if (workspace_dev == nullptr || workspace_bytes < p.bytes())
+  if (p.bytes() > 0 && (workspace_dev == nullptr || workspace_bytes < p.bytes()))
     return set_error(CBK_ERR_WORKSPACE, "paged attention workspace %zu < %zu bytes", workspace_bytes, p.bytes());
   CBK_REQUIRE((reinterpret_cast<uintptr_t>(workspace_dev) & 255) == 0, "workspace must be 256-byte aligned");
   PagedAttnArgs a;

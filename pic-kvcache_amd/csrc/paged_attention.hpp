@@ -442,8 +442,7 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
 
     // The logits of the wave's tiles wait in LDS and leave it together: written tile by
     // tile they break up the reads of all memory channels (64 sequences of 4 K to 16 K
-    // keys, 3% of the bytes: 555 us, 400 without them; the
-    // whole call 586, 515 so).
+    // keys, 3% of the bytes: 555 us, 400 without them; the whole call 586, 515 so).
     float* const stage = lds[wave];
     const uint32_t stage_floats = min(head_rows - row_tile * ROWS, uint32_t(ROWS)) * KEYS, stage_room = kLds / stage_floats;
     uint32_t staged = 0;
@@ -821,7 +820,8 @@ __global__ __launch_bounds__(32 * SUBS) void paged_attn_merge_kernel(const Paged
 }
 
 // weights[b, set, k] += the sum of key k's softmax weights over the set's rows. A
-// thread takes 4 keys and every SUBS-th row; the SUBS sums are added in their order.
+// thread takes 4 keys and every SUBS-th row; the SUBS sums are added in their order. Bound by
+// reading the logits, most of them from the last cache level.
 template <int DT, int SUBS>
 __device__ __forceinline__ void key_weights(const PagedAttnArgs& a, uint32_t seq, uint32_t len, uint32_t set, uint32_t chunk,
                                             const float2* stats) {
@@ -928,29 +928,35 @@ int launch_mode(const PagedAttnArgs& a, hipStream_t s) {
 
 template <int DT, int D>
 int launch(const PagedAttnArgs& a, hipStream_t s) {
-  if (int rc = a.rt == 1 ? launch_mode<DT, D, 1>(a, s) : launch_mode<DT, D, 2>(a, s)) return rc;
   const bool weigh = a.weights != nullptr && a.max_len != 0;
-  const uint32_t set_rows = weigh ? a.rows * a.hq / a.w_sets : 0;
-  if (weigh && !a.whole && set_rows <= kJoinRows) {
-    const uint32_t keys = set_rows <= 8 ? 1024 : 256;
-    const dim3 grid(a.rows * a.hq + (a.max_len + keys - 1) / keys * a.w_sets, a.batch);
+  const uint32_t all_rows = a.rows * a.hq, set_rows = weigh ? all_rows / a.w_sets : 0;
+  const bool join = weigh && !a.whole && set_rows <= kJoinRows;
+  // a workgroup's keys: few rows by a thread each, many by several beside each other (us of
+  // the weights alone, bf16: 2 prompts of 8 K, 32 rows of 32 heads together 286 / 11.4 with 1
+  // / 32; 24 sequences of 8 K, one row of 4 heads, 11.7 with one key a thread, 7.1 with 4)
+  const uint32_t keys = set_rows <= 8 ? 1024 : set_rows <= 64 ? 256 : 32;
+  const uint64_t chunks = weigh ? (uint64_t(a.max_len) + keys - 1) / keys : 0;
+  const uint64_t widest = join ? all_rows + chunks * a.w_sets : chunks;
+  CBK_REQUIRE(widest < (1 << 24) && all_rows < (1 << 22), "paged attention: %u rows, key weights of %llu workgroups exceed one launch",
+              all_rows, (unsigned long long)widest);
+  if (int rc = a.rt == 1 ? launch_mode<DT, D, 1>(a, s) : launch_mode<DT, D, 2>(a, s)) return rc;
+  if (join) {
+    const dim3 grid(uint32_t(widest), a.batch);
     if (set_rows <= 8) hipLaunchKernelGGL((join_kernel<DT, D, 1>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((join_kernel<DT, D, 4>), grid, dim3(256), 0, s, a);
     return launch_status("paged attention merge and key weights");
   }
   if (!a.whole) {
-    const dim3 grid(a.rows * a.hq, a.batch);
+    const dim3 grid(all_rows, a.batch);
     if (a.ranges > 16 * a.batch) hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 32>), grid, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL((paged_attn_merge_kernel<DT, D, 8>), grid, dim3(256), 0, s, a);
     if (int rc = launch_status("paged attention merge")) return rc;
   }
   if (!weigh) return CBK_OK;
-  auto run = [&](auto kernel, uint32_t keys) {
-    hipLaunchKernelGGL(kernel, dim3((a.max_len + keys - 1) / keys, a.w_sets, a.batch), dim3(256), 0, s, a);
-  };
-  if (set_rows <= 8) run(key_weights_kernel<DT, 1>, 1024);
-  else if (set_rows <= 64) run(key_weights_kernel<DT, 4>, 256);
-  else run(key_weights_kernel<DT, 32>, 32);
+  const dim3 grid(uint32_t(chunks), a.w_sets, a.batch);
+  if (set_rows <= 8) hipLaunchKernelGGL((key_weights_kernel<DT, 1>), grid, dim3(256), 0, s, a);
+  else if (set_rows <= 64) hipLaunchKernelGGL((key_weights_kernel<DT, 4>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((key_weights_kernel<DT, 32>), grid, dim3(256), 0, s, a);
   return launch_status("key weights");
 }
 

@@ -337,7 +337,7 @@ size_t padded(size_t n) { return (n + 255) & ~size_t(255); }
 // `keep` < 0: lengths of their own. A piece of a row is at least a byte: the
 // counts of tiles and chunks are those of the widest pieces that divide the row.
 int plan_of(int64_t batch, int64_t sets, int64_t set_bytes, int64_t vec, int64_t max_len, int64_t keep, Plan* p) {
-  CBK_REQUIRE(batch >= 0 && sets > 0 && batch * sets < (int64_t(1) << 31), "batch out of range");
+  CBK_REQUIRE(batch >= 0 && sets > 0 && batch < (1 << 22) && batch * sets < (1 << 22), "batch out of range");
   CBK_REQUIRE(max_len >= 0 && max_len < (int64_t(1) << 31), "context out of range");
   const int64_t pieces = set_bytes / vec, room = kMove * kPieces;
   p->most = uint32_t(keep < 0 ? max_len : std::min(keep, max_len));

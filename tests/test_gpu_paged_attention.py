@@ -16,6 +16,7 @@ import numpy as np
 import pytest
 import torch
 
+from cacheblend_vllm import _native
 from cacheblend_vllm import kv_layout as KL
 from cacheblend_vllm.attention import paged_attention
 from oracle import operators as R
@@ -373,3 +374,66 @@ def test_refusals():
     # nothing to do
     assert paged_attention(q[:0], pages, tables[:0], lens[:0], 16, 0.1).shape == (0, 4, 64)
     assert not paged_attention(q, pages, tables[:, :0], torch.tensor([0]), 16, 0.1).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_tables_of_more_than_the_caches_hold(dtype):
+    # room for 600 MB of keys and values, which are then read past the caches; few are there
+    es = 4 if dtype is F32 else 2
+    more = 600_000_000 // (4 * 16 * 2 * 4 * 128 * es)
+    _check(dtype, 8, 4, 128, [700, 33, 0, 290], seed=18, more=more)
+    _check(dtype, 8, 4, 128, [700, 33, 0, 290], rows=2, sets=4, seed=19, more=more)
+    _check(dtype, 8, 8, 64, [700, 33, 0, 290], size=48, sets=1, seed=20, more=more)
+
+
+def test_outputs_in_the_queries_place():
+    g = torch.Generator().manual_seed(21)
+    for lens, rows in (([300, 40], 1), ([9000, 40, 2], 3), ([5000], 33)):  # whole and in ranges
+        n = sum((x + 15) // 16 for x in lens)
+        pages, tables = _pages(g, n, 16, 2, 64, BF16), _tables(g, lens, n, 16, (max(lens) + 15) // 16).to(DEV)
+        q = torch.randn(len(lens), rows, 8, 64, generator=g).to(BF16).to(DEV)
+        want = paged_attention(q, pages, tables, torch.tensor(lens), 16, 0.2)
+        got = paged_attention(q, pages, tables, torch.tensor(lens), 16, 0.2, out=q)
+        assert got is q and torch.equal(q, want)
+
+
+def test_logits_of_minus_infinity_weigh_nothing():
+    # products of -3e38 and 3e38: rows of nothing else are zero, others go by the keys left
+    g = torch.Generator().manual_seed(22)
+    lens = [100, 1000]
+    pages = _pages(g, 70, 16, 1, 64, F32)
+    tables = _tables(g, lens, 70, 16, 63).to(DEV)
+    pages[0] = 0.0
+    pages[0, ..., 0] = -3e38
+    q = torch.zeros(2, 2, 64, device=DEV)
+    q[:, 0, 0] = 3e38
+    weights = torch.zeros(2, 1, 63 * 16, device=DEV)
+    got = paged_attention(q, pages, tables, torch.tensor(lens), 16, 1.0, key_weights=weights)
+    assert not got[:, 0].any() and bool(got[:, 1].any(dim=1).all())
+    for b, n in enumerate(lens):  # the second head's weights: equal
+        assert torch.allclose(weights[b, 0, :n], torch.full((n,), 1.0 / n, device=DEV), rtol=2e-6) and not weights[b, 0, n:].any()
+    # one key with another logit
+    pages[0, tables[1, 30], 5, 0, 0] = 0.0
+    got = paged_attention(q, pages, tables, torch.tensor(lens), 16, 1.0)
+    assert not got[0, 0].any() and torch.equal(got[1, 0], pages[1, tables[1, 30], 5, 0])
+
+
+def test_calls_that_need_no_scratch_take_none():
+    g = torch.Generator().manual_seed(23)
+    pages, lens = _pages(g, 8, 16, 2, 128, BF16), torch.tensor([60, 33], dtype=torch.int32, device=DEV)
+    tables = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4)
+    q = torch.randn(2, 4, 128, generator=g).to(BF16).to(DEV)
+    lib, out = _native.load(), torch.empty_like(q)
+    desc, _, _ = KL.paged_layer(pages, 16)
+    assert lib.cbk_paged_attention_workspace_bytes(2, 1, 4, 2, 128, 64, 1, 0) == 0
+    args = (q.data_ptr(), 512, 512, 128, 2, 1, 4, desc, 2, 128, tables.data_ptr(), 4, 4, lens.data_ptr(), 0.1, 1, out.data_ptr(),
+            512, 512, 128)
+    assert lib.cbk_paged_attention(*args, None, 0, 0, 0, None, 0, _native.stream_handle(DEV)) == _native.CBK_OK
+    assert torch.equal(out, paged_attention(q, pages, tables, lens, 16, 0.1))
+    # with key weights there is some to give
+    need = lib.cbk_paged_attention_workspace_bytes(2, 1, 4, 2, 128, 64, 1, 1)
+    w = torch.zeros(2, 1, 64, device=DEV)
+    assert need > 0
+    for ws, n in ((None, need), (w.data_ptr(), need - 1)):
+        rc = lib.cbk_paged_attention(*args, w.data_ptr(), 64, 64, 1, ws, n, _native.stream_handle(DEV))
+        assert rc == _native.CBK_ERR_WORKSPACE

@@ -110,7 +110,7 @@ def _evict(lib, **over):
     (dict(first=-1), b"first and recent"), (dict(recent=-1), b"first and recent"), (dict(first=1 << 31), b"first and recent"),
     (dict(sets=3), b"3 sets"), (dict(sets=0), b"0 sets"), (dict(width=-1), b"width"), (dict(ts=-1), b"width"),
     (dict(width=1 << 28), b"context"), (dict(batch=-1), b"batch"), (dict(batch=1 << 30), b"batch"),
-    (dict(batch=1 << 24, width=1 << 20, keep=1 << 24), b"too many tiles"), (dict(lens=None), b"NULL"), (dict(new=None), b"NULL"),
+    (dict(batch=1 << 20, width=1 << 20, keep=1 << 24), b"too many tiles"), (dict(batch=1 << 21), b"batch"), (dict(lens=None), b"NULL"), (dict(new=None), b"NULL"),
     (dict(weights=None), b"NULL"), (dict(tables=None), b"NULL"),
 ])
 def test_evict_entry_refuses(over, word):
