@@ -528,12 +528,14 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
  * weights that the rows give it are added, of a KV head's query heads (weight_sets
  * = hkv) or of all (1); in a fixed order, no atomics.
  * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
- * function gives on the current device, max_len = table_width * block_size (0 where no
- * scratch is needed, or where the call refuses the sizes); with key weights it holds the logits, 4 bytes for each of rows * hq and key of the
- * tables.
+ * function gives on the current device, max_len = table_width * block_size,
+ * weight_sets 0 without key weights (0 bytes where no scratch is needed, or where the
+ * call refuses the sizes). For key weights it holds the logits, 4 bytes for each of
+ * rows * hq and key of the tables, unless a set has many rows and keys: then the keys
+ * are multiplied a second time.
  */
 size_t cbk_paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
-                                           int64_t max_len, int32_t dtype, int32_t key_weights);
+                                           int64_t max_len, int32_t dtype, int64_t weight_sets);
 int cbk_paged_attention(const void* q_dev, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
                         int64_t batch, int64_t rows, int64_t hq, const cbk_kv_desc* kv, int64_t hkv, int64_t head_dim,
                         const int32_t* tables_dev, int64_t table_stride, int64_t table_width, const int32_t* lens_dev,

@@ -319,7 +319,8 @@ def paged_attention(
     weights of the rows and of the KV head's query heads give it together;
     ``[batch, 1, keys]``: of all heads. Summed over the steps they say which keys
     matter (``kv_layout.evict_paged_kv``). The call then takes scratch for the logits,
-    4 bytes for each row, query head and key of the tables.
+    4 bytes for each row, query head and key of the tables; in 16 bits not where a set of weights has
+    512 rows (128 a KV head) and many keys, which it multiplies a second time instead.
 
     Lengths on the host are checked, and the tables where both are there
     (``IndexError``). On the device they are not read back: lengths are clamped
@@ -344,7 +345,7 @@ def paged_attention(
         return out
     lib = _native.load()
     code = _native.DTYPE_CODES[query.dtype]
-    nbytes = _paged_workspace_bytes(device, batch, rows, hq, hkv, d, width * block_size, code, int(sets != 0))
+    nbytes = _paged_workspace_bytes(device, batch, rows, hq, hkv, d, width * block_size, code, sets)
     # from torch's allocator on every call: a captured graph then owns its own
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     rc = _native.on_device(

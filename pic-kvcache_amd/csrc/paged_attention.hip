@@ -33,6 +33,14 @@ constexpr int64_t kMostRanges = 64;
 // 91 / 81, 2600 (64 x 16 K) 445 / 397.
 constexpr int64_t kStreamBytes = int64_t(512) << 20;
 
+// Key weights by a second product instead of by logits in scratch: in 16 bits (float32's
+// products take longer), from so many rows of a KV head and of a set on, where workgroups of 64
+// keys of a set fill three quarters of the CUs. us a call, logits / second product, bf16, 128,
+// 32 heads over 8, one set: 1 prompt of 4 K, 32 rows, 38 / 43, of 8 K 43.7 / 46.7, of 16 K 62.8 /
+// 56.1; 24 of 2 K to 8 K 385 / 325, 16 rows 223 / 237; a set for each KV head (128 rows) 8 of
+// 2 K to 8 K, 32 rows, 138 / 168.
+constexpr int64_t kWindowRows = 128, kWindowSetRows = 512;
+
 struct Plan {
   uint32_t rt, row_tiles, ranges, heads, turns, max_tiles;
   bool whole;
@@ -42,7 +50,7 @@ struct Plan {
 
 size_t padded(size_t n) { return (n + 255) & ~size_t(255); }
 
-int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int64_t max_len, int32_t dtype, bool weights,
+int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int64_t max_len, int32_t dtype, int64_t sets,
             Plan* p) {
   CBK_REQUIRE(batch >= 0 && batch < (1 << 16), "batch out of range");
   CBK_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "query heads must be divisible by KV heads");
@@ -87,13 +95,15 @@ int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int
     }
   }
   const size_t all_rows = size_t(rows) * size_t(hq);
-  CBK_REQUIRE(!weights || size_t(most) * size_t(keys) <= (size_t(1) << 44) / all_rows, "logits of %zu rows and %lld tiles are too many",
+  const bool logits = sets > 0 && (dtype == CBK_DTYPE_F32 || n < kWindowRows || rows * hq / sets < kWindowSetRows ||
+                                   batch * sets * (max_len / kWindowKeys) < cus - cus / 4);
+  CBK_REQUIRE(!logits || size_t(most) * size_t(keys) <= (size_t(1) << 44) / all_rows, "logits of %zu rows and %lld tiles are too many",
               all_rows, (long long)most);
   const size_t parts = p->whole ? 0 : size_t(2) * p->ranges * all_rows;
   p->ml = padded(parts * sizeof(float2));
   p->o = padded(parts * size_t(d) * sizeof(float));
-  p->stats = weights ? padded(size_t(batch) * all_rows * sizeof(float2)) : 0;
-  p->logits = weights ? padded(size_t(most) * size_t(keys) * all_rows * sizeof(float)) : 0;
+  p->stats = sets > 0 ? padded(size_t(batch) * all_rows * sizeof(float2)) : 0;
+  p->logits = logits ? padded(size_t(most) * size_t(keys) * all_rows * sizeof(float)) : 0;
   return CBK_OK;
 }
 
@@ -103,10 +113,10 @@ int plan_of(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int
 extern "C" {
 
 size_t cbk_paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
-                                           int64_t max_len, int32_t dtype, int32_t key_weights) {
+                                           int64_t max_len, int32_t dtype, int64_t weight_sets) {
   using namespace cbk;
   Plan p;
-  if (batch <= 0 || head_dim <= 0 || plan_of(batch, rows, hq, hkv, head_dim, max_len, dtype, key_weights != 0, &p)) return 0;
+  if (batch <= 0 || head_dim <= 0 || plan_of(batch, rows, hq, hkv, head_dim, max_len, dtype, weight_sets, &p)) return 0;
   return p.bytes();
 }
 
@@ -133,7 +143,7 @@ int cbk_paged_attention(const void* q_dev, int64_t q_batch_stride, int64_t q_row
               (long long)weight_sets, (long long)hkv);
   const int64_t max_len = table_width * kv->block_size;
   Plan p;
-  if (int rc = plan_of(batch, rows, hq, hkv, head_dim, max_len, dtype, key_weights_dev != nullptr, &p)) return rc;
+  if (int rc = plan_of(batch, rows, hq, hkv, head_dim, max_len, dtype, key_weights_dev ? weight_sets : 0, &p)) return rc;
   if (batch == 0) return CBK_OK;
   CBK_REQUIRE(q_dev && out_dev && lens_dev && (tables_dev || table_width == 0), "NULL pointer");
   const int64_t words[6] = {int64_t(reinterpret_cast<uintptr_t>(kv->k_base)),

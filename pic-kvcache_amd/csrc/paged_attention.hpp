@@ -687,7 +687,7 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
         }
         if (j == 0 && live[t]) {
           if (!whole) a.ml[first_id + row0 + c] = make_float2(m[t], lt);
-          else if (LOGITS) a.stats[first_id + row0 + c] = statistics(m[t], lt);
+          else if (a.stats) a.stats[first_id + row0 + c] = statistics(m[t], lt);
         }
       } else {
         float* mine = lds[wave];
@@ -726,7 +726,7 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
             const float inverse = sum == 0.f ? 0.f : 1.f / sum;
             const float y[4] = {acc[0] * inverse, acc[1] * inverse, acc[2] * inverse, acc[3] * inverse};
             store_row<DT, 4>(to, y);
-            if (LOGITS && dim == 0) a.stats[(int64_t(seq) * a.hkv + h) * head_rows + n] = statistics(top, sum);
+            if (a.stats && dim == 0) a.stats[(int64_t(seq) * a.hkv + h) * head_rows + n] = statistics(top, sum);
           } else {
             const int64_t id = (int64_t(2 * range + which) * a.hkv + h) * head_rows + n;
             *reinterpret_cast<f32x4*>(a.o + id * D + dim) = acc;
@@ -908,6 +908,117 @@ __global__ __launch_bounds__(256) void join_kernel(const PagedAttnArgs a) {
   key_weights<DT, SUBS>(a, seq, len, set, chunk, stats);
 }
 
+// The same for sets and KV heads of many rows, without logits: a second product of the keys with
+// the queries, by the rows' statistics. The waves of a workgroup take its 64 keys and each a
+// part of the set's 16-row tiles, head by head; their sums are added in their order. Bound by
+// reading the rows, 4 KB for 64 keys, through a CU's first cache (32 keys instead: 25 us, 17
+// with 64, for 2 prompts of 8 K, 32 rows of 32 heads over 4; a tile more ahead: 18.5).
+constexpr uint32_t kWindowKeys = 64, kWindowWaves = 8;
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kWindowWaves, 2) void window_weights_kernel(const PagedAttnArgs a) {
+  using T = Type<DT>;
+  constexpr int KP = D * T::ES / 64, G = kWindowKeys / 16;
+  typedef typename Piece<T::ES>::V16 V;
+  __shared__ float s_sum[kWindowWaves][kWindowKeys];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane >> 4, c = lane & 15;
+  const uint32_t seq = blockIdx.z, set = blockIdx.y, key0 = blockIdx.x * kWindowKeys, len = context_of(a, seq);
+  if (key0 >= len) return;
+  const uint32_t head_rows = a.rows * a.group, heads = a.hkv / a.w_sets, head0 = set * heads;
+  const uint32_t tiles = (head_rows + 15) / 16, units = heads * tiles;
+  const uint32_t begin = units / kWindowWaves * wave + min(wave, units % kWindowWaves);
+  const uint32_t end = begin + units / kWindowWaves + (wave < units % kWindowWaves);
+  // the lane's keys, as it reads them: key0 + 16 g + c
+  const int32_t* const table = a.tables + int64_t(seq) * a.table_stride;
+  int64_t row[G];
+  bool held[G];
+  uint64_t here = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const uint32_t key = key0 + 16 * g + c, blk = a.block_div.div(min(key, len - 1)), page = uint32_t(table[blk]);
+    held[g] = key < len && page < a.num_blocks;
+    row[g] = held[g] ? int64_t(page) * a.block_stride + int64_t(key - blk * a.block_div.d) * a.token_stride : 0;
+    here |= (__ballot(held[g]) & 0xffffull) << (16 * g);
+  }
+  const bool masked = here != ~0ull >> (64 - kWindowKeys) || int32_t(key0 + kWindowKeys) > int32_t(len) - int32_t(a.rows) + 1;
+  struct Rows {
+    u32x4 q[KP];
+    float2 st;
+    int32_t last;  // a row sees keys up to it
+  };
+  f32x4 sum[G];  // keys 16 g + 4 j + i, column c's rows
+#pragma unroll
+  for (int g = 0; g < G; ++g) sum[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t u = begin; u < end;) {
+    const uint32_t head = u / tiles, kvh = head0 + head, first = u - head * tiles, past = min(tiles, end - head * tiles);
+    u = head * tiles + past;
+    u32x4 k[G][KP];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const char* p = a.k_base + row[g] + int64_t(kvh) * (D * T::ES) + 16 * j;
+#pragma unroll
+      for (int s = 0; s < KP; ++s) {
+        k[g][s] = u32x4(0u);
+        if (held[g]) k[g][s] = *reinterpret_cast<const V*>(p + 64 * s);
+      }
+    }
+    // row tile t (one past the last: the last again); a lane without a row has the last row's
+    auto rows_of = [&](uint32_t t) __attribute__((always_inline)) {
+      Rows x;
+      const uint32_t n = 16 * min(t, past - 1) + c, row = min(n, head_rows - 1);
+      const uint32_t r = row / a.group, h = kvh * a.group + (row - r * a.group);
+      const char* p = a.q + int64_t(seq) * a.q_batch + int64_t(r) * a.q_row + int64_t(h) * a.q_head + 16 * j;
+#pragma unroll
+      for (int s = 0; s < KP; ++s) x.q[s] = *reinterpret_cast<const V*>(p + 64 * s);
+      x.st = a.stats[(int64_t(seq) * a.hkv + kvh) * head_rows + row];
+      x.last = n < head_rows ? int32_t(len) - int32_t(a.rows) + int32_t(r) : -1;
+      return x;
+    };
+    auto add = [&](uint32_t t, const Rows& now) __attribute__((always_inline)) {
+      const bool some = masked || 16 * t + 16 > head_rows;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KP; ++s) x = T::mma(k[g][s], now.q[s], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= a.c;
+        if (some) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t key = 16 * g + 4 * int32_t(j) + i;
+            if (!((here >> key) & 1u) || int32_t(key0) + key > now.last) x[i] = kNegInf;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sum[g][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[i] - now.st.x, kUnit, T::kWeights)), now.st.y, sum[g][i]);
+      }
+    };
+    Rows x0 = rows_of(first), x1;
+    for (uint32_t t = first;;) {
+      x1 = rows_of(t + 1);
+      add(t, x0);
+      if (++t >= past) break;
+      x0 = rows_of(t + 1);
+      add(t, x1);
+      if (++t >= past) break;
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float all = row16_reduce(sum[g][i], [](float x, float y) { return x + y; });
+      if (c == 0) s_sum[wave][16 * g + 4 * j + i] = all;
+    }
+  __syncthreads();
+  if (threadIdx.x >= min(kWindowKeys, len - key0)) return;
+  float all = s_sum[0][threadIdx.x];
+#pragma unroll
+  for (uint32_t w = 1; w < kWindowWaves; ++w) all += s_sum[w][threadIdx.x];
+  a.weights[int64_t(seq) * a.w_batch + int64_t(set) * a.w_set + key0 + threadIdx.x] += all;
+}
+
 template <int DT, int D, int RT, int MODE>
 int launch_attn(const PagedAttnArgs& a, hipStream_t s) {
   const uint64_t groups = uint64_t(a.hkv / a.heads) * a.row_tiles * ((a.ranges + 7) / 8 * 8);
@@ -930,14 +1041,14 @@ template <int DT, int D>
 int launch(const PagedAttnArgs& a, hipStream_t s) {
   const bool weigh = a.weights != nullptr && a.max_len != 0;
   const uint32_t all_rows = a.rows * a.hq, set_rows = weigh ? all_rows / a.w_sets : 0;
-  const bool join = weigh && !a.whole && set_rows <= kJoinRows;
+  const bool window = weigh && a.logits == nullptr, join = weigh && !window && !a.whole && set_rows <= kJoinRows;
   // a workgroup's keys: few rows by a thread each, many by several beside each other (us of
   // the weights alone, bf16: 2 prompts of 8 K, 32 rows of 32 heads together 286 / 11.4 with 1
   // / 32; 24 sequences of 8 K, one row of 4 heads, 11.7 with one key a thread, 7.1 with 4)
-  const uint32_t keys = set_rows <= 8 ? 1024 : set_rows <= 64 ? 256 : 32;
+  const uint32_t keys = window ? kWindowKeys : set_rows <= 8 ? 1024 : set_rows <= 64 ? 256 : 32;
   const uint64_t chunks = weigh ? (uint64_t(a.max_len) + keys - 1) / keys : 0;
   const uint64_t widest = join ? all_rows + chunks * a.w_sets : chunks;
-  CBK_REQUIRE(widest < (1 << 24) && all_rows < (1 << 22), "paged attention: %u rows, key weights of %llu workgroups exceed one launch",
+  CBK_REQUIRE(widest < (1 << 23) && all_rows < (1 << 22), "paged attention: %u rows, key weights of %llu workgroups exceed one launch",
               all_rows, (unsigned long long)widest);
   if (int rc = a.rt == 1 ? launch_mode<DT, D, 1>(a, s) : launch_mode<DT, D, 2>(a, s)) return rc;
   if (join) {
@@ -954,7 +1065,11 @@ int launch(const PagedAttnArgs& a, hipStream_t s) {
   }
   if (!weigh) return CBK_OK;
   const dim3 grid(uint32_t(chunks), a.w_sets, a.batch);
-  if (set_rows <= 8) hipLaunchKernelGGL((key_weights_kernel<DT, 1>), grid, dim3(256), 0, s, a);
+  if (window) {
+    if constexpr (DT != CBK_DTYPE_F32)
+      hipLaunchKernelGGL((window_weights_kernel<DT, D>), grid, dim3(64 * kWindowWaves), 0, s, a);
+  }
+  else if (set_rows <= 8) hipLaunchKernelGGL((key_weights_kernel<DT, 1>), grid, dim3(256), 0, s, a);
   else if (set_rows <= 64) hipLaunchKernelGGL((key_weights_kernel<DT, 4>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((key_weights_kernel<DT, 32>), grid, dim3(256), 0, s, a);
   return launch_status("key weights");

@@ -437,3 +437,28 @@ def test_calls_that_need_no_scratch_take_none():
     for ws, n in ((None, need), (w.data_ptr(), need - 1)):
         rc = lib.cbk_paged_attention(*args, w.data_ptr(), 64, 64, 1, ws, n, _native.stream_handle(DEV))
         assert rc == _native.CBK_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,hq,hkv,d,sets", [(64, 8, 1, 128, 1), (33, 16, 4, 64, 1), (129, 4, 4, 128, 1), (40, 64, 4, 64, 4)])
+def test_key_weights_of_many_rows(rows, hq, hkv, d, sets, dtype):
+    # with room for many keys without logits in scratch (from 128 rows a KV head and 512 a set on)
+    assert _native.load().cbk_paged_attention_workspace_bytes(6, rows, hq, hkv, d, 160 * 16, 1, sets) < 6 * 2560 * rows * hq * 4
+    for more in (0, 150):
+        _check(dtype, hq, hkv, d, [33, 1, 0, 700, 257, rows], rows=rows, sets=sets, seed=rows + sets, more=more)
+    _check(dtype, hq, hkv, d, [333, 64], size=5, rows=rows, sets=sets, seed=rows, more=1300)
+
+
+def test_key_weights_of_many_rows_where_pages_are_missing():
+    g = torch.Generator().manual_seed(24)
+    pages = _pages(g, 6, 16, 2, 64, BF16)
+    pages[:, 5] = float("nan")  # of keys past the lengths
+    tables = torch.full((3, 300), 5, dtype=torch.int32)
+    tables[:, :4] = torch.tensor([[0, -1, 3, 5], [99, 6, -5, 1], [2, 1 << 30, 4, 5]])
+    lens, rows = [45, 40, 33], 64
+    q = torch.randn(3, rows, 16, 64, generator=g).to(BF16)
+    before = torch.rand(3, 1, 4800, generator=g).to(DEV)
+    weights = before.clone()
+    got = paged_attention(q.to(DEV), pages, tables.to(DEV), torch.tensor(lens, device=DEV), 16, 0.125, key_weights=weights)
+    _compare(q, pages, tables.numpy(), lens, 0.125, got, weights, before)
+    assert torch.equal(weights[1], before[1]) and torch.equal(weights[0, :, 16:32], before[0, :, 16:32])
