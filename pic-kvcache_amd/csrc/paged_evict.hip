@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void evict_choose_kernel(const EvictArgs 
           for (uint32_t u = 0; u < 4; ++u) {
             const uint32_t i = i0 + j + u * kThreads;
             const bool alike = T == 32 || ((key[u] ^ limit) >> (T & 31)) == 0;
-            if (i - lo < past - lo && alike) count_bin(counts, (key[u] >> (T - W)) & ((1u << W) - 1));
+            if (i >= lo && i < past && alike) count_bin(counts, (key[u] >> (T - W)) & ((1u << W) - 1));
           }
         }
       }

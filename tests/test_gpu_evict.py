@@ -402,3 +402,10 @@ def test_more_tiles_than_a_launch_has_workgroups():
 def test_long_tables_of_short_sequences():
     _check((4, 64), BF16, [333, 0, 64, 700, 5] * 20, 60, 4, 8, seed=8, more=900)
     _check((4, 64), BF16, [333, 0, 64, 700, 5] * 20, [300, 7, 60, 20, 0] * 20, 0, 0, seed=9, more=900, shared=True)
+
+
+@pytest.mark.parametrize("first,recent,keep", [(9000, 100, 10000), (100, 9000, 10000), (8192, 8192, 16400), (16500, 0, 16501),
+                                               (0, 16500, 16501), (8191, 1, 8192)])
+def test_ends_longer_than_a_pass_of_the_choice(first, recent, keep):
+    _check((1, 32), BF16, [20000, 17000, keep, keep + 1], keep, first, recent, kind="mass", seed=first)
+    _check((2, 16), BF16, [20000], keep, first, recent, kind="ties", seed=recent, shared=True)
