@@ -911,8 +911,9 @@ __global__ __launch_bounds__(256) void join_kernel(const PagedAttnArgs a) {
 // The same for sets and KV heads of many rows, without logits: a second product of the keys with
 // the queries, by the rows' statistics. The waves of a workgroup take its 64 keys and each a
 // part of the set's 16-row tiles, head by head; their sums are added in their order. Bound by
-// reading the rows, 4 KB for 64 keys, through a CU's first cache (32 keys instead: 25 us, 17
-// with 64, for 2 prompts of 8 K, 32 rows of 32 heads over 4; a tile more ahead: 18.5).
+// dependences at two waves a SIMD (VALU 33% busy, matrix cores 13%): 17 us for 2 prompts of 8 K,
+// 32 rows of 32 heads over 4. With 32 keys a wave 25; rows requested a tile or two ahead 17 and
+// 18.5; four waves a SIMD spill, 28.
 constexpr uint32_t kWindowKeys = 64, kWindowWaves = 8;
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kWindowWaves, 2) void window_weights_kernel(const PagedAttnArgs a) {
@@ -961,10 +962,10 @@ __global__ __launch_bounds__(64 * kWindowWaves, 2) void window_weights_kernel(co
         if (held[g]) k[g][s] = *reinterpret_cast<const V*>(p + 64 * s);
       }
     }
-    // row tile t (one past the last: the last again); a lane without a row has the last row's
+    // row tile t; a lane without a row has the last row's
     auto rows_of = [&](uint32_t t) __attribute__((always_inline)) {
       Rows x;
-      const uint32_t n = 16 * min(t, past - 1) + c, row = min(n, head_rows - 1);
+      const uint32_t n = 16 * t + c, row = min(n, head_rows - 1);
       const uint32_t r = row / a.group, h = kvh * a.group + (row - r * a.group);
       const char* p = a.q + int64_t(seq) * a.q_batch + int64_t(r) * a.q_row + int64_t(h) * a.q_head + 16 * j;
 #pragma unroll
@@ -994,15 +995,7 @@ __global__ __launch_bounds__(64 * kWindowWaves, 2) void window_weights_kernel(co
           sum[g][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[i] - now.st.x, kUnit, T::kWeights)), now.st.y, sum[g][i]);
       }
     };
-    Rows x0 = rows_of(first), x1;
-    for (uint32_t t = first;;) {
-      x1 = rows_of(t + 1);
-      add(t, x0);
-      if (++t >= past) break;
-      x0 = rows_of(t + 1);
-      add(t, x1);
-      if (++t >= past) break;
-    }
+    for (uint32_t t = first; t < past; ++t) add(t, rows_of(t));
   }
 #pragma unroll
   for (int g = 0; g < G; ++g)
