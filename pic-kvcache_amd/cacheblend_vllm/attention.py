@@ -310,8 +310,8 @@ def paged_attention(
     rows, q_heads, head_size]``: the last ``rows`` tokens, each of which sees the
     keys up to its own. Key ``k`` of sequence ``b`` is in page ``block_tables[b, k //
     block_size]``; ``context_lens[b]`` counts the keys, those of ``query``'s tokens
-    among them (append before attending). Head sizes 64 and 128; logits, softmax and
-    sums in float32. For the product with the values the softmax's terms are held to
+    among them (append before attending). Head sizes 64 and 128; ``out`` may be ``query``. Logits,
+    softmax and sums in float32. For the product with the values the softmax's terms are held to
     2^-16 (bf16) or 2^-22 (float16, those below 2^-8 of the largest to 2^-30 of that).
 
     ``key_weights`` ``[batch, kv_heads, keys]``, float32, at least as many keys as the
@@ -330,6 +330,8 @@ def paged_attention(
     """
     _check_tokens(query)
     desc, row, plane = paged_layer(kv_layer, block_size)
+    if key_weights is not None and out is not None and out.data_ptr() == query.data_ptr():
+        query = query.clone()  # the weights may need them after the outputs
     if plane.dtype != query.dtype or len(row) != 2:
         raise ValueError(f"the pages hold {plane.dtype} rows {tuple(row)}, the queries are {query.dtype}")
     hkv, d = row

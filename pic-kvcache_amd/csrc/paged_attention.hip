@@ -153,6 +153,9 @@ int cbk_paged_attention(const void* q_dev, int64_t q_batch_stride, int64_t q_row
   if (p.bytes() > 0 && (workspace_dev == nullptr || workspace_bytes < p.bytes()))
     return set_error(CBK_ERR_WORKSPACE, "paged attention workspace %zu < %zu bytes", workspace_bytes, p.bytes());
   CBK_REQUIRE((reinterpret_cast<uintptr_t>(workspace_dev) & 255) == 0, "workspace must be 256-byte aligned");
+  // (a second product reads the queries after the outputs are written)
+  CBK_REQUIRE(!key_weights_dev || p.logits > 0 || max_len == 0 || q_dev != out_dev,
+              "key weights of these sizes take the queries again: outputs cannot be in their place");
   PagedAttnArgs a;
   a.q = static_cast<const char*>(q_dev);
   a.out = static_cast<char*>(out_dev);

@@ -395,6 +395,22 @@ def test_outputs_in_the_queries_place():
         want = paged_attention(q, pages, tables, torch.tensor(lens), 16, 0.2)
         got = paged_attention(q, pages, tables, torch.tensor(lens), 16, 0.2, out=q)
         assert got is q and torch.equal(q, want)
+    # with key weights, from logits and from a second product of the keys
+    for rows, width in ((1, 20), (64, 800)):
+        pages, tables = _pages(g, 20, 16, 2, 64, BF16), torch.randint(0, 20, (1, width), generator=g).int().to(DEV)
+        q = torch.randn(1, rows, 8, 64, generator=g).to(BF16).to(DEV)
+        pairs = []
+        for out in (None, q):
+            weights = torch.zeros(1, 1, width * 16, device=DEV)
+            pairs.append((paged_attention(q, pages, tables, torch.tensor([300]), 16, 0.2, out=out, key_weights=weights), weights))
+        assert pairs[1][0] is q and torch.equal(pairs[0][0], q) and torch.equal(pairs[0][1], pairs[1][1])
+        # the entry point refuses the latter
+        desc, _, _ = KL.paged_layer(pages, 16)
+        lens, ws = torch.tensor([300], dtype=torch.int32, device=DEV), torch.empty(1 << 26, dtype=torch.uint8, device=DEV)
+        rc = _native.load().cbk_paged_attention(
+            q.data_ptr(), 0, 512, 64, 1, rows, 8, desc, 2, 64, tables.data_ptr(), width, width, lens.data_ptr(), 0.2, 1,
+            q.data_ptr(), 0, 512, 64, weights.data_ptr(), 0, 0, 1, ws.data_ptr(), ws.numel(), _native.stream_handle(DEV))
+        assert rc == (_native.CBK_OK if rows == 1 else _native.CBK_ERR_INVALID)
 
 
 def test_logits_of_minus_infinity_weigh_nothing():
@@ -462,3 +478,27 @@ def test_key_weights_of_many_rows_where_pages_are_missing():
     got = paged_attention(q.to(DEV), pages, tables.to(DEV), torch.tensor(lens, device=DEV), 16, 0.125, key_weights=weights)
     _compare(q, pages, tables.numpy(), lens, 0.125, got, weights, before)
     assert torch.equal(weights[1], before[1]) and torch.equal(weights[0, :, 16:32], before[0, :, 16:32])
+
+
+def test_many_rows_in_graphs():
+    g = torch.Generator().manual_seed(25)
+    pages, tables = _pages(g, 60, 16, 2, 128, BF16), torch.randint(0, 60, (2, 450), generator=g).int().to(DEV)
+    lens = torch.tensor([900, 70], device=DEV, dtype=torch.int32)
+    q = torch.randn(2, 40, 16, 128, generator=g).to(BF16).to(DEV)
+    w0 = torch.rand(2, 1, 7200, generator=g).to(DEV)
+
+    def once():
+        w = w0.clone()
+        return paged_attention(q, pages, tables, lens, 16, 0.09, key_weights=w), w
+
+    once()
+    graph, w = torch.cuda.CUDAGraph(), w0.clone()
+    with torch.cuda.graph(graph):
+        out = paged_attention(q, pages, tables, lens, 16, 0.09, key_weights=w)
+    for n in (900, 33, 0, 5000):
+        lens[0] = n
+        want = once()
+        w.copy_(w0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(w, want[1])
