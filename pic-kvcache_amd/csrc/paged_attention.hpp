@@ -432,13 +432,12 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
 
     float m[RT], l[RT];  // of the lane's column: reference maximum, sum of the lane's keys
     f32x4 o[RT][NT];     // rows 4 j + i of the row tile, column c of tile n: dim NT c + n (float32: 64 (n / 4) + 4 c + n % 4)
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      m[t] = kNegInf;
-      l[t] = 0.f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    // 16 bits: an infinite value's products with a weight's two parts, of which the second
+    // may be negative or 0, have no sum. So where an output is not finite the wave takes its
+    // tiles a second time, such values one by one, by the whole weight. (0.3 us a call for
+    // the look at the outputs; at every tile's values it would be over 100 VALU instructions
+    // beside 250.)
+    bool careful = false;
 
     // The logits of the wave's tiles wait in LDS and leave it together: written tile by
     // tile they break up the reads of all memory channels (64 sequences of 4 K to 16 K
@@ -478,8 +477,8 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
           for (int r = 0; r < 4; ++r) x[t][h][r] = s[r] * a.c;
         }
       // not all keys of the tile, for all rows (uniform)
-      const bool masked = here != kAll || key0 + KEYS > int32_t(len - a.rows + 1);
-      uint32_t odd = 0;  // keys that some rows see and others do not, with an infinity or NaN among their values
+      const bool masked = careful || here != kAll || key0 + KEYS > int32_t(len - a.rows + 1);
+      uint32_t odd = 0;  // keys that some rows see and others do not (careful: any), with an infinity or NaN among their values
       if (masked) {
 #pragma unroll
         for (int t = 0; t < RT; ++t)
@@ -504,7 +503,7 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
               bad |= (tl.v[e][w] & T::kExponent) == T::kExponent ||
                      (tl.v[e][w] & (T::kExponent << 16)) == (T::kExponent << 16);
           }
-          const uint64_t who = __ballot(bad && key0 + key > int32_t(len - a.rows));
+          const uint64_t who = __ballot(bad && (careful || key0 + key > int32_t(len - a.rows)));
 #pragma unroll
           for (int g = 0; g < 4; ++g)
             if (who & (0xffffull << (16 * g))) odd |= 1u << (4 * g + (e & 3) + 16 * (e >> 2));
@@ -560,7 +559,7 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
           }
         }
       }
-      if (odd) {  // rare: infinities and NaN that only some rows see are added one by one
+      if (odd) {  // rare: infinities and NaN that not all rows see, or that have no sum, are added one by one
 #pragma unroll
         for (int e = 0; e < Tl::VK; ++e) {
           const uint32_t mine = odd >> ((e & 3) + 16 * (e >> 2));
@@ -622,29 +621,46 @@ __global__ __launch_bounds__(64 * max_waves(RT), 1) void paged_attn_kernel(const
       }
     };
 
-    if (count > 0) {
-      Tl ta, tb;
-      // a step's table entries are requested before the rows of the step before it:
-      // loads come back in order, and behind the rows they would wait for them
-      Pages pages = fetch(0), more = fetch(1);
-      uint32_t held_a = load(0, pages, ta), held_b;
-      for (int32_t i = 0;;) {
-        pages = more;
-        more = fetch(i + 2);
-        held_b = load(i + 1, pages, tb);
-        if constexpr (FAST) __builtin_amdgcn_sched_barrier(0);
-        compute(i, ta, held_a);
-        if (++i >= count) break;
-        pages = more;
-        more = fetch(i + 2);
-        held_a = load(i + 1, pages, ta);
-        if constexpr (FAST) __builtin_amdgcn_sched_barrier(0);
-        compute(i, tb, held_b);
-        if (++i >= count) break;
+    for (;; careful = true) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        m[t] = kNegInf;
+        l[t] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
+      if (count > 0) {
+        Tl ta, tb;
+        // a step's table entries are requested before the rows of the step before it:
+        // loads come back in order, and behind the rows they would wait for them
+        Pages pages = fetch(0), more = fetch(1);
+        uint32_t held_a = load(0, pages, ta), held_b;
+        for (int32_t i = 0;;) {
+          pages = more;
+          more = fetch(i + 2);
+          held_b = load(i + 1, pages, tb);
+          if constexpr (FAST) __builtin_amdgcn_sched_barrier(0);
+          compute(i, ta, held_a);
+          if (++i >= count) break;
+          pages = more;
+          more = fetch(i + 2);
+          held_a = load(i + 1, pages, ta);
+          if constexpr (FAST) __builtin_amdgcn_sched_barrier(0);
+          compute(i, tb, held_b);
+          if (++i >= count) break;
+        }
+      }
+      if constexpr (LOGITS) flush(count);
+      if (F32 || careful) break;
+      float none = 0.f;  // NaN if an output is infinite or NaN
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) none = fmaf(o[t][n][r], 0.f, none);
+      if (!__any(none != none)) break;
     }
-
-    if constexpr (LOGITS) flush(count);
 
     // The lane's dims of output row r, in their order: (its tiles n one after
     // another, or four by four)

@@ -502,3 +502,46 @@ def test_many_rows_in_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(w, want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,hq,d", [(1, 4, 128), (1, 8, 64), (3, 4, 128), (9, 6, 64), (40, 4, 128)])
+def test_infinities_that_all_rows_see(rows, hq, d, dtype):
+    """An infinite value that has any weight is the row's, of opposite ones there is no sum; other dims notice nothing."""
+    inf, nan = float("inf"), float("nan")
+    for lens, size, sets in (([70], 16, None), ([70, 64], 5, 2), ([600], 16, 1), ([9000, 100], 16, None), ([9000, 100], 16, 2),
+                             ([300] * 40, 48, 2), ([2600] * 3, 16, 1)):
+        g = torch.Generator().manual_seed(rows + d + len(lens))
+        blocks = sum((n + size - 1) // size for n in lens)
+        clean = _pages(g, blocks, size, 2, d, dtype)
+        tables = _tables(g, lens, blocks, size, (max(lens) + size - 1) // size)
+        q = torch.randn(len(lens), rows, hq, d, generator=g).to(dtype).to(DEV)
+
+        def run(pages):
+            w = torch.zeros(len(lens), sets, tables.shape[1] * size, device=DEV) if sets else None
+            return paged_attention(q, pages, tables.to(DEV), torch.tensor(lens), size, 0.1, key_weights=w), w
+
+        want, weights = run(clean)
+        dirty = clean.clone()
+
+        def put(key, head, dim, value):
+            dirty[1, tables[0, key // size], key % size, head, dim] = value
+
+        early = [2, 0, 19, 1, 29, 17, 25]  # keys of the first sequence that every row sees
+        put(early[0], 0, 3, inf)
+        put(early[1], 0, 6, -inf)
+        put(early[2], 0, d - 1, -inf)
+        put(early[3], 1, 8, inf)
+        put(early[4], 1, 8, -inf)
+        put(early[5], 1, 9, nan)
+        put(early[6], 1, 3, inf)
+        put(lens[0] - rows, 1, d - 2, inf)  # the first row's own
+        got, again = run(dirty)
+        half = hq // 2
+        expect = want.clone()
+        expect[0, :, :half, 3], expect[0, :, half:, 3], expect[0, :, half:, d - 2] = inf, inf, inf
+        expect[0, :, :half, 6], expect[0, :, :half, d - 1] = -inf, -inf
+        expect[0, :, half:, 8], expect[0, :, half:, 9] = nan, nan
+        assert torch.equal(got.isnan(), expect.isnan()), (lens, size, sets)
+        assert torch.equal(got.nan_to_num(nan=7.0, posinf=inf, neginf=-inf), expect.nan_to_num(nan=7.0, posinf=inf, neginf=-inf))
+        assert not sets or torch.equal(again, weights)
