@@ -526,7 +526,8 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
  * key_weights_dev (NULL: none) [batch, weight_sets, max_len] float32, strides in
  * elements, contiguous keys: to key k of sequence b, k < lens_dev[b], the softmax
  * weights that the rows give it are added, of a KV head's query heads (weight_sets
- * = hkv) or of all (1); in a fixed order, no atomics.
+ * = hkv) or of all (1); in a fixed order, no atomics. A row without a number gives
+ * NaN to the keys that it sees, to others nothing.
  * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
  * function gives on the current device, max_len = table_width * block_size,
  * weight_sets 0 without key weights (0 bytes where no scratch is needed, or where the

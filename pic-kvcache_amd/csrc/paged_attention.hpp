@@ -851,12 +851,32 @@ __device__ __forceinline__ void key_weights(const PagedAttnArgs& a, uint32_t seq
   float* const to = a.weights + int64_t(seq) * a.w_batch + int64_t(set) * a.w_set + key;
   f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
   if (key < len) {
+    auto add = [](float sum, float y, const float2& st) __attribute__((always_inline)) {
+      return fmaf(__builtin_amdgcn_exp2f(fmaf(y - st.x, kUnit, kWeights)), st.y, sum);
+    };
 #pragma unroll 4
     for (uint32_t n = sub; n < rows; n += SUBS) {
       const float2 st = stats[n];
       const f32x4 y = *reinterpret_cast<const f32x4*>(x + int64_t(n) * KEYS);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(y[e] - st.x, kUnit, kWeights)), st.y, sum[e]);
+      for (int e = 0; e < 4; ++e) sum[e] = add(sum[e], y[e], st);
+    }
+    const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (all != all) {
+      // rare: a row without a number gives NaN to the keys that it sees, and nothing to others
+      // (above 0 times NaN), which their logits of -inf do not tell
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        sum[e] = 0.f;
+        const uint32_t at = min(key + e, len - 1);
+        const bool held = uint32_t(a.tables[int64_t(seq) * a.table_stride + a.block_div.div(at)]) < a.num_blocks;
+        if (!held) continue;
+#pragma unroll 1
+        for (uint32_t n = sub; n < rows; n += SUBS) {
+          const uint32_t r = n % (a.rows * a.group) / a.group;
+          if (int32_t(at) <= int32_t(len) - int32_t(a.rows) + int32_t(r)) sum[e] = add(sum[e], x[int64_t(n) * KEYS + e], stats[n]);
+        }
+      }
     }
   }
   if constexpr (SUBS > 1) {
@@ -999,16 +1019,20 @@ __global__ __launch_bounds__(64 * kWindowWaves, 2) void window_weights_kernel(co
         for (int s = 0; s < KP; ++s) x = T::mma(k[g][s], now.q[s], x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] *= a.c;
-        if (some) {
+        f32x4 y = f32x4{now.st.y, now.st.y, now.st.y, now.st.y};
+        if (some) {  // 0, not 0 times what may be no number
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int32_t key = 16 * g + 4 * int32_t(j) + i;
-            if (!((here >> key) & 1u) || int32_t(key0) + key > now.last) x[i] = kNegInf;
+            if (!((here >> key) & 1u) || int32_t(key0) + key > now.last) {
+              x[i] = kNegInf;
+              y[i] = 0.f;
+            }
           }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          sum[g][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[i] - now.st.x, kUnit, T::kWeights)), now.st.y, sum[g][i]);
+          sum[g][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[i] - now.st.x, kUnit, T::kWeights)), y[i], sum[g][i]);
       }
     };
     for (uint32_t t = first; t < past; ++t) add(t, rows_of(t));

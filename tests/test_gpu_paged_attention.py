@@ -545,3 +545,42 @@ def test_infinities_that_all_rows_see(rows, hq, d, dtype):
         assert torch.equal(got.isnan(), expect.isnan()), (lens, size, sets)
         assert torch.equal(got.nan_to_num(nan=7.0, posinf=inf, neginf=-inf), expect.nan_to_num(nan=7.0, posinf=inf, neginf=-inf))
         assert not sets or torch.equal(again, weights)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,hq,hkv,d,width", [(3, 8, 2, 64, 40), (5, 8, 2, 128, 600), (20, 8, 2, 64, 300), (40, 4, 2, 128, 3),
+                                                 (33, 16, 4, 64, 1300), (150, 8, 1, 128, 1300)])
+def test_rows_without_a_number_weigh_only_what_they_see(rows, hq, hkv, d, width, dtype):
+    """A NaN or an infinity in a query makes its row's weights NaN, those of the keys that the row sees; later keys
+    and pages out of range keep the other rows' sums to the last bit. By logits in scratch, and by a second product."""
+    g = torch.Generator().manual_seed(rows + width)
+    lens = [45, 40, 33, 0]
+    pages = _pages(g, 12, 16, hkv, d, dtype)
+    pages[0, :, ::2, :, 5] = pages[0, :, ::2, :, 5].abs() + 1  # an infinity in a query meets both signs
+    pages[0, :, 1::2, :, 5] = -pages[0, :, 1::2, :, 5].abs() - 1
+    tables = torch.zeros(4, width, dtype=torch.int32)
+    tables[:, :3] = torch.tensor([[0, 6, 3], [4, -1, 5], [7, 1 << 30, 2], [1, 1, 1]])
+    clean = torch.randn(4, rows, hq, d, generator=g).to(dtype)
+    held = [np.array([0 <= int(tables[b, k // 16]) < 12 for k in range(n)], dtype=bool) for b, n in enumerate(lens)]
+    for sets in {1, hkv}:
+        before = torch.rand(4, sets, width * 16, generator=g)
+
+        def run(q):
+            w = before.to(DEV)
+            return paged_attention(q.to(DEV), pages, tables.to(DEV), torch.tensor(lens, device=DEV), 16, 0.1, key_weights=w), w.cpu()
+
+        want, weights = run(clean)
+        for value in (float("nan"), float("inf"), -float("inf")):
+            for b, r, h in ((0, 0, 0), (0, rows - 2, hq - 1), (1, rows - 1, 1), (2, 1, hq - 1)):
+                q = clean.clone()
+                q[b, r, h, 5] = value
+                got, w = run(q)
+                seen = held[b] & (np.arange(lens[b]) <= lens[b] - rows + r)
+                none = torch.zeros_like(weights, dtype=torch.bool)
+                none[b, h // (hq // sets), :lens[b]] = torch.from_numpy(seen)
+                assert torch.equal(w.isnan(), none), (sets, value, b, r, h)
+                assert torch.equal(w[~none], weights[~none])
+                other = torch.ones(4, rows, hq, dtype=torch.bool)
+                other[b, r, h] = False
+                assert torch.equal(got.cpu()[other], want.cpu()[other])
+                assert bool(got[b, r, h].isnan().all()) if seen.any() else not got[b, r, h].any()
