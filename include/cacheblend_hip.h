@@ -133,7 +133,8 @@ int cbk_paged_gather_int4(const cbk_kv_desc* kv, const int64_t* slots_dev, int64
  * order their rows, K and V, move to the front of the sequence's pages, and their
  * weights to the front of theirs; the weights behind them, up to the old length,
  * become 0, rows behind them are left as they are. new_lens_dev[b] =
- * min(length, keep). Ties go to the lower index, NaN is heavier than any number.
+ * min(length, keep), in memory apart from lens_dev and keeps_dev. Ties go to the
+ * lower index, NaN is heavier than any number.
  * weights_dev [batch, sets, table_width * block_size] float32, strides in elements:
  * a set is a KV head's rows (sets = the row's heads), each of which chooses its own keys,
  * or the whole row (1). keep < 0: keeps_dev[b] (at least first + recent).

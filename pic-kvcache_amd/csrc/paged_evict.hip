@@ -361,6 +361,11 @@ int vec_of(const cbk_kv_desc* kv, int64_t set_bytes) {
   return common_vec_bytes(words, 5);
 }
 
+bool apart(const int32_t* x, const int32_t* y, int64_t n) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+  return (a > b ? a - b : b - a) >= uintptr_t(n) * sizeof(int32_t);
+}
+
 int check(const cbk_kv_desc* kv, int64_t sets, int64_t first, int64_t recent, int64_t keep) {
   if (int rc = validate_desc(kv)) return rc;
   CBK_REQUIRE(sets > 0 && kv->row_bytes % sets == 0, "%lld sets of heads do not divide rows of %lld bytes", (long long)sets,
@@ -401,6 +406,9 @@ int cbk_paged_evict(const cbk_kv_desc* kv, const int32_t* tables_dev, int64_t ta
   if (int rc = plan_of(batch, sets, set_bytes, vec, max_len, keep, &p)) return rc;
   if (batch == 0) return CBK_OK;
   CBK_REQUIRE(lens_dev && new_lens_dev && weights_dev && (tables_dev || table_width == 0), "NULL pointer");
+  // (a sequence's sets read its length and keep by themselves, and the first writes the new length)
+  CBK_REQUIRE(apart(new_lens_dev, lens_dev, batch) && (!keeps_dev || apart(new_lens_dev, keeps_dev, batch)),
+              "new lengths over the lengths or keeps");
   if (workspace_dev == nullptr || workspace_bytes < p.bytes())
     return set_error(CBK_ERR_WORKSPACE, "eviction workspace %zu < %zu bytes", workspace_bytes, p.bytes());
   CBK_REQUIRE((reinterpret_cast<uintptr_t>(workspace_dev) & 255) == 0, "workspace must be 256-byte aligned");

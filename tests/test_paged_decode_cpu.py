@@ -130,3 +130,15 @@ def test_evict_workspace():
     # lengths of their own may be as long as the tables; what is refused has no size
     assert lib.cbk_paged_evict_workspace_bytes(_desc(), 4, 2, 2, -1) >= need
     assert lib.cbk_paged_evict_workspace_bytes(_desc(), 4, 2, 3, 20) == 0
+
+
+@pytest.mark.parametrize("over", [dict(new=0x3000), dict(new=0x3004), dict(new=0x2ffc),
+                                  dict(new=0x7000, keep=-1, keeps=0x7000), dict(new=0x7004, keep=-1, keeps=0x7000)])
+def test_new_lengths_over_what_is_still_read(over):
+    """Sets of heads read a sequence's length and keep by themselves, while the first of them writes the new length."""
+    lib = _native.load()
+    assert _evict(lib, **over) == _native.CBK_ERR_INVALID
+    assert b"new lengths" in lib.cbk_last_error(), lib.cbk_last_error()
+    # beside them they are as good as anywhere (the scratch is missing next)
+    for new in (0x3008, 0x2ff8, 0x7008):
+        assert _evict(lib, new=new, keep=-1, keeps=0x7000) == _native.CBK_ERR_WORKSPACE
