@@ -19,7 +19,7 @@ import torch
 
 from . import _native
 from .kv_layout import (KVLayer, check_key_weights, check_tables, device_tables, int4_geometry, paged_layer, rows_apart,
-                        whole_int32)
+                        strides_apart, whole_int32)
 
 
 def blend_attention(
@@ -88,6 +88,21 @@ def _check_out(out: torch.Tensor, query: torch.Tensor) -> None:
         raise ValueError("out rows must hold contiguous dims")
     if not rows_apart(out):
         raise ValueError("out rows must not overlap")
+
+
+def _meets_otherwise(out: torch.Tensor, query: torch.Tensor) -> bool:
+    """Whether an output of ``query``'s shape shares memory with it other than element for element."""
+    if query.numel() == 0:
+        return False
+    shape, strides, o_strides = query.shape, query.stride(), out.stride()
+    apart, es = out.data_ptr() - query.data_ptr(), query.element_size()
+    if apart == 0:
+        return any(n > 1 and a != b for n, a, b in zip(shape, strides, o_strides))
+    if apart >= es * (1 + sum((n - 1) * a for n, a in zip(shape, strides))) or \
+            -apart >= es * (1 + sum((n - 1) * a for n, a in zip(shape, o_strides))):
+        return False
+    # between each other in one tensor
+    return apart % es != 0 or strides != o_strides or not strides_apart((2, *shape), (abs(apart) // es, *strides))
 
 
 def _prompt_ends(ends: torch.Tensor, tokens: int, name: str, device: torch.device) -> torch.Tensor:
@@ -310,8 +325,9 @@ def paged_attention(
     rows, q_heads, head_size]``: the last ``rows`` tokens, each of which sees the
     keys up to its own. Key ``k`` of sequence ``b`` is in page ``block_tables[b, k //
     block_size]``; ``context_lens[b]`` counts the keys, those of ``query``'s tokens
-    among them (append before attending). Head sizes 64 and 128; ``out`` may be ``query``. Logits,
-    softmax and sums in float32. For the product with the values the softmax's terms are held to
+    among them (append before attending). Head sizes 64 and 128. ``out`` may be ``query``; where it
+    shares memory with it otherwise the queries are copied first. Logits, softmax and sums in
+    float32. For the product with the values the softmax's terms are held to
     2^-16 (bf16) or 2^-22 (float16, those below 2^-8 of the largest to 2^-30 of that).
 
     ``key_weights`` ``[batch, kv_heads, keys]``, float32, at least as many keys as the
@@ -330,8 +346,10 @@ def paged_attention(
     """
     _check_tokens(query)
     desc, row, plane = paged_layer(kv_layer, block_size)
-    if key_weights is not None and out is not None and out.data_ptr() == query.data_ptr():
-        query = query.clone()  # the weights may need them after the outputs
+    if out is not None and out.shape == query.shape and out.dtype == query.dtype:
+        # the weights may need the queries after the outputs, and a place another place's after its own
+        if (key_weights is not None and out.data_ptr() == query.data_ptr()) or _meets_otherwise(out, query):
+            query = query.clone()
     if plane.dtype != query.dtype or len(row) != 2:
         raise ValueError(f"the pages hold {plane.dtype} rows {tuple(row)}, the queries are {query.dtype}")
     hkv, d = row

@@ -268,6 +268,10 @@ def rows_apart(t: torch.Tensor) -> bool:
     if len(shape) == 3 and shape[0] > 1 and shape[1] > 1 and strides[1] >= shape[2] \
             and strides[0] >= (shape[1] - 1) * strides[1] + shape[2]:
         return True  # tokens outside heads, as most are
+    return strides_apart(shape, strides)
+
+
+def strides_apart(shape: tuple, strides: tuple) -> bool:
     span = shape[-1]
     for stride, n in sorted(zip(strides[:-1], shape[:-1])):
         if n > 1 and stride < span:

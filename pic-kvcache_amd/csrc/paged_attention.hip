@@ -141,6 +141,10 @@ int cbk_paged_attention(const void* q_dev, int64_t q_batch_stride, int64_t q_row
   CBK_REQUIRE(kv->num_blocks < (int64_t(1) << 31), "num_blocks out of range");
   CBK_REQUIRE(key_weights_dev == nullptr || weight_sets == 1 || weight_sets == hkv, "%lld sets of weights for %lld KV heads",
               (long long)weight_sets, (long long)hkv);
+  CBK_REQUIRE(batch == 0 || q_dev != out_dev ||
+                  ((batch == 1 || q_batch_stride == out_batch_stride) && (rows == 1 || q_row_stride == out_row_stride) &&
+                   (hq == 1 || q_head_stride == out_head_stride)),
+              "outputs in the queries' place need their strides");
   const int64_t max_len = table_width * kv->block_size;
   Plan p;
   if (int rc = plan_of(batch, rows, hq, hkv, head_dim, max_len, dtype, key_weights_dev ? weight_sets : 0, &p)) return rc;

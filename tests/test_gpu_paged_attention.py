@@ -584,3 +584,34 @@ def test_rows_without_a_number_weigh_only_what_they_see(rows, hq, hkv, d, width,
                 other[b, r, h] = False
                 assert torch.equal(got.cpu()[other], want.cpu()[other])
                 assert bool(got[b, r, h].isnan().all()) if seen.any() else not got[b, r, h].any()
+
+
+def test_outputs_over_the_queries_otherwise():
+    """Outputs that share memory with other places' queries: of other strides, or moved by a sequence or a head."""
+    g = torch.Generator().manual_seed(26)
+    batch, hq, d = 1500, 8, 64
+    pages = _pages(g, 50, 16, 2, d, BF16)
+    tables, lens = torch.randint(0, 50, (batch, 3), generator=g).int().to(DEV), torch.full((batch,), 40, device=DEV)
+    whole = torch.randn(batch + 1, hq, d, generator=g).to(BF16)
+
+    def views(room):
+        flat = room.flatten()
+        yield room[:batch], flat[:batch * hq * d].view(hq, batch, d).transpose(0, 1)
+        yield room[:batch], room[1:]
+        yield room[1:], room[:batch]
+        yield room[:batch], flat[d:d + batch * hq * d].view(batch, hq, d)
+        yield room[:batch, None], flat[:batch * hq * d].view(hq, batch, 1, d).permute(1, 2, 0, 3)
+
+    for i in range(5):
+        for weigh in (False, True):
+            q, out = list(views(whole.to(DEV)))[i]
+            want = paged_attention(q, pages, tables, lens, 16, 0.2)
+            w = torch.zeros(batch, 1, 48, device=DEV) if weigh else None
+            got = paged_attention(q, pages, tables, lens, 16, 0.2, out=out, key_weights=w)
+            assert got is out and torch.equal(out, want), (i, weigh)
+    # beside each other in one tensor they share nothing
+    room = torch.randn(batch, 2, hq, d, generator=g).to(BF16).to(DEV)
+    q = room[:, 0].clone()
+    want = paged_attention(q, pages, tables, lens, 16, 0.2)
+    paged_attention(room[:, 0], pages, tables, lens, 16, 0.2, out=room[:, 1])
+    assert torch.equal(room[:, 1], want) and torch.equal(room[:, 0], q)

@@ -142,3 +142,37 @@ def test_new_lengths_over_what_is_still_read(over):
     # beside them they are as good as anywhere (the scratch is missing next)
     for new in (0x3008, 0x2ff8, 0x7008):
         assert _evict(lib, new=new, keep=-1, keeps=0x7000) == _native.CBK_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("over", [dict(ob=1024), dict(oh=192), dict(rows=2, orow=1024)])
+def test_outputs_in_the_queries_place_with_other_strides(over):
+    lib = _native.load()
+    base = dict(weights=None, out=0x1000)
+    assert _attention(lib, **base, **over) == _native.CBK_ERR_INVALID
+    assert b"strides" in lib.cbk_last_error(), lib.cbk_last_error()
+
+
+def test_which_outputs_meet_the_queries():
+    from cacheblend_vllm.attention import _meets_otherwise
+
+    def meets(query, out):
+        """By the addresses of all elements."""
+        mine, its = (torch.arange(4096).as_strided(t.shape, t.stride(), t.storage_offset()) for t in (query, out))
+        return bool(torch.isin(mine, its).any()) and not torch.equal(mine, its)
+
+    room = torch.zeros(4096)
+    a = room[:1024].view(4, 4, 64)
+    sure = [(a, a), (a, room[1024:2048].view(4, 4, 64)), (a, room[:1024].view(4, 4, 64).transpose(0, 1)), (a, room[256:1280].view(4, 4, 64)),
+            (a, room[64:1088].view(4, 4, 64)), (a, room[1:1025].view(4, 4, 64)), (room[256:1280].view(4, 4, 64), a)]
+    both = room.view(8, 2, 4, 64)
+    sure += [(both[:, 0], both[:, 1]), (both[:, 1], both[:, 0]), (both[:4, 0], both[4:, 0]), (both[:7, 1], both[1:, 0])]
+    beside = room.view(8, 4, 128)
+    sure += [(beside[..., :64], beside[..., 64:]), (beside[:, :2], beside[:, 2:]), (beside[:, :3], beside[:, 1:])]
+    for query, out in sure:
+        assert _meets_otherwise(out, query) == meets(query, out), (query.shape, query.stride(), out.stride(), out.storage_offset())
+    # one head or one sequence: its stride does not count
+    one = room[:64].view(1, 1, 64)
+    assert not _meets_otherwise(one.as_strided((1, 1, 64), (7, 9, 1)), one)
+    assert not _meets_otherwise(room[:0].view(0, 4, 64), room[:0].view(0, 4, 64))
+    # memory that is not the same at all
+    assert not _meets_otherwise(torch.zeros(4, 4, 64), a)
