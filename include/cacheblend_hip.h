@@ -139,7 +139,8 @@ int cbk_paged_gather_int4(const cbk_kv_desc* kv, const int64_t* slots_dev, int64
  * a set is a KV head's rows (sets = the row's heads), each of which chooses its own keys,
  * or the whole row (1). keep < 0: keeps_dev[b] (at least first + recent).
  * Rows of a page out of range stay as they are, their weights move. Pages of
- * different sequences, and of one table, must differ (else the rows in them are undefined).
+ * different sequences, and of one table, must differ (else the rows in them are undefined);
+ * keys and values in the same rows are refused.
  * workspace_dev: 256-byte aligned scratch of at least what the _workspace_bytes
  * function gives.
  */

@@ -488,7 +488,8 @@ def evict_paged_kv(
     there start from nothing. Ties go to the lower index, a NaN is heavier than any number.
     ``keep`` may be a tensor with a number for each sequence.
 
-    Any paged layer, rows ``[kv_heads, ...]`` of any type, 4-bit ones among them.
+    Any paged layer, rows ``[kv_heads, ...]`` of any type, 4-bit ones among them; keys and
+    values each in memory of their own (``ValueError``).
     The pages must be the sequences' own (a page that two tables, or one table twice,
     name holds undefined rows afterwards). Lengths, tables and ``keep`` are checked where they
     are on the host (``IndexError``, ``ValueError``); on the device they are not read

@@ -368,6 +368,9 @@ bool apart(const int32_t* x, const int32_t* y, int64_t n) {
 
 int check(const cbk_kv_desc* kv, int64_t sets, int64_t first, int64_t recent, int64_t keep) {
   if (int rc = validate_desc(kv)) return rc;
+  // (a plane's tiles do not wait for the other's)
+  const intptr_t apart = static_cast<const char*>(kv->v_base) - static_cast<const char*>(kv->k_base);
+  CBK_REQUIRE((apart < 0 ? -apart : apart) >= kv->row_bytes, "keys and values in the same rows");
   CBK_REQUIRE(sets > 0 && kv->row_bytes % sets == 0, "%lld sets of heads do not divide rows of %lld bytes", (long long)sets,
               (long long)kv->row_bytes);
   CBK_REQUIRE(kv->num_blocks < (int64_t(1) << 31), "num_blocks out of range");

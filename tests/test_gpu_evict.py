@@ -409,3 +409,11 @@ def test_long_tables_of_short_sequences():
 def test_ends_longer_than_a_pass_of_the_choice(first, recent, keep):
     _check((1, 32), BF16, [20000, 17000, keep, keep + 1], keep, first, recent, kind="mass", seed=first)
     _check((2, 16), BF16, [20000], keep, first, recent, kind="ties", seed=recent, shared=True)
+
+
+def test_keys_and_values_in_one_tensor_are_refused():
+    pages = torch.zeros(4, 16, 2, 64, dtype=BF16, device=DEV)
+    tables, lens, w = torch.arange(4, dtype=torch.int32)[None], torch.tensor([60]), torch.zeros(1, 2, 64, device=DEV)
+    for layer in ((pages, pages), pages.expand(2, 4, 16, 2, 64)):
+        with pytest.raises(ValueError, match="same rows"):
+            KL.evict_paged_kv(layer, tables, lens, 16, w, 8)

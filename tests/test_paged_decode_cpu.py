@@ -176,3 +176,17 @@ def test_which_outputs_meet_the_queries():
     assert not _meets_otherwise(room[:0].view(0, 4, 64), room[:0].view(0, 4, 64))
     # memory that is not the same at all
     assert not _meets_otherwise(torch.zeros(4, 4, 64), a)
+
+
+@pytest.mark.parametrize("apart", [0, 511, -256])
+def test_keys_and_values_in_the_same_rows_do_not_move(apart):
+    """The two planes move by themselves, so that one would write rows that the other has yet to read."""
+    lib = _native.load()
+    kv = _native.KVDesc(0x10000, 0x10000 + apart, 8, 16, 16 * 1024, 1024, 512)
+    assert _evict(lib, kv=kv) == _native.CBK_ERR_INVALID
+    assert b"same rows" in lib.cbk_last_error(), lib.cbk_last_error()
+    assert lib.cbk_paged_evict_workspace_bytes(kv, 4, 2, 2, 20) == 0
+    # beside each other they do (the scratch is missing next)
+    for apart in (512, -512):
+        kv = _native.KVDesc(0x10000, 0x10000 + apart, 8, 16, 16 * 1024, 1024, 512)
+        assert _evict(lib, kv=kv) == _native.CBK_ERR_WORKSPACE
