@@ -536,7 +536,8 @@ int cbk_paged_attention_int4(const void* q_dev, int64_t q_batch_stride, int64_t 
  * call refuses the sizes). For key weights it holds the logits, 4 bytes for each of
  * rows * hq and key of the tables, unless a set has many rows and keys: then the keys
  * are multiplied a second time. out may be q with the same strides, in this last
- * case not, and must not overlap it otherwise.
+ * case not, and must not overlap it otherwise. Scratch and the split of the work go by
+ * the tables' width: best no wider than the longest context.
  */
 size_t cbk_paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
                                            int64_t max_len, int32_t dtype, int64_t weight_sets);

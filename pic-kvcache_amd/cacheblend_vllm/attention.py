@@ -336,7 +336,9 @@ def paged_attention(
     ``[batch, 1, keys]``: of all heads. Summed over the steps they say which keys
     matter (``kv_layout.evict_paged_kv``). The call then takes scratch for the logits,
     4 bytes for each row, query head and key of the tables; in 16 bits not where a set of weights has
-    512 rows (128 a KV head) and many keys, which it multiplies a second time instead.
+    512 rows (128 a KV head) and many keys, which it multiplies a second time instead. Scratch and
+    the split of the work go by the tables' width: best cut to the longest context
+    (``block_tables[:, :n]``).
 
     Lengths on the host are checked, and the tables where both are there
     (``IndexError``). On the device they are not read back: lengths are clamped

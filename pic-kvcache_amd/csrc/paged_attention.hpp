@@ -8,7 +8,8 @@
 // over keys k <= len_b - R + r of sequence b (row r of its R rows is the
 // token at that place), G = Hq / Hkv; a set is a KV head's G heads, or all heads.
 //
-// Bound by HBM: each key and value row is read once for all rows of a group.
+// Bound by HBM: each key and value row is read once for up to 32 rows of a group
+// (more are 32-row tiles, each of which reads it, and bound by their dependences).
 // Beside that the matrix cores and the VALU have little to do (a 32-key tile of
 // a KV head, 16 KB, is 24 MFMAs and some 250 VALU instructions for up to 16
 // rows, a tenth of the time its bytes take), so the kernel is laid out for loads
@@ -947,7 +948,7 @@ __global__ __launch_bounds__(256) void join_kernel(const PagedAttnArgs a) {
 // The same for sets and KV heads of many rows, without logits: a second product of the keys with
 // the queries, by the rows' statistics. The waves of a workgroup take its 64 keys and each a
 // part of the set's 16-row tiles, head by head; their sums are added in their order. Bound by
-// dependences at two waves a SIMD (VALU 33% busy, matrix cores 13%): 17 us for 2 prompts of 8 K,
+// dependences at two waves a SIMD (VALU 34% busy, matrix cores 10%): 17 us for 2 prompts of 8 K,
 // 32 rows of 32 heads over 4. With 32 keys a wave 25; rows requested a tile or two ahead 17 and
 // 18.5; four waves a SIMD spill, 28.
 constexpr uint32_t kWindowKeys = 64, kWindowWaves = 8;

@@ -22,8 +22,8 @@
 // the others that the tables and `keep` have room for end at once.
 // Bound by HBM: the rows behind the first one that leaves are read and written once. A
 // workgroup takes one tile and ends: one that went on to the next waited for its stores
-// before it had its next loads (32 sequences of 2 K to 8 K to 4 K, 8 x 128, bf16, 0.7 GB: the
-// move 217 us, 114 now, 6.2 TB/s). A set's tiles turn through the XCDs, which a column of
+// before it had its next loads (32 sequences of 2 K to 8 K to 4 K, 8 x 128, bf16, 0.56 GB: the
+// move 217 us, 115 now, 4.85 TB/s, as a plain copy). A set's tiles turn through the XCDs, which a column of
 // its own on one leaves unequal work (both kernels there 149 us, 131 turned), and take 68
 // registers, so that 7 fit a SIMD (350 us with 254, to which the compiler unrolls the pieces'
 // addresses). 32 KB a tile: 16 KB and 64 KB take 33.6 us for 4 sequences of 8 K to 2 K, not
