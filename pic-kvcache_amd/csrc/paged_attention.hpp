@@ -865,7 +865,8 @@ __device__ __forceinline__ void key_weights(const PagedAttnArgs& a, uint32_t seq
     const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     if (all != all) {
       // rare: a row without a number gives NaN to the keys that it sees, and nothing to others
-      // (above 0 times NaN), which their logits of -inf do not tell
+      // (above 0 times NaN), which their logits of -inf do not tell. (Marks for hidden keys among the
+      // logits made the waves that write them slower: 24 sequences of 8 K 99.8 us, 107 to 110 with.)
 #pragma unroll
       for (uint32_t e = 0; e < 4; ++e) {
         sum[e] = 0.f;
